@@ -44,6 +44,7 @@ extern "C" {
 #define TL_I32 4
 #define TL_U32 5
 #define TL_I16 6   /* integer row sums only */
+#define TL_U4G 7   /* cache format only: 4-bit codes with a step and a minimum per group of columns */
 
 /* ---- library management ---------------------------------------------------
  * Replaces init()/post() of the generated host (main_template.cpp:14-37).    */
@@ -272,6 +273,61 @@ int tl_b200_mla_decode_paged_noalloc(const void* q, const void* kv_cache, const 
                                      void* out, int64_t batch, int64_t heads, int64_t page_size,
                                      int64_t max_pages_per_seq, int64_t num_pages, float softmax_scale,
                                      int q_dtype, void* stream);
+
+/* ---- quantised key/value cache: write and read back ---------------------------------
+ * Writes rows of a 16-bit type into a paged cache held in fewer bits, and reads them back.  Token t goes to (comes
+ * from) slot slots[t] = page * page_size + position, int64; tokens whose slot lies outside the cache (a negative slot
+ * marks padding) are skipped: neither the cache nor the output row is touched.  Slots that are written must be distinct.
+ *   format TL_U4G: k, v [tokens, heads, dim] with k_stride / v_stride elements from token to token; cache
+ *     [num_pages, heads, page_size, dim/2] bytes, the even column in a byte's low four bits; scale
+ *     [num_pages, heads, page_size, dim/group, 2] of `dtype`: per group of `group` columns the step
+ *     s = rn((max - min) / 15) and the minimum lo; code = clamp(rne((x - lo) / s), 0, 15) (0 where s is 0) with fp32
+ *     arithmetic and IEEE division, value = s * code + lo.  dim 64, 128 or 256; group 32, 64 or 128, at most dim.
+ *     The cache of tl_b200_attn_decode_paged_int4.
+ *   format TL_E4M3: heads 1; k [tokens, dim], cache [num_pages, page_size, dim] e4m3, scale [num_pages, page_size]
+ *     fp32: s = max(amax |x|, 1e-4) / 448, byte = e4m3(x / s), value = s * byte.  dim a multiple of 8, at most 1024;
+ *     `group` is ignored.  The cache of tl_b200_mla_decode_paged.
+ * A group (row) with a NaN or an infinity, or one whose max - min exceeds fp32, reads back as NaN.  v, v_cache, v_scale: the values, in the same launch
+ * (all three NULL: only k).  Rows and caches 16-byte aligned, strides a multiple of 8 elements; dtype TL_BF16 or
+ * TL_F16.  (The reference quantises per token and per block on the host side of its FP8 examples,
+ * examples/deepseek_deepgemm/example_deepgemm_fp8_2xAcc.py:93-112; it has no cache writer.)                       */
+int tl_b200_kv_cache_write(const int64_t* slots, const void* k, void* k_cache, void* k_scale, const void* v, void* v_cache,
+                           void* v_scale, int64_t tokens, int64_t k_stride, int64_t v_stride, int64_t heads, int64_t dim,
+                           int64_t group, int64_t num_pages, int64_t page_size, int format, int dtype, void* stream);
+int tl_b200_kv_cache_read(const int64_t* slots, const void* k_cache, const void* k_scale, void* k, const void* v_cache,
+                          const void* v_scale, void* v, int64_t tokens, int64_t k_stride, int64_t v_stride, int64_t heads,
+                          int64_t dim, int64_t group, int64_t num_pages, int64_t page_size, int format, int dtype, void* stream);
+
+/* ---- attention over a 4-bit paged cache ---------------------------------------------
+ * out[b,i,h,:] = softmax(softmax_scale * q[b,i,h,:] . K^T) V over the first cache_seqlens[b] tokens of sequence b's
+ * page list block_table[b, :]; query token i sees the keys before position len - s_q + i + 1 (as in
+ * tl_b200_mla_decode_paged_gqa); head h reads kv head h / (h_q / h_kv).  K and V are caches of format TL_U4G (above).
+ * q [batch, s_q, h_q, dim] with q_stride_batch / q_stride_token elements between sequences / tokens (heads of a token
+ * contiguous), out dense.  A row that sees no key is zero; lengths are clamped to the table's width, tokens of a page id
+ * outside the cache are masked, and cache rows behind a sequence's last token may hold anything.
+ * `workspace`: tl_b200_attn_decode_paged_int4_workspace_bytes(...) bytes, 16-byte aligned.  Its first
+ * tl_b200_attn_decode_paged_int4_zero_bytes(...) bytes must be zero before the first call and are zero again after each
+ * call; calls that may overlap on the GPU need workspaces of their own.                                            */
+int64_t tl_b200_attn_decode_paged_int4_workspace_bytes(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim);
+int64_t tl_b200_attn_decode_paged_int4_zero_bytes(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim);
+int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache, const void* k_scale, const void* v_cache,
+                                   const void* v_scale, const int32_t* block_table, const int32_t* cache_seqlens, void* out,
+                                   int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim, int64_t group,
+                                   int64_t q_stride_batch, int64_t q_stride_token, int64_t page_size,
+                                   int64_t max_pages_per_seq, int64_t num_pages, float softmax_scale, int dtype,
+                                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- dense GEMM with epilogue -------------------------------------------------------
+ * c = act(a b + bias) + residual, products accumulated and the epilogue evaluated in fp32, one rounding to out_dtype.
+ * a, b, trans_b, in_dtype and out_dtype as in tl_b200_gemm (TL_F32, TL_F16, TL_BF16); bias [n] and residual [m, n] of
+ * in_dtype, either may be NULL; residual may be c itself where out_dtype is in_dtype.                              */
+#define TL_B200_ACT_NONE 0
+#define TL_B200_ACT_RELU 1
+#define TL_B200_ACT_GELU 2        /* x/2 (1 + erf(x / sqrt 2)) */
+#define TL_B200_ACT_GELU_TANH 3   /* x/2 (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) */
+#define TL_B200_ACT_SILU 4        /* x / (1 + exp(-x)) */
+int tl_b200_gemm_epilogue(const void* a, const void* b, const void* bias, const void* residual, void* c, int64_t m, int64_t n,
+                          int64_t k, int trans_b, int act, int in_dtype, int out_dtype, void* stream);
 
 /* ---- fused row-local tile programs ------------------------------------------------
  * Runs a whole `ppl_*` program whose ops all work row by row - ppl_copy (load, store, cast), ppl_fill,

@@ -312,3 +312,67 @@ def mla_decode_paged_gqa(q: torch.Tensor, kv_pages: torch.Tensor, block_table: t
         w = torch.nan_to_num(w)                        # a query token that sees no key at all gives zeros
         out[i] = (w @ k[..., :dv]).transpose(0, 1).to(q.dtype)
     return out
+
+
+# ------------------------------------------------------------------ quantised cache, attention over it, GEMM with epilogue
+# No reference program exists for these three; the formulas are the definitions in include/tl_b200.h, in 64 bits except
+# where the format itself fixes fp32 or 16-bit roundings (the codes, the steps).
+def quantise_u4g(x: torch.Tensor, group: int):
+    """(..., D) -> codes (..., D/2) uint8 and scale (..., D/group, 2) of x's dtype; fp32 arithmetic as the format says."""
+    xf = x.float().unflatten(-1, (x.shape[-1] // group, group))
+    lo, hi = xf.amin(-1, keepdim=True), xf.amax(-1, keepdim=True)
+    step = ((hi - lo) / torch.full_like(lo, 15.0)).to(x.dtype).float()
+    code = torch.where(step > 0, torch.round((xf - lo) / step), torch.zeros_like(xf)).nan_to_num(0.0).clamp(0, 15).to(torch.uint8).flatten(-2)
+    return code[..., 0::2] | (code[..., 1::2] << 4), torch.cat((step, lo), -1).to(x.dtype)
+
+
+def values_u4g(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """Values of 4-bit rows, in 64 bits."""
+    c = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).double()
+    sc = scale.double()
+    c = c.unflatten(-1, (scale.shape[-2], c.shape[-1] // scale.shape[-2]))
+    return (c * sc[..., :1] + sc[..., 1:]).flatten(-2)
+
+
+def quantise_row_e4m3(x: torch.Tensor):
+    """(..., D) -> e4m3 bytes and one fp32 scale per row."""
+    xf = x.float()
+    s = xf.abs().amax(-1).clamp(min=1e-4)
+    s = s / torch.full_like(s, 448.0)
+    return (xf / s[..., None]).to(torch.float8_e4m3fn), s
+
+
+def attn_decode_paged_u4g(q, k_cache, k_scale, v_cache, v_scale, block_table, cache_seqlens, scale):
+    """(B, s_q, h_q, D) in 64 bits; a page id outside the cache masks its tokens."""
+    b, s_q, h_q, d = q.shape
+    pages, h_kv, page, _ = k_cache.shape
+    per = h_q // h_kv
+    out = torch.zeros(b, s_q, h_q, d, dtype=torch.float64)
+    for i in range(b):
+        n = max(0, min(int(cache_seqlens[i]), block_table.shape[1] * page))
+        at = torch.arange(n)
+        pg = block_table[i].long()[at // page] if n else at
+        ok = (pg >= 0) & (pg < pages)
+        pg = pg.clamp(0, max(pages - 1, 0))
+        for h in range(h_kv):
+            k = values_u4g(k_cache[pg, h, at % page], k_scale[pg, h, at % page])
+            v = values_u4g(v_cache[pg, h, at % page], v_scale[pg, h, at % page])
+            for t in range(s_q):
+                see = ok & (at < n - s_q + t + 1)
+                if see.any():
+                    w = torch.softmax(q[i, t, h * per:(h + 1) * per].double() @ k[see].t() * scale, -1)
+                    out[i, t, h * per:(h + 1) * per] = w @ v[see]
+    return out
+
+
+def gemm_epilogue(a, b, bias=None, activation=None, residual=None, transpose_b=False):
+    x = a.double() @ (b.double().t() if transpose_b else b.double())
+    if bias is not None:
+        x = x + bias.double()
+    if activation == "relu":
+        x = x.clamp_min(0)
+    elif activation == "silu":
+        x = x * torch.sigmoid(x)
+    elif activation in ("gelu", "gelu_tanh"):
+        x = torch.nn.functional.gelu(x, approximate="tanh" if activation == "gelu_tanh" else "none")
+    return x if residual is None else x + residual.double()

@@ -15,7 +15,7 @@ from pathlib import Path
 _PKG_ROOT = Path(__file__).resolve().parent.parent
 DEFAULT_LIB = _PKG_ROOT / "lib" / "libtl_b200.so"
 
-TL_F32, TL_F16, TL_BF16, TL_E4M3, TL_I32, TL_U32, TL_I16 = range(7)
+TL_F32, TL_F16, TL_BF16, TL_E4M3, TL_I32, TL_U32, TL_I16, TL_U4G = range(8)
 ABI_VERSION = 100          # TL_B200_VERSION of include/tl_b200.h
 
 # name -> (restype, argtypes).  Kept in declaration order of include/tl_b200.h.
@@ -55,6 +55,12 @@ PROTOTYPES = {
     "tl_b200_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_void_p]),
     "tl_b200_gemm_tiled": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     "tl_b200_mlp_gate_up": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]),
+    "tl_b200_kv_cache_write": (c_int, [c_void_p] * 7 + [c_int64] * 8 + [c_int, c_int, c_void_p]),
+    "tl_b200_kv_cache_read": (c_int, [c_void_p] * 7 + [c_int64] * 8 + [c_int, c_int, c_void_p]),
+    "tl_b200_attn_decode_paged_int4_workspace_bytes": (c_int64, [c_int64] * 5),
+    "tl_b200_attn_decode_paged_int4_zero_bytes": (c_int64, [c_int64] * 5),
+    "tl_b200_attn_decode_paged_int4": (c_int, [c_void_p] * 8 + [c_int64] * 11 + [c_float, c_int, c_void_p, c_int64, c_void_p]),
+    "tl_b200_gemm_epilogue": (c_int, [c_void_p] * 5 + [c_int64] * 3 + [c_int] * 4 + [c_void_p]),
     "tl_b200_tile_program_registers": (c_int, [c_int64]),
     "tl_b200_tile_program": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int64, c_void_p]),
     "tl_b200_run": (c_int, [c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64), c_void_p]),

@@ -471,3 +471,178 @@ def mla_decode_paged(q: torch.Tensor, kv_cache: torch.Tensor, kv_scale: torch.Te
                                                block_table.shape[1], num_pages, float(softmax_scale),
                                                dtype_code(q.dtype), dtype_code(kv_cache.dtype), _ptr(ws), ws_bytes, s),
                    "tl_b200_mla_decode_paged")
+
+
+def _rows(t: torch.Tensor, rows_shape, dtype, what: str) -> int:
+    """Elements from one token to the next of a (tokens, ...) tensor whose rows are dense."""
+    if tuple(t.shape[1:]) != tuple(rows_shape) or t.dtype != dtype:
+        raise ValueError(f"{what} must be (tokens, {', '.join(map(str, rows_shape))}) {dtype}, not {tuple(t.shape)} {t.dtype}")
+    if t.numel() and not t[:1].is_contiguous():
+        raise ValueError(f"{what}: the columns of a token must be contiguous")
+    dense = 1
+    for n in rows_shape:
+        dense *= n
+    return t.stride(0) if t.shape[0] > 1 else dense
+
+
+def _cache_call(fn: str, slots, k, k_cache, k_scale, v, v_cache, v_scale) -> int:
+    given = [x is not None for x in (v, v_cache, v_scale)]
+    if any(given) and not all(given):
+        raise ValueError(f"{fn}: v, v_cache and v_scale go together")
+    if slots.dtype != torch.int64 or slots.dim() != 1:
+        raise ValueError(f"{fn}: slots must be (tokens,) int64")
+    tokens = slots.shape[0]
+    sides = [("k", k, k_cache, k_scale)] + ([("v", v, v_cache, v_scale)] if given[0] else [])
+    if any(x.shape[:1] != slots.shape for _, x, _, _ in sides):
+        raise ValueError(f"{fn}: one slot per row")
+    dtype = k.dtype
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{fn}: rows must be bfloat16 or float16, not {dtype}")
+    strides = []
+    if k_cache.dtype == torch.uint8:
+        if k_cache.dim() != 4 or k_scale.dim() != 5:
+            raise ValueError(f"{fn}: a 4-bit cache is (num_pages, heads, page, dim / 2) uint8 with a scale (num_pages, heads, page, groups, 2)")
+        num_pages, heads, page, half = k_cache.shape
+        dim, groups = 2 * half, k_scale.shape[3]
+        if groups < 1 or dim % groups:
+            raise ValueError(f"{fn}: {groups} groups do not divide {dim} columns")
+        group, fmt = dim // groups, N.TL_U4G
+        for name, x, cache, scale in sides:
+            if cache.dtype != torch.uint8 or cache.shape != k_cache.shape or tuple(scale.shape) != (num_pages, heads, page, groups, 2) \
+                    or scale.dtype != dtype:
+                raise ValueError(f"{fn}: {name}_cache must be {tuple(k_cache.shape)} uint8 and {name}_scale "
+                                 f"{(num_pages, heads, page, groups, 2)} {dtype}")
+            strides.append(_rows(x, (heads, dim), dtype, f"{fn}: {name}"))
+    elif k_cache.dtype == torch.float8_e4m3fn:
+        if k_cache.dim() == 4 and k_cache.shape[2] != 1 or k_cache.dim() not in (3, 4):
+            raise ValueError(f"{fn}: an e4m3 cache is (num_pages, page, dim) or (num_pages, page, 1, dim)")
+        num_pages, page, dim = k_cache.shape[0], k_cache.shape[1], k_cache.shape[-1]
+        heads, group, fmt = 1, dim, N.TL_E4M3
+        for name, x, cache, scale in sides:
+            if cache.dtype != torch.float8_e4m3fn or cache.shape != k_cache.shape or scale.dtype != torch.float32 \
+                    or tuple(scale.shape) != (num_pages, page):
+                raise ValueError(f"{fn}: {name}_cache must be {tuple(k_cache.shape)} e4m3 and {name}_scale ({num_pages}, {page}) float32")
+            if x.dim() == 3 and x.shape[1] == 1:
+                strides.append(_rows(x, (1, dim), dtype, f"{fn}: {name}"))
+            else:
+                strides.append(_rows(x, (dim,), dtype, f"{fn}: {name}"))
+    else:
+        raise ValueError(f"{fn}: the cache must be uint8 (4-bit codes) or float8_e4m3fn, not {k_cache.dtype}")
+    if len(strides) == 1:
+        strides.append(0)
+    s = _prepare(slots, k_cache, k_scale, v_cache, v_scale, k[:1], v[:1] if v is not None else None)
+    lib = N.load()
+    if fn == "kv_cache_write":
+        rc = lib.tl_b200_kv_cache_write(_ptr(slots), _ptr(k), _ptr(k_cache), _ptr(k_scale), _ptr(v), _ptr(v_cache), _ptr(v_scale), tokens,
+                                        strides[0], strides[1], heads, dim, group, num_pages, page, fmt, dtype_code(dtype), s)
+    else:
+        rc = lib.tl_b200_kv_cache_read(_ptr(slots), _ptr(k_cache), _ptr(k_scale), _ptr(k), _ptr(v_cache), _ptr(v_scale), _ptr(v), tokens,
+                                       strides[0], strides[1], heads, dim, group, num_pages, page, fmt, dtype_code(dtype), s)
+    return N.check(rc, "tl_b200_" + fn)
+
+
+def kv_cache_write(slots: torch.Tensor, k: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor, v: torch.Tensor | None = None,
+                   v_cache: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> int:
+    """Quantise rows into a paged cache: token t goes to slot slots[t] = page * page_size + position (int64, distinct;
+    a slot outside the cache, such as -1 for padding, is skipped).
+
+    4-bit cache (the one attn_decode_paged_int4 reads): k, v (tokens, heads, dim); cache (num_pages, heads, page, dim / 2)
+    uint8; scale (num_pages, heads, page, groups, 2) of k's dtype, a step and a minimum per group of dim / groups columns
+    (32, 64 or 128; dim 64, 128 or 256).  e4m3 cache (the one mla_decode_paged reads): k (tokens, dim); cache
+    (num_pages, page, dim) e4m3; scale (num_pages, page) float32.  k and v may be slices of a wider projection: only the
+    columns of a token have to be contiguous.  Keys and values go in one launch when both are given."""
+    return _cache_call("kv_cache_write", slots, k, k_cache, k_scale, v, v_cache, v_scale)
+
+
+def kv_cache_read(slots: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor, k: torch.Tensor, v_cache: torch.Tensor | None = None,
+                  v_scale: torch.Tensor | None = None, v: torch.Tensor | None = None) -> int:
+    """Read rows of a quantised cache back in 16 bits: k[t] = value of slot slots[t]; layouts as in kv_cache_write.  Rows
+    whose slot lies outside the cache are left as they are; a slot may be named more than once."""
+    return _cache_call("kv_cache_read", slots, k, k_cache, k_scale, v, v_cache, v_scale)
+
+
+_int4_workspaces: dict = {}
+
+
+def _int4_workspace(device: torch.device, nbytes: int, zero_bytes: int) -> torch.Tensor:
+    """Scratch of attn_decode_paged_int4, kept apart from the other operators': its counters have to be zero between calls.
+    One buffer per (device, stream), as in _workspace; a call that is being captured gets one of its own from the graph's
+    pool, so that two graphs never share counters, however their replays overlap."""
+    if torch.cuda.is_current_stream_capturing():
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        buf[:zero_bytes].zero_()
+        return buf
+    key = (device, torch.cuda.current_stream(device).cuda_stream)
+    buf = _int4_workspaces.get(key)
+    if buf is None or buf.numel() < nbytes:
+        buf = _int4_workspaces[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return buf
+
+
+def attn_decode_paged_int4(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor, v_cache: torch.Tensor, v_scale: torch.Tensor,
+                           block_table: torch.Tensor, cache_seqlens: torch.Tensor, out: torch.Tensor,
+                           softmax_scale: float | None = None) -> int:
+    """Attention of s_q new tokens per sequence over a paged 4-bit cache (written by kv_cache_write): q (B, s_q, h_q, D) with
+    the heads of a token contiguous, caches (num_pages, h_kv, page, D / 2) uint8 with scales
+    (num_pages, h_kv, page, groups, 2) of q's dtype, block_table (B, max_pages) int32, cache_seqlens (B,) int32 (the new
+    tokens included), out (B, s_q, h_q, D).  Query token i sees the keys before len - s_q + i + 1; a row that sees none
+    is zero.  D 64, 128 or 256."""
+    if q.dim() != 4 or out.shape != q.shape or out.dtype != q.dtype or q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("attn_decode_paged_int4: q and out must be (B, s_q, h_q, D) bfloat16 or float16")
+    b, s_q, h_q, d = q.shape
+    if k_cache.dim() != 4 or k_cache.dtype != torch.uint8 or k_cache.shape[3] * 2 != d or v_cache.shape != k_cache.shape \
+            or v_cache.dtype != torch.uint8:
+        raise ValueError("attn_decode_paged_int4: caches must be (num_pages, h_kv, page, D / 2) uint8")
+    num_pages, h_kv, page, _ = k_cache.shape
+    if k_scale.dim() != 5 or tuple(k_scale.shape[:3]) != (num_pages, h_kv, page) or k_scale.shape[4] != 2 or k_scale.shape[3] < 1 \
+            or d % k_scale.shape[3] or v_scale.shape != k_scale.shape or k_scale.dtype != q.dtype or v_scale.dtype != q.dtype:
+        raise ValueError("attn_decode_paged_int4: scales must be (num_pages, h_kv, page, groups, 2) of q's dtype")
+    if h_kv < 1 or h_q % h_kv:
+        raise ValueError("attn_decode_paged_int4: h_q must be a multiple of h_kv")
+    if block_table.dtype != torch.int32 or cache_seqlens.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != b \
+            or cache_seqlens.numel() != b:
+        raise ValueError("attn_decode_paged_int4: block_table (B, max_pages) and cache_seqlens (B,) must be int32")
+    if q.numel() and not q[:1, :1].is_contiguous():
+        raise ValueError("attn_decode_paged_int4: the heads of a token must be contiguous")
+    if softmax_scale is None:
+        softmax_scale = d ** -0.5
+    s = _prepare(k_cache, k_scale, v_cache, v_scale, block_table, cache_seqlens, out, q[:1, :1])
+    lib = N.load()
+    nbytes = int(lib.tl_b200_attn_decode_paged_int4_workspace_bytes(b, s_q, h_q, h_kv, d))
+    zero = int(lib.tl_b200_attn_decode_paged_int4_zero_bytes(b, s_q, h_q, h_kv, d))
+    ws = _int4_workspace(q.device, nbytes, zero)
+    return N.check(lib.tl_b200_attn_decode_paged_int4(
+        _ptr(q), _ptr(k_cache), _ptr(k_scale), _ptr(v_cache), _ptr(v_scale), _ptr(block_table), _ptr(cache_seqlens), _ptr(out), b, s_q, h_q,
+        h_kv, d, d // k_scale.shape[3], q.stride(0) if b > 1 else 0, q.stride(1) if s_q > 1 else 0, page, block_table.shape[1], num_pages,
+        float(softmax_scale), dtype_code(q.dtype), _ptr(ws), nbytes, s), "tl_b200_attn_decode_paged_int4")
+
+
+_ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def gemm_epilogue(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+                  residual: torch.Tensor | None = None, transpose_b: bool = False) -> int:
+    """c = act(a @ b + bias) + residual (b is (K, N)), or with b.T (b is (N, K), transpose_b=True); fp32 accumulation and
+    epilogue, one rounding.  bias (N,) and residual (M, N) share a's dtype, c has it or float32; residual may be c itself.
+    activation: None, "relu", "gelu" (erf), "gelu_tanh" or "silu"."""
+    if a.dim() != 2 or b.dim() != 2 or c.dim() != 2:
+        raise ValueError("gemm_epilogue: a, b, c must be 2-D")
+    m, k = a.shape
+    n, kb = (b.shape[0], b.shape[1]) if transpose_b else (b.shape[1], b.shape[0])
+    if kb != k:
+        raise ValueError("gemm K shape check failed")          # message of ppl_gemm's assert
+    if tuple(c.shape) != (m, n):
+        raise ValueError(f"gemm_epilogue: c must be ({m}, {n})")
+    if a.dtype not in (torch.float16, torch.bfloat16, torch.float32) or b.dtype != a.dtype or c.dtype not in (a.dtype, torch.float32):
+        raise ValueError("gemm_epilogue: a and b must share float16, bfloat16 or float32; c has that dtype or float32")
+    if bias is not None and (bias.numel() != n or bias.dtype != a.dtype):
+        raise ValueError(f"gemm_epilogue: bias must hold {n} elements of a's dtype")
+    if residual is not None and (residual.shape != c.shape or residual.dtype != a.dtype):
+        raise ValueError(f"gemm_epilogue: residual must be ({m}, {n}) of a's dtype")
+    try:
+        act = _ACTIVATIONS[activation]
+    except (KeyError, TypeError):
+        raise ValueError(f"gemm_epilogue: unknown activation {activation!r}") from None
+    s = _prepare(a, b, c, bias, residual)
+    return N.check(N.load().tl_b200_gemm_epilogue(_ptr(a), _ptr(b), _ptr(bias), _ptr(residual), _ptr(c), m, n, k, 1 if transpose_b else 0, act,
+                                                 dtype_code(a.dtype), dtype_code(c.dtype), s), "tl_b200_gemm_epilogue")
