@@ -305,11 +305,11 @@ int tl_b200_kv_cache_read(const int64_t* slots, const void* k_cache, const void*
  * q [batch, s_q, h_q, dim] with q_stride_batch / q_stride_token elements between sequences / tokens (heads of a token
  * contiguous), out dense.  A row that sees no key is zero; lengths are clamped to the table's width, tokens of a page id
  * outside the cache are masked, and cache rows behind a sequence's last token may hold anything.
- * `workspace`: tl_b200_attn_decode_paged_int4_workspace_bytes(...) bytes, 16-byte aligned.  Its first
- * tl_b200_attn_decode_paged_int4_zero_bytes(...) bytes must be zero before the first call and are zero again after each
- * call; calls that may overlap on the GPU need workspaces of their own.                                            */
+ * `workspace`: tl_b200_attn_decode_paged_int4_workspace_bytes(...) bytes (0 for sizes the call refuses), 16-byte aligned.
+ * Its first TL_B200_ATTN_INT4_ZERO_BYTES bytes must be zero before the first call and are zero again after each call,
+ * whatever the sizes of the calls; calls that may overlap on the GPU need workspaces of their own.                 */
+#define TL_B200_ATTN_INT4_ZERO_BYTES 4096
 int64_t tl_b200_attn_decode_paged_int4_workspace_bytes(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim);
-int64_t tl_b200_attn_decode_paged_int4_zero_bytes(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim);
 int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache, const void* k_scale, const void* v_cache,
                                    const void* v_scale, const int32_t* block_table, const int32_t* cache_seqlens, void* out,
                                    int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim, int64_t group,

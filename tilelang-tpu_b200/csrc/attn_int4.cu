@@ -1,9 +1,29 @@
-// Attention over a paged cache held in 4 bits (TL_U4G, see kv_cache.cu), grouped query heads, s_q query tokens a sequence.
+// Attention over a paged cache held in 4 bits (TL_U4G, see kv_cache.cu): grouped query heads, s_q query tokens a sequence.
 //
 //   out[b,i,h] = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale * q[b,i,h] . k_t),  t < len_b - s_q + i + 1,
-//   k_t = s c + lo per group (likewise v_t); a row that sees no key is zero.
+//   k_t = s c + lo per group of columns (likewise v_t); a row that sees no key is zero.
 //
-// One warp per (sequence, query token, head): lanes share the columns, keys one after the other with a running maximum.
+// What bounds it.  A key of one kv head is dim/2 + 4 groups bytes, twice with its value (136 bytes at dim 128 and one
+// group), against 4 dim flop for each of the few query heads that share it: HBM, if the codes can be widened fast enough.
+// At the measured copy rate an SM receives 43 codes a clock, so every instruction spent on eight codes counts; a score
+// costs next to nothing beside that.
+//
+// Layout.  The MMAs are the warp-level m16n8k16 ones: at most 8 or 16 query rows share a key, so a 128-row tensor-memory
+// tile would be 90% padding, and codes have to pass through registers to be widened anyway.  Keys (and columns of V) are
+// the 16 rows, queries the 8 columns:  S^T = K Q^T  and  O^T = V^T P^T.  Widening folds into the operand layouts:
+//   * K: a lane holds whole 32-bit words of a key; (word >> 4i) & 0x000f000f are columns i and i + 4 of the word, one
+//     register of the A operand.  The columns of Q are permuted likewise when they are loaded, once a sequence.
+//   * V: a register of the A operand is one column of two neighbouring tokens: one byte permute joins half words of the two
+//     before they are widened.
+//   * Steps and minima never touch the codes:  q . k = s (q . c) + lo sum(q) per group, and the value's step multiplies p
+//     (held in fp16 with a power-of-two factor per warp that keeps p s in range), its minimum adds p lo in fp32.
+// Every group of columns has its own MMAs, so a group's step can multiply the score or the weight.
+//
+// Work.  Sequences are cut into units of 128 tokens; the list of all (sequence, kv head, query tile, unit) is dealt out in
+// equal contiguous ranges to the CTAs, whatever the lengths.  A warp takes 16 tokens of every unit through its own ring of
+// cp.async stages, which runs ahead across the ends of sequences.  The eight warps' results are joined in shared memory at
+// the end of a segment; a segment that CTAs share leaves fp32 partial sums, and the CTA that arrives last adds them up in
+// their fixed order, so the result does not depend on who that is.
 #include "sm100.cuh"
 #include "mla_common.cuh"
 
@@ -16,70 +36,677 @@ struct AttnInt4Params {
   const void* q;
   int64_t q_sb, q_ss;                  // elements from one sequence / query token to the next
   const uint8_t *k_codes, *v_codes;
-  const void *k_scale, *v_scale;
+  const uint32_t *k_scale, *v_scale;   // (step, minimum) pairs of the 16-bit type
   const int *table, *lens;
   void* out;
-  int batch, s_q, h_q, h_kv, page_size, max_pages, num_pages, len_cap;
-  float scale;
+  int batch, s_q, h_q, h_kv, per, page_size, max_pages, num_pages, len_cap;
+  int rows, q_tiles;                   // query rows of a kv head (s_q * per), tiles of them
+  uint32_t page_mul, page_shift;       // t / page_size = mulhi(t, page_mul) >> page_shift for page sizes that are no power of two
+  float scale_log2;
+  int* counters;                       // one per CTA, zero between calls
+  float* partial;                      // [2 * gridDim.x][kRows * (dim + 2)]
 };
 
-template <typename T> __device__ __forceinline__ float2 scale_pair(const void* base, int64_t i) {
-  const T* p = reinterpret_cast<const T*>(base) + 2 * i;
-  return make_float2(to_f32(p[0]), to_f32(p[1]));
+constexpr int kWarps = 8, kUnit = 16 * kWarps;
+
+template <int DIM, int GROUP, int NT> struct I4Cfg {
+  static constexpr int kGroups = DIM / GROUP;
+  static constexpr int kCodes = 16 * DIM / 2;                          // codes of 16 tokens
+  static constexpr int kStage = 2 * kCodes + 2 * 16 * 4 * kGroups + 16; // K, V, their scales, the mask of live tokens
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kPitch = DIM + 4;                                // floats of a row of the join buffer
+  static constexpr int kJoin = kWarps * kRows * (kPitch + 2) * 4;       // partial rows, maxima and sums of the eight warps
+  static constexpr int kCtas = DIM * NT <= 128 ? 2 : 1;                 // resident per SM: registers and shared memory
+  static constexpr int kFit = ((227 * 1024 / kCtas) - 1024 - kJoin - 128) / (kWarps * kStage);
+  static constexpr int kStages = kFit > 6 ? 6 : kFit;
+  static constexpr int kSmem = kWarps * kStages * kStage + kJoin + 128;
+  static_assert(kStages >= 3, "ring too short");
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+template <int N> __device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <int WORDS> __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[WORDS]) {
+  if constexpr (WORDS == 4)
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
+  else if constexpr (WORDS == 2)
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
+  else
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
 }
 
-template <typename T, int DIM>
-__global__ void __launch_bounds__(128)
-attn_int4_rows_kernel(const AttnInt4Params p, const int group) {
-  constexpr int E = DIM / 32;                      // columns a lane holds: lane * E ..
-  const int lane = threadIdx.x % 32;
-  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
-  if (row >= (int64_t)p.batch * p.s_q * p.h_q) return;
-  const int h = (int)(row % p.h_q), i = (int)(row / p.h_q % p.s_q), b = (int)(row / ((int64_t)p.h_q * p.s_q));
-  const int kvh = h / (p.h_q / p.h_kv), groups = DIM / group, g = lane * E / group;
-  const int len = mla_len(p.lens, b, p.len_cap), seen = len - p.s_q + i + 1;
-  float q[E], acc[E];
-  const T* qp = reinterpret_cast<const T*>(p.q) + b * p.q_sb + i * p.q_ss + (int64_t)h * DIM + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) { q[e] = to_f32(qp[e]); acc[e] = 0.f; }
-  float m = -INFINITY, l = 0.f;
-  for (int t = 0; t < seen; ++t) {
-    const int page = __ldg(p.table + (int64_t)b * p.max_pages + t / p.page_size);
-    if (!mla_page_ok(page, p.num_pages)) continue;
-    const int64_t r = ((int64_t)page * p.h_kv + kvh) * p.page_size + t % p.page_size;
-    const float2 ks = scale_pair<T>(p.k_scale, r * groups + g), vs = scale_pair<T>(p.v_scale, r * groups + g);
-    float dot = 0.f, v[E];
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const uint32_t kc = p.k_codes[r * (DIM / 2) + (lane * E + e) / 2], vc = p.v_codes[r * (DIM / 2) + (lane * E + e) / 2];
-      dot = fmaf(q[e], fmaf(ks.x, (float)(kc & 15u), ks.y), dot);
-      dot = fmaf(q[e + 1], fmaf(ks.x, (float)(kc >> 4), ks.y), dot);
-      v[e] = fmaf(vs.x, (float)(vc & 15u), vs.y);
-      v[e + 1] = fmaf(vs.x, (float)(vc >> 4), vs.y);
-    }
-    const float s = warp_sum(dot) * p.scale;
-    const float m_new = fmaxf(m, s);
-    const float alpha = m == -INFINITY ? 0.f : expf(m - m_new), w = expf(s - m_new);
-    l = fmaf(l, alpha, w);
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(acc[e], alpha, w * v[e]);
-    m = m_new;
+template <typename T> __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <uint32_t MASK, uint32_t OR> __device__ __forceinline__ uint32_t and_or(uint32_t v) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "n"(MASK), "n"(OR));      // (v & MASK) | OR
+  return r;
+}
+__device__ __forceinline__ uint32_t hfma2_bits(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
+// Four nibbles of each half of `r` as fp16 pairs of code - 8, exactly: 0x6400 | c is 1024 + c and 0x6400 | 16 c is 1024 + 16 c.
+__device__ __forceinline__ void widen4_f16(uint32_t r, uint32_t (&u)[4]) {
+  constexpr uint32_t kOne = 0x3c003c00u, kSixteenth = 0x2c002c00u, kM1032 = 0xe408e408u, kM72 = 0xd480d480u;
+  const uint32_t h = r >> 8;
+  u[0] = hfma2_bits(and_or<0x000f000fu, 0x64006400u>(r), kOne, kM1032);
+  u[1] = hfma2_bits(and_or<0x00f000f0u, 0x64006400u>(r), kSixteenth, kM72);
+  u[2] = hfma2_bits(and_or<0x000f000fu, 0x64006400u>(h), kOne, kM1032);
+  u[3] = hfma2_bits(and_or<0x00f000f0u, 0x64006400u>(h), kSixteenth, kM72);
+}
+// The same for keys.  bf16 has seven mantissa bits: 0x4300 | c is 128 + c, and the 128 is taken back once per score (its
+// share of the fp32 sum is 2^-24 of 144 sum |q|, far below the score's own rounding); fp16 as above.
+template <typename T> struct KeyOffset { static constexpr float value = -8.f; };
+template <> struct KeyOffset<__nv_bfloat16> { static constexpr float value = 128.f; };
+template <typename T> __device__ __forceinline__ void widen4_key(uint32_t r, uint32_t (&u)[4]) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    u[0] = and_or<0x000f000fu, 0x43004300u>(r);
+    u[1] = and_or<0x000f000fu, 0x43004300u>(r >> 4);
+    u[2] = and_or<0x000f000fu, 0x43004300u>(r >> 8);
+    u[3] = and_or<0x000f000fu, 0x43004300u>(r >> 12);
+  } else {
+    widen4_f16(r, u);
   }
-  T* o = reinterpret_cast<T*>(p.out) + row * DIM + lane * E;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = from_f32<T>(acc[e] * inv);
+}
+template <typename T> __device__ __forceinline__ float2 widen_scale(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <typename T>
-static int launch_int4(const AttnInt4Params& p, int64_t dim, int64_t group, cudaStream_t s) {
-  const int64_t rows = (int64_t)p.batch * p.s_q * p.h_q;
-  const unsigned grid = (unsigned)((rows + 3) / 4);
-  if (dim == 64) attn_int4_rows_kernel<T, 64><<<grid, 128, 0, s>>>(p, (int)group);
-  else if (dim == 128) attn_int4_rows_kernel<T, 128><<<grid, 128, 0, s>>>(p, (int)group);
-  else attn_int4_rows_kernel<T, 256><<<grid, 128, 0, s>>>(p, (int)group);
-  TL_LAUNCH_CHECK("attn_int4_rows_kernel");
+// Where a warp is in the list of units.  Units of a sequence: max(1, ceil(len / 128)), so an empty sequence still has its
+// zero rows written.
+struct UnitIter {
+  int b, h, qt, u, units, len;
+};
+__device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + kUnit - 1) / kUnit : 1; }
+__device__ __forceinline__ bool advance(UnitIter& it, const AttnInt4Params& p) {      // true: a new segment begins
+  if (++it.u < it.units) return false;
+  it.u = 0;
+  if (++it.qt == p.q_tiles) {
+    it.qt = 0;
+    if (++it.h == p.h_kv) {
+      it.h = 0;
+      if (++it.b < p.batch) {
+        it.len = mla_len(p.lens, it.b, p.len_cap);
+        it.units = units_of(it.len);
+      }
+    }
+  }
+  return true;
+}
+
+template <typename T, int DIM, int GROUP, int NT>
+__global__ void __launch_bounds__(32 * kWarps, I4Cfg<DIM, GROUP, NT>::kCtas)
+attn_int4_kernel(const AttnInt4Params p) {
+  using Cfg = I4Cfg<DIM, GROUP, NT>;
+  constexpr int NG = Cfg::kGroups, ST = Cfg::kStages, MT = DIM / 16, MG = GROUP / 16;
+  constexpr int kLines = 256 / DIM, kChunks = DIM / 32;          // rows per 128 bytes of shared memory, 16-byte chunks per row
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
+  uint8_t* tail = smem + kWarps * ST * Cfg::kStage;
+  float* join = reinterpret_cast<float*>(tail);                  // [warps][rows][pitch]
+  float* join_m = join + kWarps * Cfg::kRows * Cfg::kPitch;      // [warps][rows]
+  float* join_l = join_m + kWarps * Cfg::kRows;
+  int* shared_int = reinterpret_cast<int*>(join_l + kWarps * Cfg::kRows);
+  const uint32_t ring = smem_u32(smem) + warp * ST * Cfg::kStage;
+
+  // ---- this CTA's range of the list --------------------------------------------------------------------------------
+  int64_t total, ctas, start, end, seq_base;         // seq_base: first unit of sequence it.b
+  UnitIter it;
+  {
+    const int64_t per_unit = (int64_t)p.h_kv * p.q_tiles;
+    const int chunk = (p.batch + 32 * kWarps - 1) / (32 * kWarps);
+    const int b0 = min((int)threadIdx.x * chunk, p.batch), b1 = min(b0 + chunk, p.batch);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += units_of(mla_len(p.lens, b, p.len_cap));
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    int64_t* warp_sum64 = reinterpret_cast<int64_t*>(shared_int);        // 8 sums, then the found position in two more
+    int64_t* found = reinterpret_cast<int64_t*>(join);
+    if (lane == 31) warp_sum64[warp] = incl;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += warp_sum64[w];
+      total += warp_sum64[w];
+    }
+    total *= per_unit;
+    ctas = total < gridDim.x ? total : gridDim.x;                        // every one of them has a unit
+    if (blockIdx.x >= ctas) return;                                      // the whole CTA
+    start = (int64_t)blockIdx.x * total / ctas;
+    end = ((int64_t)blockIdx.x + 1) * total / ctas;
+    int64_t base = before + incl - mine;
+    if (base * per_unit <= start && start < (base + mine) * per_unit) {  // exactly one thread
+      int b = b0, units = 0;
+      for (; b < b1; ++b) {
+        units = units_of(mla_len(p.lens, b, p.len_cap));
+        if (start < (base + units) * per_unit) break;
+        base += units;
+      }
+      found[0] = b;
+      found[1] = base * per_unit;
+    }
+    __syncthreads();
+    it.b = (int)found[0];
+    seq_base = found[1];
+    it.len = mla_len(p.lens, it.b, p.len_cap);
+    it.units = units_of(it.len);
+    const int64_t off = start - seq_base;
+    const int seg = (int)(off / it.units);
+    it.u = (int)(off - (int64_t)seg * it.units);
+    it.h = seg / p.q_tiles;
+    it.qt = seg - it.h * p.q_tiles;
+    __syncthreads();                                                     // `found` lies in the join buffer
+  }
+
+  // ---- loads: 16 tokens of unit `w` into a stage; one commit group each, empty ones included ---------------------------
+  const bool tile_in_page = p.page_size % 16 == 0;
+  auto page_div = [&](uint32_t t) { return p.page_mul ? __umulhi(t, p.page_mul) >> p.page_shift : t >> p.page_shift; };
+  auto load = [&](const UnitIter& w, int stage, int first_page) {
+    const uint32_t at = ring + stage * Cfg::kStage;
+    const int t0 = w.u * kUnit + warp * 16;
+    const int* row_of_table = p.table + (int64_t)w.b * p.max_pages;
+    const int my = lane % 16;                                            // the token whose scales this lane loads
+    int64_t base = 0;                                                    // cache row of token t0 (of token `my` when pages end inside)
+    bool live = t0 + my < w.len;
+    if (tile_in_page) {
+      live = live && mla_page_ok(first_page, p.num_pages);
+      base = ((int64_t)first_page * p.h_kv + w.h) * p.page_size + (t0 - (int)page_div(t0) * p.page_size);
+    } else if (live) {
+      const int pg = (int)page_div(t0 + my), page = __ldg(row_of_table + pg);
+      live = mla_page_ok(page, p.num_pages);
+      base = ((int64_t)page * p.h_kv + w.h) * p.page_size + (t0 + my - pg * p.page_size);
+    }
+    const uint32_t mask = __ballot_sync(0xffffffffu, live) & 0xffffu;
+#pragma unroll
+    for (int i = 0; i < DIM / 64; ++i) {
+      const int id = lane + 32 * i, row = id / kChunks, c = id % kChunks;
+      int64_t src;
+      if (tile_in_page) {
+        src = base + row;
+      } else {
+        src = __shfl_sync(0xffffffffu, base, row);
+      }
+      if (mask >> row & 1) {
+        const int kf = (row / kLines * (GROUP / 32)) % kChunks;
+        const int rho = (row >> 1 & 3) | (row & 1) << 2 | (row & 8), vf = (rho / kLines * 2) % kChunks;
+        cp_async16(at + row * (DIM / 2) + (c ^ kf) * 16, p.k_codes + src * (DIM / 2) + c * 16);
+        cp_async16(at + Cfg::kCodes + rho * (DIM / 2) + (c ^ vf) * 16, p.v_codes + src * (DIM / 2) + c * 16);
+      }
+    }
+    if (live) {
+      const int64_t src = tile_in_page ? base + my : base;
+      const uint32_t* from = (lane < 16 ? p.k_scale : p.v_scale) + src * NG;
+      const uint32_t to = at + 2 * Cfg::kCodes + lane * (4 * NG);
+      if constexpr (NG <= 2) cp_async_small<4 * NG>(to, from);
+      else
+#pragma unroll
+        for (int i = 0; i < NG / 4; ++i) cp_async16(to + 16 * i, from + 4 * i);
+    }
+    if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 2 * Cfg::kCodes + 128 * NG), "r"(mask) : "memory");
+  };
+  auto page_at = [&](const UnitIter& w) {            // page id of the first token of this warp's tile (0 where it has none)
+    const int t0 = w.u * kUnit + warp * 16;
+    return tile_in_page && t0 < w.len ? __ldg(p.table + (int64_t)w.b * p.max_pages + page_div(t0)) : 0;
+  };
+
+  int64_t to_load = end - start, left = to_load;
+  UnitIter ahead = it;
+  int next_page = page_at(ahead);
+#pragma unroll 1
+  for (int s = 0; s < ST - 1; ++s) {
+    if (to_load > 0) {
+      load(ahead, s, next_page);
+      if (--to_load > 0) { advance(ahead, p); next_page = page_at(ahead); }
+    }
+    cp_async_commit();
+  }
+
+  // ---- segments -------------------------------------------------------------------------------------------------------
+  int stage = 0;
+  while (left > 0) {
+    const int rows = min(Cfg::kRows, p.rows - it.qt * Cfg::kRows);
+    // the columns of Q as the B operand, permuted like the columns of the widened keys
+    uint32_t qf[NT][DIM / 16][2];
+    float qsum[NG][NT][2];                            // scale * sum of q over the group, for queries 2j and 2j + 1
+    int limit[NT][2];                                 // keys that queries 2j and 2j + 1 see
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = nt * 8 + g, row = it.qt * Cfg::kRows + r;
+      const bool ok = r < rows;
+      const int qi = ok ? row / p.per : 0;
+      const T* src = reinterpret_cast<const T*>(p.q) + it.b * p.q_sb + qi * p.q_ss + ((int64_t)it.h * p.per + (ok ? row - qi * p.per : 0)) * DIM;
+#pragma unroll
+      for (int gg = 0; gg < NG; ++gg)
+#pragma unroll
+        for (int x = 0; x < GROUP / 32; ++x) {
+          const uint4 v = ok ? __ldg(reinterpret_cast<const uint4*>(src + gg * GROUP + (j * (GROUP / 32) + x) * 8)) : make_uint4(0, 0, 0, 0);
+          uint32_t(&f0)[2] = qf[nt][gg * MG + 2 * x], (&f1)[2] = qf[nt][gg * MG + 2 * x + 1];
+          f0[0] = __byte_perm(v.x, v.z, 0x5410);      // columns 0 and 4 of the word
+          f0[1] = __byte_perm(v.x, v.z, 0x7632);      // 1 and 5
+          f1[0] = __byte_perm(v.y, v.w, 0x5410);
+          f1[1] = __byte_perm(v.y, v.w, 0x7632);
+        }
+#pragma unroll
+      for (int gg = 0; gg < NG; ++gg) {               // sums of q: an MMA with keys of ones
+        constexpr uint32_t one = std::is_same<T, __nv_bfloat16>::value ? 0x3f803f80u : 0x3c003c00u;
+        const uint32_t ones[4] = {one, one, one, one};
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < MG; ++ks) mma16816<T>(d, ones, qf[nt][gg * MG + ks][0], qf[nt][gg * MG + ks][1]);
+        qsum[gg][nt][0] = d[0] * p.scale_log2;
+        qsum[gg][nt][1] = d[1] * p.scale_log2;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int rr = it.qt * Cfg::kRows + nt * 8 + 2 * j + e;
+        limit[nt][e] = it.len - p.s_q + rr / p.per + 1;
+      }
+    }
+    const int all_see = it.len - p.s_q + 1;           // tokens before this one are seen by every query
+
+    float acc[MT][NT][4], low[NG][NT][2], m[NT][2], l[NT][2];
+    float f = 0.f;                                    // the weights are p * step * f; 0: no step seen yet
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[nt][e] = -INFINITY;
+        l[nt][e] = 0.f;
+#pragma unroll
+        for (int gg = 0; gg < NG; ++gg) low[gg][nt][e] = 0.f;
+      }
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][nt][e] = 0.f;
+    }
+
+    const UnitIter seg = it;                          // its u is the first unit of this CTA's share
+    bool more = true;
+    while (more) {
+      cp_async_wait<ST - 2>();
+      __syncwarp();                                   // every lane's copies have landed, and every lane has left the stage refilled below
+      if (to_load > 0) {
+        load(ahead, stage == 0 ? ST - 1 : stage - 1, next_page);
+        if (--to_load > 0) { advance(ahead, p); next_page = page_at(ahead); }
+      }
+      cp_async_commit();
+      const uint32_t at = ring + stage * Cfg::kStage;
+      if (++stage == ST) stage = 0;
+      const int t0 = it.u * kUnit + warp * 16;
+      uint32_t mask[1];
+      lds_words(at + 2 * Cfg::kCodes + 128 * NG, mask);
+      if (mask[0]) {                                  // uniform in the warp
+        const bool live0 = mask[0] >> g & 1, live1 = mask[0] >> (g + 8) & 1;
+        // ---- S^T = K Q^T, log2 domain -------------------------------------------------------------------------------------
+        float sc[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[nt][e] = 0.f;
+#pragma unroll
+        for (int gg = 0; gg < NG; ++gg) {
+          constexpr int W = GROUP / 32;
+          uint32_t w0[W], w1[W];
+          {
+            const int b = gg * (GROUP / 2) + j * (GROUP / 8), c = b / 16, in = b % 16;       // byte in the row, chunk, byte in the chunk
+            const int f0 = (g / kLines * (GROUP / 32)) % kChunks, f1 = ((g + 8) / kLines * (GROUP / 32)) % kChunks;
+            lds_words(at + g * (DIM / 2) + (c ^ f0) * 16 + in, w0);
+            lds_words(at + (g + 8) * (DIM / 2) + (c ^ f1) * 16 + in, w1);
+          }
+          float d[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[nt][e] = 0.f;
+#pragma unroll
+          for (int x = 0; x < W; ++x) {
+            uint32_t u0[4], u1[4];
+            widen4_key<T>(w0[x], u0);
+            widen4_key<T>(w1[x], u1);
+            const uint32_t a0[4] = {u0[0], u1[0], u0[1], u1[1]}, a1[4] = {u0[2], u1[2], u0[3], u1[3]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<T>(d[nt], a0, qf[nt][gg * MG + 2 * x][0], qf[nt][gg * MG + 2 * x][1]);
+              mma16816<T>(d[nt], a1, qf[nt][gg * MG + 2 * x + 1][0], qf[nt][gg * MG + 2 * x + 1][1]);
+            }
+          }
+          uint32_t s0[1], s1[1];
+          lds_words(at + 2 * Cfg::kCodes + (g * NG + gg) * 4, s0);
+          lds_words(at + 2 * Cfg::kCodes + ((g + 8) * NG + gg) * 4, s1);
+          const float2 k0 = widen_scale<T>(s0[0]), k1 = widen_scale<T>(s1[0]);
+          const float a0 = k0.x * p.scale_log2, a1 = k1.x * p.scale_log2;
+          const float b0 = fmaf(-KeyOffset<T>::value, k0.x, k0.y), b1 = fmaf(-KeyOffset<T>::value, k1.x, k1.y);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              sc[nt][e] += fmaf(a0, d[nt][e], b0 * qsum[gg][nt][e]);
+              sc[nt][2 + e] += fmaf(a1, d[nt][2 + e], b1 * qsum[gg][nt][e]);
+            }
+        }
+        // ---- the values' steps, and whether the running maximum or the factor f has to move ------------------------------
+        float2 v0[NG], v1[NG];
+        float big = 0.f;
+#pragma unroll
+        for (int gg = 0; gg < NG; ++gg) {
+          uint32_t s0[1], s1[1];
+          lds_words(at + 2 * Cfg::kCodes + 64 * NG + (g * NG + gg) * 4, s0);
+          lds_words(at + 2 * Cfg::kCodes + 64 * NG + ((g + 8) * NG + gg) * 4, s1);
+          v0[gg] = live0 ? widen_scale<T>(s0[0]) : make_float2(0.f, 0.f);        // a stage's rows behind the last token hold anything
+          v1[gg] = live1 ? widen_scale<T>(s1[0]) : make_float2(0.f, 0.f);
+          v0[gg].y = fmaf(8.f, v0[gg].x, v0[gg].y);                              // the middle of the range: codes are widened to c - 8
+          v1[gg].y = fmaf(8.f, v1[gg].x, v1[gg].y);
+          big = fmaxf(big, fmaxf(fabsf(v0[gg].x), fabsf(v1[gg].x)));
+        }
+        bool see[NT][4];
+        bool grow = big * f > 64.f || (f == 0.f && big > 0.f);
+        const bool tail_tile = t0 + 16 > all_see;     // uniform
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            see[nt][e] = e < 2 ? live0 : live1;
+            if (tail_tile) see[nt][e] = see[nt][e] && t0 + g + (e < 2 ? 0 : 8) < limit[nt][e & 1];
+            // the maximum may lag by 2^8: p stays below 256, and sums are exact whatever the reference is
+            grow = grow || (see[nt][e] && sc[nt][e] > m[nt][e & 1] + 8.f);
+          }
+        if (__any_sync(0xffffffffu, grow)) {
+          float top[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              top[nt][e] = fmaxf(see[nt][e] ? sc[nt][e] : -INFINITY, see[nt][2 + e] ? sc[nt][2 + e] : -INFINITY);
+#pragma unroll
+          for (int o = 4; o < 32; o *= 2) {
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) top[nt][e] = fmaxf(top[nt][e], __shfl_xor_sync(0xffffffffu, top[nt][e], o));
+          }
+          float ratio = 1.f;                          // what the factor f changes by
+          if (big * f > 64.f || (f == 0.f && big > 0.f)) {
+            // f = 2^(4 - exponent): the largest step times f lies in [16, 32); exponents of f stay normal
+            const int ex = max((int)(__float_as_uint(big) >> 23) - 127, -112);
+            const float f_new = __uint_as_float((uint32_t)(127 + 4 - min(ex, 127)) << 23);
+            ratio = f == 0.f ? 0.f : f_new / f;
+            f = f_new;
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float m_new = fmaxf(m[nt][e], top[nt][e]);
+              const float alpha = m[nt][e] == -INFINITY ? 0.f : ex2_approx(m[nt][e] - m_new);
+              m[nt][e] = m_new;
+              l[nt][e] *= alpha;
+#pragma unroll
+              for (int gg = 0; gg < NG; ++gg) low[gg][nt][e] *= alpha;
+#pragma unroll
+              for (int t = 0; t < MT; ++t) {
+                acc[t][nt][e] *= alpha * ratio;
+                acc[t][nt][2 + e] *= alpha * ratio;
+              }
+            }
+        }
+        // ---- p, its sum, the minima's share --------------------------------------------------------------------------------
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sc[nt][e] = see[nt][e] ? ex2_approx(sc[nt][e] - m[nt][e & 1]) : 0.f;
+            l[nt][e & 1] += sc[nt][e];
+          }
+        // ---- O^T += V^T P^T, group by group ----------------------------------------------------------------------------------
+#pragma unroll
+        for (int gg = 0; gg < NG; ++gg) {
+          uint32_t pb[NT][2];
+          const float f0 = v0[gg].x * f, f1 = v1[gg].x * f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float w[4] = {sc[nt][0] * f0, sc[nt][1] * f0, sc[nt][2] * f1, sc[nt][3] * f1};
+            if (!tail_tile) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                low[gg][nt][e] = fmaf(sc[nt][e], v0[gg].y, fmaf(sc[nt][2 + e], v1[gg].y, low[gg][nt][e]));
+            } else {                                  // a value that a query does not see may be NaN, which 0 does not cancel
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                w[e] = see[nt][e] ? w[e] : 0.f;
+                low[gg][nt][e & 1] += see[nt][e] ? sc[nt][e] * (e < 2 ? v0[gg].y : v1[gg].y) : 0.f;
+              }
+            }
+            pb[nt][0] = movmatrix_trans(pack_f16(w[0], w[1]));
+            pb[nt][1] = movmatrix_trans(pack_f16(w[2], w[3]));
+          }
+          // words of tokens 2j, 2j + 1, 2j + 8, 2j + 9: rows j, j + 4, j + 8, j + 12 of the stage
+          constexpr int W = GROUP >= 64 ? GROUP / 64 : 1;
+          uint32_t w[4][W];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int rho = j + 4 * i, vf = (rho / kLines * 2) % kChunks;
+            const int b = gg * (GROUP / 2) + (GROUP >= 64 ? g * (GROUP / 16) : (g >> 1) * 4), c = b / 16, in = b % 16;
+            lds_words(at + Cfg::kCodes + rho * (DIM / 2) + (c ^ vf) * 16 + in, w[i]);
+          }
+#pragma unroll
+          for (int x = 0; x < W; ++x)
+#pragma unroll
+            for (int half = 0; half < (GROUP >= 64 ? 2 : 1); ++half) {
+              const uint32_t sel = GROUP >= 64 ? (half ? 0x7632u : 0x5410u) : ((g & 1) ? 0x7632u : 0x5410u);
+              uint32_t ua[4], ub[4];
+              widen4_f16(__byte_perm(w[0][x], w[1][x], sel), ua);
+              widen4_f16(__byte_perm(w[2][x], w[3][x], sel), ub);
+              const int t = gg * MG + (GROUP >= 64 ? 4 * x + 2 * half : 0);
+              const uint32_t a0[4] = {ua[0], ua[1], ub[0], ub[1]}, a1[4] = {ua[2], ua[3], ub[2], ub[3]};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<__half>(acc[t][nt], a0, pb[nt][0], pb[nt][1]);
+                mma16816<__half>(acc[t + 1][nt], a1, pb[nt][0], pb[nt][1]);
+              }
+            }
+        }
+      }
+      --left;
+      more = !advance(it, p) && left > 0;
+    }
+
+    // ---- join the warps ---------------------------------------------------------------------------------------------------
+#pragma unroll
+    for (int o = 4; o < 32; o *= 2)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], o);
+#pragma unroll
+          for (int gg = 0; gg < NG; ++gg) low[gg][nt][e] += __shfl_xor_sync(0xffffffffu, low[gg][nt][e], o);
+        }
+    if (g == 0)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) join_m[warp * Cfg::kRows + nt * 8 + 2 * j + e] = m[nt][e];
+    __syncthreads();
+    const float inv_f = f == 0.f ? 0.f : 1.f / f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = nt * 8 + 2 * j + e;
+        float top = join_m[r];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, join_m[w * Cfg::kRows + r]);
+        const float a = m[nt][e] == -INFINITY && l[nt][e] == 0.f ? 0.f : ex2_approx(m[nt][e] - top);
+        if (g == 0) join_l[warp * Cfg::kRows + r] = l[nt][e] * a;
+        float* dst = join + (warp * Cfg::kRows + r) * Cfg::kPitch;
+#pragma unroll
+        for (int gg = 0; gg < NG; ++gg)
+#pragma unroll
+          for (int t = 0; t < MG; ++t) {
+            const int d = gg * GROUP + g * (GROUP / 8) + 2 * t;
+            *reinterpret_cast<float2*>(dst + d) = make_float2((acc[gg * MG + t][nt][e] * inv_f + low[gg][nt][e]) * a,
+                                                              (acc[gg * MG + t][nt][2 + e] * inv_f + low[gg][nt][e]) * a);
+          }
+      }
+    __syncthreads();
+
+    // ---- the segment's rows: to the output, or to the partial sums --------------------------------------------------------
+    const int64_t seg_first = seq_base + ((int64_t)seg.h * p.q_tiles + seg.qt) * seg.units, seg_end = seg_first + seg.units;
+    const bool whole = seg_first >= start && seg_end <= end;
+    auto store_out = [&](int r, int d, float4 v) {
+      const int row = seg.qt * Cfg::kRows + r, qi = row / p.per;
+      T* dst = reinterpret_cast<T*>(p.out) + (((int64_t)seg.b * p.s_q + qi) * p.h_q + (int64_t)seg.h * p.per + (row - qi * p.per)) * DIM + d;
+      union { uint2 raw; T e[4]; } o;
+      o.e[0] = from_f32<T>(v.x); o.e[1] = from_f32<T>(v.y); o.e[2] = from_f32<T>(v.z); o.e[3] = from_f32<T>(v.w);
+      *reinterpret_cast<uint2*>(dst) = o.raw;
+    };
+    constexpr int kSlot = Cfg::kRows * (DIM + 2);      // floats of one partial result: rows, maxima, sums
+    float* slot = p.partial + ((int64_t)blockIdx.x * 2 + (seg_first + seg.u > start ? 1 : 0)) * kSlot;
+    for (int i = threadIdx.x; i < rows * (DIM / 4); i += 32 * kWarps) {
+      const int r = i / (DIM / 4), d = i % (DIM / 4) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum = 0.f, top = join_m[r];
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float4 a = *reinterpret_cast<const float4*>(join + (w * Cfg::kRows + r) * Cfg::kPitch + d);
+        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+        sum += join_l[w * Cfg::kRows + r];
+        top = fmaxf(top, join_m[w * Cfg::kRows + r]);
+      }
+      if (whole) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        store_out(r, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+      } else {
+        __stcg(reinterpret_cast<float4*>(slot + r * DIM + d), v);
+        if (d == 0) {
+          __stcg(slot + Cfg::kRows * DIM + r, top);
+          __stcg(slot + Cfg::kRows * (DIM + 1) + r, sum);
+        }
+      }
+    }
+    if (!whole) {
+      // CTAs c0 .. c1 share the segment; the last to arrive adds up their partial sums
+      const int c0 = (int)(((seg_first + 1) * ctas - 1) / total), c1 = (int)((seg_end * ctas - 1) / total);
+      int* counter = p.counters + c0;                // only one shared segment begins in a CTA's range: its last
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) shared_int[0] = atomicAdd(counter, 1) == c1 - c0;
+      __syncthreads();
+      if (shared_int[0]) {
+        __threadfence();
+        if (threadIdx.x == 0) *counter = 0;            // ready for the next call
+        auto slot_of = [&](int c) {                    // a CTA's first segment is in its slot 0, its last in slot 1
+          const int64_t c_start = (int64_t)c * total / ctas;
+          return p.partial + ((int64_t)c * 2 + (seg_first > c_start ? 1 : 0)) * kSlot;
+        };
+        for (int i = threadIdx.x; i < rows * (DIM / 4); i += 32 * kWarps) {
+          const int r = i / (DIM / 4), d = i % (DIM / 4) * 4;
+          float top = -INFINITY;
+          for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(slot_of(c) + Cfg::kRows * DIM + r));
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          float sum = 0.f;
+#pragma unroll 4
+          for (int c = c0; c <= c1; ++c) {
+            const float* s = slot_of(c);
+            const float mc = __ldcg(s + Cfg::kRows * DIM + r), lc = __ldcg(s + Cfg::kRows * (DIM + 1) + r);
+            const float a = mc == -INFINITY && lc == 0.f ? 0.f : ex2_approx(mc - top);
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(s + r * DIM + d));
+            v.x = fmaf(x.x, a, v.x); v.y = fmaf(x.y, a, v.y); v.z = fmaf(x.z, a, v.z); v.w = fmaf(x.w, a, v.w);
+            sum = fmaf(lc, a, sum);
+          }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          store_out(r, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        }
+      }
+    }
+    if (left > 0 && it.b != seg.b) seq_base += (int64_t)seg.units * p.h_kv * p.q_tiles;
+    __syncthreads();                                   // the join buffer is free again
+  }
+  cp_async_wait<0>();
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------
+// Query rows of a kv head go in tiles of 8; from 9 rows on of 16 (dim 64, 128), where a widened key serves twice as many.
+static int q_tile_rows(int64_t rows, int64_t dim) { return rows > 8 && dim <= 128 ? 16 : 8; }
+static int ctas_per_sm(int64_t dim, int tile_rows) { return dim * (tile_rows / 8) <= 128 ? 2 : 1; }
+
+struct I4Plan {
+  int tile_rows, q_tiles, grid;
+  int64_t bytes;
+};
+static I4Plan i4_plan(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim) {
+  I4Plan r;
+  const int64_t rows = s_q * (h_q / h_kv);
+  r.tile_rows = q_tile_rows(rows, dim);
+  r.q_tiles = (int)((rows + r.tile_rows - 1) / r.tile_rows);
+  r.grid = sm_count() * ctas_per_sm(dim, r.tile_rows);
+  r.bytes = TL_B200_ATTN_INT4_ZERO_BYTES + (int64_t)r.grid * 2 * r.tile_rows * (dim + 2) * 4;
+  return r;
+}
+
+template <typename T, int DIM, int GROUP, int NT>
+static int launch_i4(const AttnInt4Params& p, int grid, cudaStream_t s) {
+  auto kernel = attn_int4_kernel<T, DIM, GROUP, NT>;
+  constexpr int smem = I4Cfg<DIM, GROUP, NT>::kSmem;
+  TL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kernel<<<grid, 32 * kWarps, smem, s>>>(p);
+  TL_LAUNCH_CHECK("attn_int4_kernel");
   return TL_B200_OK;
+}
+template <typename T, int DIM, int GROUP>
+static int launch_i4_tile(const AttnInt4Params& p, const I4Plan& plan, cudaStream_t s) {
+  if constexpr (DIM <= 128)
+    if (plan.tile_rows == 16) return launch_i4<T, DIM, GROUP, 2>(p, plan.grid, s);
+  return launch_i4<T, DIM, GROUP, 1>(p, plan.grid, s);
+}
+template <typename T>
+static int launch_i4_dim(const AttnInt4Params& p, const I4Plan& plan, int64_t dim, int64_t group, cudaStream_t s) {
+  if (dim == 64) return group == 32 ? launch_i4_tile<T, 64, 32>(p, plan, s) : launch_i4_tile<T, 64, 64>(p, plan, s);
+  if (dim == 128) {
+    if (group == 32) return launch_i4_tile<T, 128, 32>(p, plan, s);
+    return group == 64 ? launch_i4_tile<T, 128, 64>(p, plan, s) : launch_i4_tile<T, 128, 128>(p, plan, s);
+  }
+  if (group == 32) return launch_i4_tile<T, 256, 32>(p, plan, s);
+  return group == 64 ? launch_i4_tile<T, 256, 64>(p, plan, s) : launch_i4_tile<T, 256, 128>(p, plan, s);
+}
+
+static bool i4_sizes_ok(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim) {
+  return batch >= 0 && s_q >= 0 && h_q >= 1 && h_kv >= 1 && h_q % h_kv == 0 && batch < (1 << 24) && s_q < (1 << 24) && h_q <= 65536 &&
+         batch * s_q * h_q < (1ll << 31) && (dim == 64 || dim == 128 || dim == 256);
 }
 
 }  // namespace tl
@@ -87,13 +714,7 @@ static int launch_int4(const AttnInt4Params& p, int64_t dim, int64_t group, cuda
 using namespace tl;
 
 extern "C" int64_t tl_b200_attn_decode_paged_int4_workspace_bytes(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim) {
-  (void)batch; (void)s_q; (void)h_q; (void)h_kv; (void)dim;
-  return 0;
-}
-
-extern "C" int64_t tl_b200_attn_decode_paged_int4_zero_bytes(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim) {
-  (void)batch; (void)s_q; (void)h_q; (void)h_kv; (void)dim;
-  return 0;
+  return i4_sizes_ok(batch, s_q, h_q, h_kv, dim) ? i4_plan(batch, s_q, h_q, h_kv, dim).bytes : 0;
 }
 
 extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache, const void* k_scale, const void* v_cache,
@@ -119,18 +740,31 @@ extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache
              "attn_decode_paged_int4: null tensor pointer");
   TL_REQUIRE(aligned16(q) && aligned16(out) && aligned16(k_cache) && aligned16(v_cache) && aligned16(k_scale) && aligned16(v_scale) &&
                  q_stride_batch % 8 == 0 && q_stride_token % 8 == 0, "attn_decode_paged_int4: tensors and rows of q must be 16-byte aligned");
+  const I4Plan plan = i4_plan(batch, s_q, h_q, h_kv, dim);
+  TL_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= plan.bytes,
+             "attn_decode_paged_int4: needs a 16-byte aligned workspace of %lld bytes, got %lld", (long long)plan.bytes,
+             (long long)workspace_bytes);
   AttnInt4Params p;
   p.q = q; p.q_sb = q_stride_batch; p.q_ss = q_stride_token;
   p.k_codes = (const uint8_t*)k_cache; p.v_codes = (const uint8_t*)v_cache;
-  p.k_scale = k_scale; p.v_scale = v_scale;
+  p.k_scale = (const uint32_t*)k_scale; p.v_scale = (const uint32_t*)v_scale;
   p.table = block_table; p.lens = cache_seqlens; p.out = out;
-  p.batch = (int)batch; p.s_q = (int)s_q; p.h_q = (int)h_q; p.h_kv = (int)h_kv;
+  p.batch = (int)batch; p.s_q = (int)s_q; p.h_q = (int)h_q; p.h_kv = (int)h_kv; p.per = (int)(h_q / h_kv);
   p.page_size = (int)page_size; p.max_pages = (int)max_pages_per_seq; p.num_pages = (int)num_pages;
   const int64_t cap = max_pages_per_seq * page_size;           // a sequence may name a page more than once
-  p.len_cap = (int)(cap < 0x7fffff00ll ? cap : 0x7fffff00ll);
-  if (num_pages == 0) p.len_cap = 0;
-  p.scale = softmax_scale;
-  (void)workspace; (void)workspace_bytes;
-  return dtype == TL_BF16 ? launch_int4<__nv_bfloat16>(p, dim, group, (cudaStream_t)stream)
-                          : launch_int4<__half>(p, dim, group, (cudaStream_t)stream);
+  p.len_cap = num_pages == 0 ? 0 : (int)(cap < 0x7fff0000ll ? cap : 0x7fff0000ll);
+  p.rows = (int)(s_q * (h_q / h_kv)); p.q_tiles = plan.q_tiles;
+  // t / page_size for 0 <= t < 2^31: a shift for powers of two, else floor(t m / 2^(32 + k)) with k = floor(log2 page_size)
+  // and m = ceil(2^(32 + k) / page_size) < 2^32; m page_size exceeds 2^(32 + k) by less than page_size < 2^(k + 1), so the
+  // quotient is exact for t < 2^31
+  int k = 0;
+  while ((page_size >> (k + 1)) != 0) ++k;
+  p.page_shift = (uint32_t)k;
+  p.page_mul = (page_size & (page_size - 1)) == 0 ? 0u : (uint32_t)(((1ull << (32 + k)) + (uint64_t)page_size - 1) / (uint64_t)page_size);
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  TL_REQUIRE(plan.grid * 4 <= TL_B200_ATTN_INT4_ZERO_BYTES, "attn_decode_paged_int4: more SMs than counters");
+  p.counters = (int*)workspace;
+  p.partial = (float*)((uint8_t*)workspace + TL_B200_ATTN_INT4_ZERO_BYTES);
+  cudaStream_t s = (cudaStream_t)stream;
+  return dtype == TL_BF16 ? launch_i4_dim<__nv_bfloat16>(p, plan, dim, group, s) : launch_i4_dim<__half>(p, plan, dim, group, s);
 }

@@ -17,6 +17,7 @@ DEFAULT_LIB = _PKG_ROOT / "lib" / "libtl_b200.so"
 
 TL_F32, TL_F16, TL_BF16, TL_E4M3, TL_I32, TL_U32, TL_I16, TL_U4G = range(8)
 ABI_VERSION = 100          # TL_B200_VERSION of include/tl_b200.h
+ATTN_INT4_ZERO_BYTES = 4096   # TL_B200_ATTN_INT4_ZERO_BYTES
 
 # name -> (restype, argtypes).  Kept in declaration order of include/tl_b200.h.
 PROTOTYPES = {
@@ -58,7 +59,6 @@ PROTOTYPES = {
     "tl_b200_kv_cache_write": (c_int, [c_void_p] * 7 + [c_int64] * 8 + [c_int, c_int, c_void_p]),
     "tl_b200_kv_cache_read": (c_int, [c_void_p] * 7 + [c_int64] * 8 + [c_int, c_int, c_void_p]),
     "tl_b200_attn_decode_paged_int4_workspace_bytes": (c_int64, [c_int64] * 5),
-    "tl_b200_attn_decode_paged_int4_zero_bytes": (c_int64, [c_int64] * 5),
     "tl_b200_attn_decode_paged_int4": (c_int, [c_void_p] * 8 + [c_int64] * 11 + [c_float, c_int, c_void_p, c_int64, c_void_p]),
     "tl_b200_gemm_epilogue": (c_int, [c_void_p] * 5 + [c_int64] * 3 + [c_int] * 4 + [c_void_p]),
     "tl_b200_tile_program_registers": (c_int, [c_int64]),

@@ -564,13 +564,13 @@ def kv_cache_read(slots: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Ten
 _int4_workspaces: dict = {}
 
 
-def _int4_workspace(device: torch.device, nbytes: int, zero_bytes: int) -> torch.Tensor:
+def _int4_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """Scratch of attn_decode_paged_int4, kept apart from the other operators': its counters have to be zero between calls.
     One buffer per (device, stream), as in _workspace; a call that is being captured gets one of its own from the graph's
     pool, so that two graphs never share counters, however their replays overlap."""
     if torch.cuda.is_current_stream_capturing():
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        buf[:zero_bytes].zero_()
+        buf[:N.ATTN_INT4_ZERO_BYTES].zero_()
         return buf
     key = (device, torch.cuda.current_stream(device).cuda_stream)
     buf = _int4_workspaces.get(key)
@@ -609,8 +609,7 @@ def attn_decode_paged_int4(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torc
     s = _prepare(k_cache, k_scale, v_cache, v_scale, block_table, cache_seqlens, out, q[:1, :1])
     lib = N.load()
     nbytes = int(lib.tl_b200_attn_decode_paged_int4_workspace_bytes(b, s_q, h_q, h_kv, d))
-    zero = int(lib.tl_b200_attn_decode_paged_int4_zero_bytes(b, s_q, h_q, h_kv, d))
-    ws = _int4_workspace(q.device, nbytes, zero)
+    ws = _int4_workspace(q.device, nbytes)
     return N.check(lib.tl_b200_attn_decode_paged_int4(
         _ptr(q), _ptr(k_cache), _ptr(k_scale), _ptr(v_cache), _ptr(v_scale), _ptr(block_table), _ptr(cache_seqlens), _ptr(out), b, s_q, h_q,
         h_kv, d, d // k_scale.shape[3], q.stride(0) if b > 1 else 0, q.stride(1) if s_q > 1 else 0, page, block_table.shape[1], num_pages,
