@@ -1,7 +1,15 @@
 // Matrix product with its epilogue:  C = act(A B + bias) + residual,  fp32 accumulation and epilogue, one rounding.
 //
-// A plain FMA kernel: 64 x 64 tiles of C through shared memory.
-#include "common.cuh"
+// Three kernels, by the number of rows m of A:
+//   m > 128   the GEMM's tcgen05 kernels (gemm_kernels.cuh) with the epilogue applied to the accumulator columns a thread
+//             holds, before they are rounded: bound by the tensor core, the epilogue runs under the next tile's MMAs.
+//   m <= 128  the product has to stream the weights once, 2 n k bytes: bound by HBM.  The weights are the 128-row operand
+//             and the m rows of A (rounded up to 16, 32, 64 or 128) the columns, D = W A^T, so no tile is mostly padding;
+//             K is cut over the CTAs of a cluster until two CTAs per SM have a share, each with its own ring of TMA loads,
+//             and the cluster adds its partial tiles up through distributed shared memory in a fixed order: no scratch, no
+//             atomics, one launch.
+//   else      (fp32, or rows that TMA cannot describe) a plain FMA kernel through shared memory.
+#include "gemm_kernels.cuh"
 
 namespace tl {
 
@@ -21,6 +29,308 @@ __device__ __forceinline__ float activate(float x, int act) {
   }
 }
 
+// 32 accumulator columns of one row (tcgen05 kernels of gemm_kernels.cuh).
+template <typename T> struct RowEpilogue {
+  const T* bias;
+  const T* residual;
+  int64_t ld;
+  int act;
+  int vec;                // rows of the residual and the bias are 16-byte aligned
+  __device__ __forceinline__ void add(uint32_t (&v)[32], const T* src, int valid) const {
+    if (vec && valid == 32) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 8) {
+        Vec16<T> x;
+        x.raw = *reinterpret_cast<const uint4*>(src + j);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j + e] = __float_as_uint(__uint_as_float(v[j + e]) + to_f32(x.e[e]));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j < valid) v[j] = __float_as_uint(__uint_as_float(v[j]) + to_f32(src[j]));
+    }
+  }
+  __device__ __forceinline__ void operator()(uint32_t (&v)[32], int row, int col, int valid) const {
+    if (bias) add(v, bias + col, valid);
+    if (act != TL_B200_ACT_NONE) {
+      switch (act) {      // the switch outside the loop: one copy of each function
+        case TL_B200_ACT_RELU:
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(activate(__uint_as_float(v[j]), TL_B200_ACT_RELU));
+          break;
+        case TL_B200_ACT_GELU:
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(activate(__uint_as_float(v[j]), TL_B200_ACT_GELU));
+          break;
+        case TL_B200_ACT_GELU_TANH:
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(activate(__uint_as_float(v[j]), TL_B200_ACT_GELU_TANH));
+          break;
+        default:
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(activate(__uint_as_float(v[j]), TL_B200_ACT_SILU));
+      }
+    }
+    if (residual) add(v, residual + (int64_t)row * ld + col, valid);
+  }
+};
+
+// =================================================================================
+// Few rows: D[128 weight rows, MT rows of A] per CTA, K split over a cluster
+// =================================================================================
+template <int MT> struct SkinnyCfg {
+  static constexpr int kStageW = kBM * kRowBytes;               // 128 weight rows (or 64 k rows of 2 x 64 weight columns)
+  static constexpr int kStageX = MT * kRowBytes;
+  static constexpr int kStage = kStageW + kStageX;
+  static constexpr int kStages = (113 * 1024 - 1024 - 256) / kStage;             // two CTAs per SM
+  static constexpr int kPitch = kBM + 4;                        // floats of a row (one row of A) of the partial tile
+  static constexpr int kSmemBytes = kStages * kStage + 1024 + 256;
+  static constexpr int kTmemCols = MT < 32 ? 32 : MT;
+  static_assert(MT * kPitch * 4 <= kStages * kStage, "the partial tile reuses the ring");
+};
+
+struct SkinnyParams {
+  void* c;
+  int m, n, k, splits, in_fmt;
+  int* status;
+};
+
+template <int MT, bool W_MN_MAJOR, typename T, typename TOut>
+__global__ void __launch_bounds__(128, 2)
+gemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const SkinnyParams p,
+                   const EpilogueArgs ep) {
+  using Cfg = SkinnyCfg<MT>;
+  constexpr int STAGES = Cfg::kStages, kBK = kRowBytes / 2;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - raw_addr);
+  uint8_t* tail = base_ptr + STAGES * Cfg::kStage;
+  const uint32_t bar_full = smem_u32(tail), bar_empty = bar_full + 8 * STAGES, bar_done = bar_empty + 8 * STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 8 * (2 * STAGES + 1));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int tile = blockIdx.x / p.splits, split = blockIdx.x % p.splits;         // the splits of a tile are one cluster
+  const int num_kb = (p.k + kBK - 1) / kBK;
+  const int kb0 = (int)((int64_t)split * num_kb / p.splits), kb1 = (int)((int64_t)(split + 1) * num_kb / p.splits);
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    mbar_init(bar_done, 1);
+    mbar_fence_init();
+    prefetch_tensormap(&tm_w);
+    prefetch_tensormap(&tm_x);
+  }
+  if (warp == 2) {
+    tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int stage = (kb - kb0) % STAGES;
+        if (!mbar_wait(bar_empty + 8 * stage, (((kb - kb0) / STAGES) & 1) ^ 1, abort_flag)) break;
+        const uint32_t full = bar_full + 8 * stage, dst = base + stage * Cfg::kStage;
+        mbar_expect_tx(full, Cfg::kStage);
+        if constexpr (W_MN_MAJOR) {          // weights [k, n]: two slabs of 64 columns x 64 k rows
+          tma_load_2d(dst, &tm_w, full, tile * kBM, kb * kBK);
+          tma_load_2d(dst + kBK * kRowBytes, &tm_w, full, tile * kBM + 64, kb * kBK);
+        } else {
+          tma_load_2d(dst, &tm_w, full, kb * kBK, tile * kBM);
+        }
+        tma_load_2d(dst + Cfg::kStageW, &tm_x, full, kb * kBK, 0);
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = make_idesc(p.in_fmt, p.in_fmt, W_MN_MAJOR, false, kBM, MT);
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int stage = (kb - kb0) % STAGES;
+        if (!(ok = mbar_wait(bar_full + 8 * stage, ((kb - kb0) / STAGES) & 1, abort_flag))) break;
+        tc_fence_after_sync();
+        const uint32_t w = base + stage * Cfg::kStage, x = w + Cfg::kStageW;
+#pragma unroll
+        for (int kk = 0; kk < kRowBytes / kUmmaBytes; ++kk) {
+          const uint64_t a = W_MN_MAJOR ? smem_desc_sw128(w + kk * 16 * kRowBytes, kBK * kRowBytes, 1024)
+                                        : smem_desc_sw128(w + kk * kUmmaBytes, 16, 1024);
+          mma_f16_ss(tmem_base, a, smem_desc_sw128(x + kk * kUmmaBytes, 16, 1024), idesc, (kb > kb0 || kk) ? 1u : 0u);
+        }
+        mma_commit(bar_empty + 8 * stage);
+      }
+      if (ok) mma_commit(bar_done);
+    }
+  }
+  __syncwarp();
+  // ---- the tile: thread = weight row (column of C), registers = rows of A --------------------------------------------
+  bool ok = mbar_wait(bar_done, 0, abort_flag);
+  ok = __all_sync(0xffffffffu, ok);
+  tc_fence_after_sync();
+  const int col = tile * kBM + warp * 32 + lane;
+  const T* residual = reinterpret_cast<const T*>(ep.residual);
+  TOut* c = reinterpret_cast<TOut*>(p.c);
+  auto finish = [&](float x, int row) {
+    if (ep.bias) x += to_f32(reinterpret_cast<const T*>(ep.bias)[col]);
+    x = activate(x, ep.act);
+    const int64_t at = (int64_t)row * p.n + col;
+    if (residual) x += to_f32(residual[at]);
+    c[at] = from_f32<TOut>(x);
+  };
+  const uint32_t t_addr = tmem_base + ((uint32_t)(warp * 32) << 16);
+  float* part = reinterpret_cast<float*>(base_ptr);               // [MT][kPitch]: every MMA that read the ring has retired
+  if (ok) {
+#pragma unroll 1
+    for (int c0 = 0; c0 < MT; c0 += 16) {
+      if (c0 >= p.m) break;
+      uint32_t v[16];
+      tmem_ld_32x16(t_addr + c0, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (p.splits == 1) {
+          if (c0 + e < p.m && col < p.n) finish(__uint_as_float(v[e]), c0 + e);
+        } else {
+          part[(c0 + e) * Cfg::kPitch + warp * 32 + lane] = __uint_as_float(v[e]);
+        }
+      }
+    }
+  }
+  if (p.splits > 1) {
+    cluster_sync_all();                                           // also publishes the partial tiles
+    if (ok) {
+      // this CTA's share of the tile's elements, four neighbouring columns a thread
+      const int r0 = (int)((int64_t)split * p.m / p.splits), r1 = (int)((int64_t)(split + 1) * p.m / p.splits);
+      for (int r = r0 + warp; r < r1; r += 4) {
+        const uint32_t at = smem_u32(part + r * Cfg::kPitch + lane * 4);
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < p.splits; ++s) {
+          float y[4];
+          asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3])
+                       : "r"(map_to_cta(at, s)) : "memory");
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] += y[e];
+        }
+        const int n0 = tile * kBM + lane * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n0 + e < p.n) {
+            float z = x[e];
+            if (ep.bias) z += to_f32(reinterpret_cast<const T*>(ep.bias)[n0 + e]);
+            z = activate(z, ep.act);
+            const int64_t o = (int64_t)r * p.n + n0 + e;
+            if (residual) z += to_f32(residual[o]);
+            c[o] = from_f32<TOut>(z);
+          }
+      }
+    }
+  }
+
+  // ---- teardown -------------------------------------------------------------------------------------------------------
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(20000);
+    if (threadIdx.x == 0 && p.status) *p.status = *abort_flag;
+    __syncthreads();
+  }
+  if (p.splits > 1) cluster_sync_all();                           // nobody leaves while its partial tile is being read
+  if (warp == 2) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, Cfg::kTmemCols);
+  }
+}
+
+template <int MT, bool W_MN_MAJOR, typename T, typename TOut>
+static int launch_skinny(const CUtensorMap& tw, const CUtensorMap& tx, const SkinnyParams& p, const EpilogueArgs& ep, cudaStream_t s) {
+  auto kernel = gemm_skinny_kernel<MT, W_MN_MAJOR, T, TOut>;
+  TL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SkinnyCfg<MT>::kSmemBytes));
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)p.splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.n + kBM - 1) / kBM * p.splits));
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = SkinnyCfg<MT>::kSmemBytes;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  TL_CUDA(cudaLaunchKernelEx(&cfg, kernel, tw, tx, p, ep));
+  TL_LAUNCH_CHECK("gemm_skinny_kernel");
+  return TL_B200_OK;
+}
+
+template <int MT, typename T>
+static int launch_skinny_out(const CUtensorMap& tw, const CUtensorMap& tx, const SkinnyParams& p, const EpilogueArgs& ep, bool mn, bool f32,
+                             cudaStream_t s) {
+  if (f32) return mn ? launch_skinny<MT, true, T, float>(tw, tx, p, ep, s) : launch_skinny<MT, false, T, float>(tw, tx, p, ep, s);
+  return mn ? launch_skinny<MT, true, T, T>(tw, tx, p, ep, s) : launch_skinny<MT, false, T, T>(tw, tx, p, ep, s);
+}
+
+constexpr int kSkinnyRows = 128;
+
+template <typename T>
+static int gemm_skinny(const void* a, const void* b, void* c, int m, int n, int k, bool trans_b, bool c_f32, const EpilogueArgs& ep,
+                       cudaStream_t s) {
+  const bool bf = std::is_same<T, __nv_bfloat16>::value;
+  const CUtensorMapDataType dt = bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const int mt = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+  CUtensorMap tw, tx;
+  {
+    uint64_t dims[2] = {(uint64_t)k, (uint64_t)m};
+    uint64_t strides[1] = {(uint64_t)k * 2};
+    uint32_t box[2] = {64u, (uint32_t)mt};
+    if (int rc = make_tensor_map(&tx, dt, 2, a, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  }
+  {
+    uint64_t dims[2] = {(uint64_t)(trans_b ? k : n), (uint64_t)(trans_b ? n : k)};
+    uint64_t strides[1] = {dims[0] * 2};
+    uint32_t box[2] = {64u, trans_b ? (uint32_t)kBM : 64u};
+    if (int rc = make_tensor_map(&tw, dt, 2, b, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  }
+  SkinnyParams p;
+  p.c = c; p.m = m; p.n = n; p.k = k;
+  p.in_fmt = bf ? kFmtBF16 : kFmtF16;
+  p.status = device_status_word();
+  // as many splits of K (1, 2, 4, 8: a portable cluster) as two CTAs per SM have room for, with at least four K blocks each
+  const int tiles = (n + kBM - 1) / kBM, num_kb = (k + 63) / 64;
+  p.splits = 1;
+  while (p.splits < 8 && (int64_t)tiles * p.splits * 2 <= 2 * sm_count() && num_kb >= p.splits * 2 * 4) p.splits *= 2;
+  const bool mn = !trans_b;
+  switch (mt) {
+    case 16: return launch_skinny_out<16, T>(tw, tx, p, ep, mn, c_f32, s);
+    case 32: return launch_skinny_out<32, T>(tw, tx, p, ep, mn, c_f32, s);
+    case 64: return launch_skinny_out<64, T>(tw, tx, p, ep, mn, c_f32, s);
+    default: return launch_skinny_out<128, T>(tw, tx, p, ep, mn, c_f32, s);
+  }
+}
+
+template <typename T>
+static int gemm_epilogue_tc(const void* a, const void* b, void* c, int m, int n, int k, bool trans_b, bool c_f32, const EpilogueArgs& ep,
+                            cudaStream_t s) {
+  if (m <= kSkinnyRows) return gemm_skinny<T>(a, b, c, m, n, k, trans_b, c_f32, ep, s);
+  RowEpilogue<T> e;
+  e.bias = (const T*)ep.bias;
+  e.residual = (const T*)ep.residual;
+  e.ld = n;
+  e.act = ep.act;
+  e.vec = n % 8 == 0 && aligned16(ep.bias) && aligned16(ep.residual);
+  return gemm_tc<T, RowEpilogue<T>>(a, b, c, m, n, k, trans_b, c_f32, s, 0, 0, e);
+}
+
+// =================================================================================
+// Plain FMA kernel: fp32, and 16-bit shapes without a tensor map; 64 x 64 tiles of C through shared memory
+// =================================================================================
 template <typename TIn, typename TOut, bool TRANS_B>
 __global__ void __launch_bounds__(256)
 gemm_epilogue_fma_kernel(const TIn* __restrict__ a, const TIn* __restrict__ b, TOut* c, int m, int n, int k, const EpilogueArgs ep) {
@@ -96,6 +406,10 @@ extern "C" int tl_b200_gemm_epilogue(const void* a, const void* b, const void* b
   const int M = (int)m, N = (int)n, K = (int)k;
   cudaStream_t s = (cudaStream_t)stream;
   if (in_dtype == TL_F32) return launch_epilogue_fma<float, float>(a, b, c, M, N, K, tb, ep, s);
+  // TMA needs 16-byte aligned bases and row strides
+  if (aligned16(a) && aligned16(b) && K % 8 == 0 && (tb || N % 8 == 0))
+    return in_dtype == TL_BF16 ? gemm_epilogue_tc<__nv_bfloat16>(a, b, c, M, N, K, tb, out_dtype == TL_F32, ep, s)
+                               : gemm_epilogue_tc<__half>(a, b, c, M, N, K, tb, out_dtype == TL_F32, ep, s);
   if (in_dtype == TL_BF16)
     return out_dtype == TL_F32 ? launch_epilogue_fma<__nv_bfloat16, float>(a, b, c, M, N, K, tb, ep, s)
                                : launch_epilogue_fma<__nv_bfloat16, __nv_bfloat16>(a, b, c, M, N, K, tb, ep, s);
