@@ -41,7 +41,7 @@ struct AttnInt4Params {
   void* out;
   int batch, s_q, h_q, h_kv, per, page_size, max_pages, num_pages, len_cap;
   int rows, q_tiles;                   // query rows of a kv head (s_q * per), tiles of them
-  uint32_t page_mul, page_shift;       // t / page_size = mulhi(t, page_mul) >> page_shift for page sizes that are no power of two
+  FastDiv page_div;                    // t / page_size
   float scale_log2;
   int* counters;                       // one per CTA, zero between calls
   float* partial;                      // [2 * gridDim.x][kRows * (dim + 2)]
@@ -232,7 +232,6 @@ attn_int4_kernel(const AttnInt4Params p) {
 
   // ---- loads: 16 tokens of unit `w` into a stage; one commit group each, empty ones included ---------------------------
   const bool tile_in_page = p.page_size % 16 == 0;
-  auto page_div = [&](uint32_t t) { return p.page_mul ? __umulhi(t, p.page_mul) >> p.page_shift : t >> p.page_shift; };
   auto load = [&](const UnitIter& w, int stage, int first_page) {
     const uint32_t at = ring + stage * Cfg::kStage;
     const int t0 = w.u * kUnit + warp * 16;
@@ -242,9 +241,9 @@ attn_int4_kernel(const AttnInt4Params p) {
     bool live = t0 + my < w.len;
     if (tile_in_page) {
       live = live && mla_page_ok(first_page, p.num_pages);
-      base = ((int64_t)first_page * p.h_kv + w.h) * p.page_size + (t0 - (int)page_div(t0) * p.page_size);
+      base = ((int64_t)first_page * p.h_kv + w.h) * p.page_size + (t0 - (int)p.page_div(t0) * p.page_size);
     } else if (live) {
-      const int pg = (int)page_div(t0 + my), page = __ldg(row_of_table + pg);
+      const int pg = (int)p.page_div(t0 + my), page = __ldg(row_of_table + pg);
       live = mla_page_ok(page, p.num_pages);
       base = ((int64_t)page * p.h_kv + w.h) * p.page_size + (t0 + my - pg * p.page_size);
     }
@@ -278,7 +277,7 @@ attn_int4_kernel(const AttnInt4Params p) {
   };
   auto page_at = [&](const UnitIter& w) {            // page id of the first token of this warp's tile (0 where it has none)
     const int t0 = w.u * kUnit + warp * 16;
-    return tile_in_page && t0 < w.len ? __ldg(p.table + (int64_t)w.b * p.max_pages + page_div(t0)) : 0;
+    return tile_in_page && t0 < w.len ? __ldg(p.table + (int64_t)w.b * p.max_pages + p.page_div(t0)) : 0;
   };
 
   int64_t to_load = end - start, left = to_load;
@@ -754,13 +753,7 @@ extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache
   const int64_t cap = max_pages_per_seq * page_size;           // a sequence may name a page more than once
   p.len_cap = num_pages == 0 ? 0 : (int)(cap < 0x7fff0000ll ? cap : 0x7fff0000ll);
   p.rows = (int)(s_q * (h_q / h_kv)); p.q_tiles = plan.q_tiles;
-  // t / page_size for 0 <= t < 2^31: a shift for powers of two, else floor(t m / 2^(32 + k)) with k = floor(log2 page_size)
-  // and m = ceil(2^(32 + k) / page_size) < 2^32; m page_size exceeds 2^(32 + k) by less than page_size < 2^(k + 1), so the
-  // quotient is exact for t < 2^31
-  int k = 0;
-  while ((page_size >> (k + 1)) != 0) ++k;
-  p.page_shift = (uint32_t)k;
-  p.page_mul = (page_size & (page_size - 1)) == 0 ? 0u : (uint32_t)(((1ull << (32 + k)) + (uint64_t)page_size - 1) / (uint64_t)page_size);
+  p.page_div = FastDiv((uint32_t)page_size);
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   TL_REQUIRE(plan.grid * 4 <= TL_B200_ATTN_INT4_ZERO_BYTES, "attn_decode_paged_int4: more SMs than counters");
   p.counters = (int*)workspace;

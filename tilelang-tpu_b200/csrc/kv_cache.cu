@@ -13,7 +13,7 @@
 // skipped, and nothing else in the cache or in the output is touched.
 //
 // HBM-bound: a 16-bit row is read (written) once and its codes written (read) once.
-#include "common.cuh"
+#include "sm100.cuh"
 
 #include <type_traits>
 
@@ -21,12 +21,13 @@ namespace tl {
 
 struct CacheArgs {
   const int64_t* slots;
-  int64_t tokens;
+  uint32_t tokens, rows;      // rows = tokens * heads
   void* x[2];                 // rows of keys and of values (x[1] only with gridDim.y == 2)
   int64_t x_stride[2];        // elements from one token to the next
   void* cache[2];
   void* scale[2];
   int heads, page_size;
+  FastDiv head_div, page_div, vec_div;
   int64_t total_slots;
 };
 
@@ -37,16 +38,39 @@ __device__ __forceinline__ __half2 min2_nan(__half2 a, __half2 b) { return __hmi
 __device__ __forceinline__ __half2 max2_nan(__half2 a, __half2 b) { return __hmax2_nan(a, b); }
 
 template <typename T> struct Pair;
-template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
-template <> struct Pair<__half> { using type = __half2; };
+template <> struct Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static constexpr float kTiny = 0x1p-100f;       // smallest step of the quick division below
+};
+template <> struct Pair<__half> {
+  using type = __half2;
+  static constexpr float kTiny = 0x1p-14f;        // steps below are subnormal: coarser than 2^-9, a code can pass 15
+};
 
 __device__ __forceinline__ float2 widen2(__nv_bfloat162 v) { return __bfloat1622float2(v); }
 __device__ __forceinline__ float2 widen2(__half2 v) { return __half22float2(v); }
+template <typename T> __device__ __forceinline__ uint32_t narrow2(float2 f) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 h = __float22bfloat162_rn(f);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __float22half2_rn(f);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
 
 template <typename P> __device__ __forceinline__ P shfl_xor_pair(P v, int o) {
   uint32_t w = *reinterpret_cast<uint32_t*>(&v);
   w = __shfl_xor_sync(0xffffffffu, w, o);
   return *reinterpret_cast<P*>(&w);
+}
+
+// a / s for two values at once, correctly rounded, given y = rn(1 / s): Markstein's theorem (IBM J. Res. Dev. 34, 1990) -
+// q = rn(a y), then rn(q + (a - q s) y) is rn(a / s) as long as nothing leaves the normal range.  The codes have to be those
+// of the IEEE division of the definition, ties included; a division per element would cost three times the memory traffic.
+__device__ __forceinline__ float2 div2(float2 a, float2 neg_s, float2 y) {
+  const float2 q = sm100::mul2(a, y);
+  return sm100::fma2(sm100::fma2(q, neg_s, a), y, q);
 }
 
 // ---- 4 bits: a thread holds 16 columns (32 bytes in, 8 bytes of codes out); GROUP/16 neighbouring lanes own a group -----
@@ -56,16 +80,15 @@ kv_write_u4g_kernel(const CacheArgs p) {
   using P = typename Pair<T>::type;
   constexpr int kLanes = DIM / 16, kGroupLanes = GROUP / 16;
   const int which = blockIdx.y;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = idx / kLanes;
-  const int part = (int)(idx % kLanes);
-  const int64_t t = row / p.heads;
+  const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const int part = threadIdx.x % kLanes;
+  const uint32_t t = p.head_div(row);
   const int h = (int)(row - t * p.heads);
-  const int64_t slot = t < p.tokens ? __ldg(p.slots + t) : -1;
+  const int64_t slot = row < p.rows ? __ldg(p.slots + t) : -1;
   const bool live = slot >= 0 && slot < p.total_slots;
   union { uint4 raw[2]; P v[8]; } in;
   in.raw[0] = in.raw[1] = make_uint4(0, 0, 0, 0);
-  if (live) {
+  if (row < p.rows) {                 // whatever the slot: the two loads need not wait for each other
     const T* src = reinterpret_cast<const T*>(p.x[which]) + t * p.x_stride[which] + h * DIM + part * 16;
     in.raw[0] = ld_stream16(src);
     in.raw[1] = ld_stream16(src + 8);
@@ -84,15 +107,33 @@ kv_write_u4g_kernel(const CacheArgs p) {
   const T step16 = from_f32<T>((to_f32(hi16) - lo) / 15.0f);
   const float step = to_f32(step16);
   uint32_t w[2] = {0, 0};
+  if (step >= Pair<T>::kTiny && step <= 0x1p100f) {
+    // (x - lo) / step < 15.5 here, since the step is within 2^-8 of a fifteenth of the range: no clamp.  Adding 1.5 * 2^23
+    // rounds to the nearest even integer and leaves the code in the low bits; eight of them are joined by shifts and adds,
+    // and the eight exponent fields taken off at the end.
+    const float y = __frcp_rn(step);
+    const float2 y2 = make_float2(y, y), s2 = make_float2(-step, -step), l2 = make_float2(-lo, -lo), magic = make_float2(12582912.f, 12582912.f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 f = widen2(in.v[i]);
-    // the same fp32 subtraction, IEEE division and round-to-even as the definition: codes agree bit for bit
-    const float a = step > 0.f ? rintf((f.x - lo) / step) : 0.f, b = step > 0.f ? rintf((f.y - lo) / step) : 0.f;
-    const uint32_t ca = (uint32_t)fminf(fmaxf(a, 0.f), 15.f), cb = (uint32_t)fminf(fmaxf(b, 0.f), 15.f);
-    w[i / 4] |= (ca | (cb << 4)) << (8 * (i & 3));
+    for (int half = 0; half < 2; ++half) {
+      uint32_t acc = 0;
+#pragma unroll
+      for (int i = 3; i >= 0; --i) {
+        const float2 r = sm100::add2(div2(sm100::add2(widen2(in.v[half * 4 + i]), l2), s2, y2), magic);
+        acc = (acc << 4) + __float_as_uint(r.y);
+        acc = (acc << 4) + __float_as_uint(r.x);
+      }
+      w[half] = acc - 0x4b400000u * 0x11111111u;
+    }
+  } else if (step > 0.f) {            // steps near the ends of the range, and NaN and infinity, whose codes do not matter
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = widen2(in.v[i]);
+      const uint32_t ca = (uint32_t)fminf(fmaxf(rintf((f.x - lo) / step), 0.f), 15.f);
+      const uint32_t cb = (uint32_t)fminf(fmaxf(rintf((f.y - lo) / step), 0.f), 15.f);
+      w[i / 4] |= (ca | (cb << 4)) << (8 * (i & 3));
+    }
   }
-  const uint32_t s32 = (uint32_t)slot, page = s32 / (uint32_t)p.page_size, off = s32 - page * (uint32_t)p.page_size;
+  const uint32_t s32 = (uint32_t)slot, page = p.page_div(s32), off = s32 - page * (uint32_t)p.page_size;
   const int64_t dst = ((int64_t)page * p.heads + h) * p.page_size + off;
   *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(p.cache[which]) + dst * (DIM / 2) + part * 8) = make_uint2(w[0], w[1]);
   if (part % kGroupLanes == 0) {
@@ -109,59 +150,70 @@ kv_read_u4g_kernel(const CacheArgs p) {
   using P = typename Pair<T>::type;
   constexpr int kLanes = DIM / 16, kGroupLanes = GROUP / 16;
   const int which = blockIdx.y;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = idx / kLanes;
-  const int part = (int)(idx % kLanes);
-  const int64_t t = row / p.heads;
+  const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const int part = threadIdx.x % kLanes;
+  if (row >= p.rows) return;
+  const uint32_t t = p.head_div(row);
   const int h = (int)(row - t * p.heads);
-  const int64_t slot = t < p.tokens ? __ldg(p.slots + t) : -1;
+  const int64_t slot = __ldg(p.slots + t);
   if (slot < 0 || slot >= p.total_slots) return;
-  const uint32_t s32 = (uint32_t)slot, page = s32 / (uint32_t)p.page_size, off = s32 - page * (uint32_t)p.page_size;
+  const uint32_t s32 = (uint32_t)slot, page = p.page_div(s32), off = s32 - page * (uint32_t)p.page_size;
   const int64_t src = ((int64_t)page * p.heads + h) * p.page_size + off;
-  const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(p.cache[which]) + src * (DIM / 2) + part * 8);
+  const uint2 codes = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(p.cache[which]) + src * (DIM / 2) + part * 8);
   const float2 sc = widen2(reinterpret_cast<const P*>(p.scale[which])[src * (DIM / GROUP) + part / kGroupLanes]);
-  union { uint4 raw[2]; T e[16]; } out;
+  const float2 s2 = make_float2(sc.x, sc.x), l2 = make_float2(sc.y, sc.y), m128 = make_float2(-128.f, -128.f);
+  uint32_t out[8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t c = ((i < 8 ? w.x : w.y) >> (4 * (i & 7))) & 15u;
-    out.e[i] = from_f32<T>(fmaf(sc.x, (float)c, sc.y));      // s * code is exact in fp32, so this is one rounding, then the output's
+  for (int half = 0; half < 2; ++half) {
+    const uint32_t w = half ? codes.y : codes.x;
+    float2 f[4];                      // columns i and i + 4 of the word
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;          // bf16 pair of 128 + code
+      const float2 c = sm100::add2(make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)), m128);
+      f[i] = sm100::fma2(s2, c, l2);  // s * code is exact in fp32, so this is one rounding; then the output's
+    }
+    out[half * 4 + 0] = narrow2<T>(make_float2(f[0].x, f[1].x));
+    out[half * 4 + 1] = narrow2<T>(make_float2(f[2].x, f[3].x));
+    out[half * 4 + 2] = narrow2<T>(make_float2(f[0].y, f[1].y));
+    out[half * 4 + 3] = narrow2<T>(make_float2(f[2].y, f[3].y));
   }
-  T* dst = reinterpret_cast<T*>(p.x[which]) + t * p.x_stride[which] + h * DIM + part * 16;
-  reinterpret_cast<uint4*>(dst)[0] = out.raw[0];
-  reinterpret_cast<uint4*>(dst)[1] = out.raw[1];
+  uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.x[which]) + t * p.x_stride[which] + h * DIM + part * 16);
+  dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
+  dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
 }
 
 // ---- e4m3: a warp owns a row and keeps it in registers, 8 columns (16 bytes) a lane and pass ----------------------------
 template <typename T, int PASSES>
 __global__ void __launch_bounds__(256)
 kv_write_e4m3_kernel(const CacheArgs p, const int dim) {
+  using P = typename Pair<T>::type;
   const int which = blockIdx.y;
   const int lane = threadIdx.x % 32;
-  const int64_t t = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  const int64_t slot = t < p.tokens ? __ldg(p.slots + t) : -1;
-  if (slot < 0 || slot >= p.total_slots) return;               // the whole warp
+  const uint32_t t = blockIdx.x * 8 + threadIdx.x / 32;
+  if (t >= p.tokens) return;                                   // the whole warp
+  const int64_t slot = __ldg(p.slots + t);
   const T* src = reinterpret_cast<const T*>(p.x[which]) + t * p.x_stride[which];
-  Vec16<T> v[PASSES];
+  union { uint4 raw; P v[4]; } in[PASSES];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
     const int c = (i * 32 + lane) * 8;
-    v[i].raw = c < dim ? ld_stream16(src + c) : make_uint4(0, 0, 0, 0);
+    in[i].raw = c < dim ? ld_stream16(src + c) : make_uint4(0, 0, 0, 0);
   }
-  float amax = 0.f;
+  P top = __habs2(in[0].v[0]);
 #pragma unroll
   for (int i = 0; i < PASSES; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = fabsf(to_f32(v[i].e[e]));
-      asm("max.NaN.f32 %0, %0, %1;" : "+f"(amax) : "f"(a));
-    }
+    for (int e = 0; e < 4; ++e) top = max2_nan(top, __habs2(in[i].v[e]));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float a = __shfl_xor_sync(0xffffffffu, amax, o);
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(amax) : "f"(a));
-  }
+  for (int o = 16; o > 0; o >>= 1) top = max2_nan(top, shfl_xor_pair(top, o));
+  if (slot < 0 || slot >= p.total_slots) return;
+  float amax = to_f32(__hmax_nan(top.x, top.y));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(amax) : "f"(1e-4f));
   const float s = amax / 448.0f;
+  const float y = __frcp_rn(s);
+  const float2 y2 = make_float2(y, y), s2 = make_float2(-s, -s);
+  const bool quick = s <= 0x1p100f;                            // s >= 2^-23 always
   uint8_t* dst = reinterpret_cast<uint8_t*>(p.cache[which]) + slot * dim;
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
@@ -169,10 +221,10 @@ kv_write_e4m3_kernel(const CacheArgs p, const int dim) {
     if (c < dim) {
       uint32_t w[2] = {0, 0};
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const __nv_fp8x2_storage_t two =
-            __nv_cvt_float2_to_fp8x2(make_float2(to_f32(v[i].e[e]) / s, to_f32(v[i].e[e + 1]) / s), __NV_SATFINITE, __NV_E4M3);
-        w[e / 4] |= (uint32_t)two << (8 * (e & 3));
+      for (int e = 0; e < 4; ++e) {
+        const float2 a = widen2(in[i].v[e]);
+        const float2 q = quick ? div2(a, s2, y2) : make_float2(a.x / s, a.y / s);
+        w[e / 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(q, __NV_SATFINITE, __NV_E4M3) << (16 * (e & 1));
       }
       *reinterpret_cast<uint2*>(dst + c) = make_uint2(w[0], w[1]);
     }
@@ -180,34 +232,37 @@ kv_write_e4m3_kernel(const CacheArgs p, const int dim) {
   if (lane == 0) reinterpret_cast<float*>(p.scale[which])[slot] = s;
 }
 
+// 8 columns a thread; a block takes kReadTokens tokens, their columns dealt out over its threads.
+constexpr int kReadTokens = 8;
 template <typename T>
 __global__ void __launch_bounds__(256)
 kv_read_e4m3_kernel(const CacheArgs p, const int dim) {
-  const int which = blockIdx.y;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int vecs = dim / 8;
-  const int64_t t = idx / vecs;
-  const int c = (int)(idx - t * vecs) * 8;
-  const int64_t slot = t < p.tokens ? __ldg(p.slots + t) : -1;
-  if (slot < 0 || slot >= p.total_slots) return;
-  const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(p.cache[which]) + slot * dim + c);
-  const float s = reinterpret_cast<const float*>(p.scale[which])[slot];
-  Vec16<T> out;
+  const int which = blockIdx.y, vecs = dim / 8;
+  const uint32_t t0 = blockIdx.x * kReadTokens;
+  const int items = (int)min((uint32_t)kReadTokens, p.tokens - t0) * vecs;
+  for (int i = threadIdx.x; i < items; i += 256) {
+    const uint32_t k = p.vec_div((uint32_t)i), t = t0 + k;
+    const int c = (i - (int)k * vecs) * 8;
+    const int64_t slot = __ldg(p.slots + t);
+    if (slot < 0 || slot >= p.total_slots) continue;
+    const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(p.cache[which]) + slot * dim + c);
+    const float s = reinterpret_cast<const float*>(p.scale[which])[slot];
+    uint32_t out[4];
 #pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xffffu), __NV_E4M3);
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));      // e4m3 -> fp16 is exact
-    out.e[e] = from_f32<T>(f.x * s);
-    out.e[e + 1] = from_f32<T>(f.y * s);
+    for (int e = 0; e < 4; ++e) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((e < 2 ? w.x : w.y) >> (16 * (e & 1))), __NV_E4M3);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));      // e4m3 -> fp16 is exact
+      out[e] = narrow2<T>(make_float2(f.x * s, f.y * s));
+    }
+    *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.x[which]) + t * p.x_stride[which] + c) = make_uint4(out[0], out[1], out[2], out[3]);
   }
-  *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.x[which]) + t * p.x_stride[which] + c) = out.raw;
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
 template <typename T, int DIM>
 static int launch_u4g(const CacheArgs& a, int group, int sides, bool write, cudaStream_t s) {
-  const int64_t threads = a.tokens * a.heads * (DIM / 16);
-  const dim3 grid((unsigned)((threads + 255) / 256), (unsigned)sides);
+  constexpr unsigned kRowsPerBlock = 256 / (DIM / 16);
+  const dim3 grid((a.rows + kRowsPerBlock - 1) / kRowsPerBlock, (unsigned)sides);
   auto go = [&](auto g) {
     constexpr int G = decltype(g)::value;
     if constexpr (G <= DIM) {
@@ -238,8 +293,8 @@ static int launch_cache(const CacheArgs& a, int64_t dim, int64_t group, int form
     else kv_write_e4m3_kernel<T, 4><<<grid, 256, 0, s>>>(a, d);
     TL_LAUNCH_CHECK("kv_write_e4m3_kernel");
   } else {
-    const int64_t threads = a.tokens * (dim / 8);
-    kv_read_e4m3_kernel<T><<<dim3((unsigned)((threads + 255) / 256), (unsigned)sides), 256, 0, s>>>(a, (int)dim);
+    const dim3 grid((a.tokens + kReadTokens - 1) / kReadTokens, (unsigned)sides);
+    kv_read_e4m3_kernel<T><<<grid, 256, 0, s>>>(a, (int)dim);
     TL_LAUNCH_CHECK("kv_read_e4m3_kernel");
   }
   return TL_B200_OK;
@@ -259,8 +314,7 @@ static int cache_call(const char* who, const int64_t* slots, int64_t tokens, con
     TL_REQUIRE(dim % 8 == 0 && dim <= 1024, "%s: e4m3 rows have a multiple of 8 columns, at most 1024", who);
   }
   TL_REQUIRE(num_pages <= (1ll << 31) && page_size <= (1ll << 31) && num_pages * page_size < (1ll << 31), "%s: cache too large", who);
-  // grid.x < 2^31 blocks of 256 threads of at least 8 columns; the products below cannot overflow
-  TL_REQUIRE(heads <= 65536 && tokens < (1ll << 31) && tokens * heads * dim < (1ll << 41), "%s: size too large", who);
+  TL_REQUIRE(heads <= 65536 && tokens < (1ll << 31) && tokens * heads < (1ll << 31) - 256, "%s: size too large", who);
   if (tokens == 0) return TL_B200_OK;
   const bool both = v != nullptr || v_cache != nullptr || v_scale != nullptr;
   TL_REQUIRE(slots && k && k_cache && k_scale, "%s: null tensor pointer", who);
@@ -272,7 +326,8 @@ static int cache_call(const char* who, const int64_t* slots, int64_t tokens, con
   if (!write) TL_REQUIRE(tokens == 1 || (k_stride >= heads * dim && (!both || v_stride >= heads * dim)), "%s: output rows overlap", who);
   CacheArgs a;
   a.slots = slots;
-  a.tokens = tokens;
+  a.tokens = (uint32_t)tokens;
+  a.rows = (uint32_t)(tokens * heads);
   a.x[0] = const_cast<void*>(k); a.x[1] = const_cast<void*>(v);
   a.x_stride[0] = k_stride; a.x_stride[1] = v_stride;
   a.cache[0] = const_cast<void*>(k_cache); a.cache[1] = const_cast<void*>(v_cache);
@@ -280,6 +335,9 @@ static int cache_call(const char* who, const int64_t* slots, int64_t tokens, con
   a.heads = (int)heads;
   a.page_size = (int)page_size;
   a.total_slots = num_pages * page_size;
+  a.head_div = FastDiv((uint32_t)heads);
+  a.page_div = FastDiv((uint32_t)page_size);
+  a.vec_div = FastDiv((uint32_t)(dim / 8));
   cudaStream_t s = (cudaStream_t)stream;
   const int sides = both ? 2 : 1;
   return dtype == TL_BF16 ? launch_cache<__nv_bfloat16>(a, dim, group, format, sides, write, s)
