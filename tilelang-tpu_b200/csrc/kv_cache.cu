@@ -19,13 +19,15 @@
 
 namespace tl {
 
+struct Side {
+  void* x;                    // 16-bit rows
+  int64_t stride;             // elements from one token to the next
+  void *cache, *scale;
+};
 struct CacheArgs {
   const int64_t* slots;
   uint32_t tokens, rows;      // rows = tokens * heads
-  void* x[2];                 // rows of keys and of values (x[1] only with gridDim.y == 2)
-  int64_t x_stride[2];        // elements from one token to the next
-  void* cache[2];
-  void* scale[2];
+  Side k, v;                  // v only with gridDim.y == 2
   int heads, page_size;
   FastDiv head_div, page_div, vec_div;
   int64_t total_slots;
@@ -79,7 +81,7 @@ __global__ void __launch_bounds__(256)
 kv_write_u4g_kernel(const CacheArgs p) {
   using P = typename Pair<T>::type;
   constexpr int kLanes = DIM / 16, kGroupLanes = GROUP / 16;
-  const int which = blockIdx.y;
+  const Side side = blockIdx.y ? p.v : p.k;
   const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   const int part = threadIdx.x % kLanes;
   const uint32_t t = p.head_div(row);
@@ -89,7 +91,7 @@ kv_write_u4g_kernel(const CacheArgs p) {
   union { uint4 raw[2]; P v[8]; } in;
   in.raw[0] = in.raw[1] = make_uint4(0, 0, 0, 0);
   if (row < p.rows) {                 // whatever the slot: the two loads need not wait for each other
-    const T* src = reinterpret_cast<const T*>(p.x[which]) + t * p.x_stride[which] + h * DIM + part * 16;
+    const T* src = reinterpret_cast<const T*>(side.x) + t * side.stride + h * DIM + part * 16;
     in.raw[0] = ld_stream16(src);
     in.raw[1] = ld_stream16(src + 8);
   }
@@ -135,12 +137,12 @@ kv_write_u4g_kernel(const CacheArgs p) {
   }
   const uint32_t s32 = (uint32_t)slot, page = p.page_div(s32), off = s32 - page * (uint32_t)p.page_size;
   const int64_t dst = ((int64_t)page * p.heads + h) * p.page_size + off;
-  *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(p.cache[which]) + dst * (DIM / 2) + part * 8) = make_uint2(w[0], w[1]);
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(side.cache) + dst * (DIM / 2) + part * 8) = make_uint2(w[0], w[1]);
   if (part % kGroupLanes == 0) {
     P sc;
     sc.x = step16;
     sc.y = lo16;
-    reinterpret_cast<P*>(p.scale[which])[dst * (DIM / GROUP) + part / kGroupLanes] = sc;
+    reinterpret_cast<P*>(side.scale)[dst * (DIM / GROUP) + part / kGroupLanes] = sc;
   }
 }
 
@@ -149,7 +151,7 @@ __global__ void __launch_bounds__(256)
 kv_read_u4g_kernel(const CacheArgs p) {
   using P = typename Pair<T>::type;
   constexpr int kLanes = DIM / 16, kGroupLanes = GROUP / 16;
-  const int which = blockIdx.y;
+  const Side side = blockIdx.y ? p.v : p.k;
   const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   const int part = threadIdx.x % kLanes;
   if (row >= p.rows) return;
@@ -159,8 +161,8 @@ kv_read_u4g_kernel(const CacheArgs p) {
   if (slot < 0 || slot >= p.total_slots) return;
   const uint32_t s32 = (uint32_t)slot, page = p.page_div(s32), off = s32 - page * (uint32_t)p.page_size;
   const int64_t src = ((int64_t)page * p.heads + h) * p.page_size + off;
-  const uint2 codes = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(p.cache[which]) + src * (DIM / 2) + part * 8);
-  const float2 sc = widen2(reinterpret_cast<const P*>(p.scale[which])[src * (DIM / GROUP) + part / kGroupLanes]);
+  const uint2 codes = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(side.cache) + src * (DIM / 2) + part * 8);
+  const float2 sc = widen2(reinterpret_cast<const P*>(side.scale)[src * (DIM / GROUP) + part / kGroupLanes]);
   const float2 s2 = make_float2(sc.x, sc.x), l2 = make_float2(sc.y, sc.y), m128 = make_float2(-128.f, -128.f);
   uint32_t out[8];
 #pragma unroll
@@ -178,7 +180,7 @@ kv_read_u4g_kernel(const CacheArgs p) {
     out[half * 4 + 2] = narrow2<T>(make_float2(f[0].y, f[1].y));
     out[half * 4 + 3] = narrow2<T>(make_float2(f[2].y, f[3].y));
   }
-  uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.x[which]) + t * p.x_stride[which] + h * DIM + part * 16);
+  uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(side.x) + t * side.stride + h * DIM + part * 16);
   dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
   dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
 }
@@ -188,12 +190,12 @@ template <typename T, int PASSES>
 __global__ void __launch_bounds__(256)
 kv_write_e4m3_kernel(const CacheArgs p, const int dim) {
   using P = typename Pair<T>::type;
-  const int which = blockIdx.y;
+  const Side side = blockIdx.y ? p.v : p.k;
   const int lane = threadIdx.x % 32;
   const uint32_t t = blockIdx.x * 8 + threadIdx.x / 32;
   if (t >= p.tokens) return;                                   // the whole warp
   const int64_t slot = __ldg(p.slots + t);
-  const T* src = reinterpret_cast<const T*>(p.x[which]) + t * p.x_stride[which];
+  const T* src = reinterpret_cast<const T*>(side.x) + t * side.stride;
   union { uint4 raw; P v[4]; } in[PASSES];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
@@ -214,7 +216,7 @@ kv_write_e4m3_kernel(const CacheArgs p, const int dim) {
   const float y = __frcp_rn(s);
   const float2 y2 = make_float2(y, y), s2 = make_float2(-s, -s);
   const bool quick = s <= 0x1p100f;                            // s >= 2^-23 always
-  uint8_t* dst = reinterpret_cast<uint8_t*>(p.cache[which]) + slot * dim;
+  uint8_t* dst = reinterpret_cast<uint8_t*>(side.cache) + slot * dim;
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
     const int c = (i * 32 + lane) * 8;
@@ -229,7 +231,7 @@ kv_write_e4m3_kernel(const CacheArgs p, const int dim) {
       *reinterpret_cast<uint2*>(dst + c) = make_uint2(w[0], w[1]);
     }
   }
-  if (lane == 0) reinterpret_cast<float*>(p.scale[which])[slot] = s;
+  if (lane == 0) reinterpret_cast<float*>(side.scale)[slot] = s;
 }
 
 // 8 columns a thread; a block takes kReadTokens tokens, their columns dealt out over its threads.
@@ -237,7 +239,8 @@ constexpr int kReadTokens = 8;
 template <typename T>
 __global__ void __launch_bounds__(256)
 kv_read_e4m3_kernel(const CacheArgs p, const int dim) {
-  const int which = blockIdx.y, vecs = dim / 8;
+  const Side side = blockIdx.y ? p.v : p.k;
+  const int vecs = dim / 8;
   const uint32_t t0 = blockIdx.x * kReadTokens;
   const int items = (int)min((uint32_t)kReadTokens, p.tokens - t0) * vecs;
   for (int i = threadIdx.x; i < items; i += 256) {
@@ -245,8 +248,8 @@ kv_read_e4m3_kernel(const CacheArgs p, const int dim) {
     const int c = (i - (int)k * vecs) * 8;
     const int64_t slot = __ldg(p.slots + t);
     if (slot < 0 || slot >= p.total_slots) continue;
-    const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(p.cache[which]) + slot * dim + c);
-    const float s = reinterpret_cast<const float*>(p.scale[which])[slot];
+    const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(side.cache) + slot * dim + c);
+    const float s = reinterpret_cast<const float*>(side.scale)[slot];
     uint32_t out[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -254,7 +257,7 @@ kv_read_e4m3_kernel(const CacheArgs p, const int dim) {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));      // e4m3 -> fp16 is exact
       out[e] = narrow2<T>(make_float2(f.x * s, f.y * s));
     }
-    *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.x[which]) + t * p.x_stride[which] + c) = make_uint4(out[0], out[1], out[2], out[3]);
+    *reinterpret_cast<uint4*>(reinterpret_cast<T*>(side.x) + t * side.stride + c) = make_uint4(out[0], out[1], out[2], out[3]);
   }
 }
 
@@ -328,10 +331,8 @@ static int cache_call(const char* who, const int64_t* slots, int64_t tokens, con
   a.slots = slots;
   a.tokens = (uint32_t)tokens;
   a.rows = (uint32_t)(tokens * heads);
-  a.x[0] = const_cast<void*>(k); a.x[1] = const_cast<void*>(v);
-  a.x_stride[0] = k_stride; a.x_stride[1] = v_stride;
-  a.cache[0] = const_cast<void*>(k_cache); a.cache[1] = const_cast<void*>(v_cache);
-  a.scale[0] = const_cast<void*>(k_scale); a.scale[1] = const_cast<void*>(v_scale);
+  a.k = Side{const_cast<void*>(k), k_stride, const_cast<void*>(k_cache), const_cast<void*>(k_scale)};
+  a.v = Side{const_cast<void*>(v), v_stride, const_cast<void*>(v_cache), const_cast<void*>(v_scale)};
   a.heads = (int)heads;
   a.page_size = (int)page_size;
   a.total_slots = num_pages * page_size;

@@ -473,72 +473,95 @@ def mla_decode_paged(q: torch.Tensor, kv_cache: torch.Tensor, kv_scale: torch.Te
                    "tl_b200_mla_decode_paged")
 
 
-def _rows(t: torch.Tensor, rows_shape, dtype, what: str) -> int:
-    """Elements from one token to the next of a (tokens, ...) tensor whose rows are dense."""
-    if tuple(t.shape[1:]) != tuple(rows_shape) or t.dtype != dtype:
-        raise ValueError(f"{what} must be (tokens, {', '.join(map(str, rows_shape))}) {dtype}, not {tuple(t.shape)} {t.dtype}")
-    if t.numel() and not t[:1].is_contiguous():
+def _stream_of(tensors) -> int:
+    """The device checks of `_prepare`, without the one on layout, for operators whose tensors may be strided; the calls of
+    one decode step are short, so each tensor is asked once."""
+    index = -1
+    for t in tensors:
+        if t is None:
+            continue
+        i = t.get_device()
+        if i < 0:
+            raise ValueError("b200 ops take CUDA tensors (there is no CPU path)")
+        if i != index:
+            if index >= 0:
+                raise ValueError(f"tensors on different devices: cuda:{index} and cuda:{i}")
+            index = i
+    if index not in _initialised_devices:
+        torch.cuda.current_device()            # torch's own initialisation
+        if index == torch.cuda.current_device():
+            N.check(N.load().tl_b200_init(index), "tl_b200_init")
+            _initialised_devices.add(index)
+    if index != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors are on cuda:{index} but the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _dense(name: str, *tensors) -> None:
+    for t in tensors:
+        if t is not None and not t.is_contiguous():
+            raise ValueError(f"{name}: b200 ops take contiguous tensors")
+
+
+def _token_rows(t: torch.Tensor, tokens: int, heads: int, dim: int, dtype, what: str) -> int:
+    """Elements from one token to the next of a (tokens, heads, dim) tensor (or (tokens, dim) where heads is 1) whose
+    tokens are dense in themselves."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype != dtype or shape[-1] != dim or len(shape) not in (2, 3) or (shape[1] if len(shape) == 3 else 1) != heads:
+        raise ValueError(f"{what} must be (tokens, {heads}, {dim}) {dtype}, not {tuple(shape)} {t.dtype}")
+    if shape[0] != tokens:
+        raise ValueError(f"{what}: one slot per row")
+    if stride[-1] != 1 or (heads > 1 and stride[1] != dim):
         raise ValueError(f"{what}: the columns of a token must be contiguous")
-    dense = 1
-    for n in rows_shape:
-        dense *= n
-    return t.stride(0) if t.shape[0] > 1 else dense
+    return stride[0] if tokens > 1 else heads * dim
 
 
-def _cache_call(fn: str, slots, k, k_cache, k_scale, v, v_cache, v_scale) -> int:
-    given = [x is not None for x in (v, v_cache, v_scale)]
-    if any(given) and not all(given):
+def _cache_call(fn: str, entry: str, slots, k, k_cache, k_scale, v, v_cache, v_scale, write: bool) -> int:
+    both = v is not None
+    if both != (v_cache is not None) or both != (v_scale is not None):
         raise ValueError(f"{fn}: v, v_cache and v_scale go together")
     if slots.dtype != torch.int64 or slots.dim() != 1:
         raise ValueError(f"{fn}: slots must be (tokens,) int64")
     tokens = slots.shape[0]
-    sides = [("k", k, k_cache, k_scale)] + ([("v", v, v_cache, v_scale)] if given[0] else [])
-    if any(x.shape[:1] != slots.shape for _, x, _, _ in sides):
-        raise ValueError(f"{fn}: one slot per row")
     dtype = k.dtype
     if dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"{fn}: rows must be bfloat16 or float16, not {dtype}")
-    strides = []
+    shape, sshape = k_cache.shape, k_scale.shape
     if k_cache.dtype == torch.uint8:
-        if k_cache.dim() != 4 or k_scale.dim() != 5:
+        if len(shape) != 4 or len(sshape) != 5:
             raise ValueError(f"{fn}: a 4-bit cache is (num_pages, heads, page, dim / 2) uint8 with a scale (num_pages, heads, page, groups, 2)")
-        num_pages, heads, page, half = k_cache.shape
-        dim, groups = 2 * half, k_scale.shape[3]
+        num_pages, heads, page, half = shape
+        dim, groups = 2 * half, sshape[3]
         if groups < 1 or dim % groups:
             raise ValueError(f"{fn}: {groups} groups do not divide {dim} columns")
         group, fmt = dim // groups, N.TL_U4G
-        for name, x, cache, scale in sides:
-            if cache.dtype != torch.uint8 or cache.shape != k_cache.shape or tuple(scale.shape) != (num_pages, heads, page, groups, 2) \
-                    or scale.dtype != dtype:
-                raise ValueError(f"{fn}: {name}_cache must be {tuple(k_cache.shape)} uint8 and {name}_scale "
-                                 f"{(num_pages, heads, page, groups, 2)} {dtype}")
-            strides.append(_rows(x, (heads, dim), dtype, f"{fn}: {name}"))
+        if sshape[:3] != shape[:3] or sshape[4] != 2 or k_scale.dtype != dtype:
+            raise ValueError(f"{fn}: k_scale must be {(num_pages, heads, page, groups, 2)} {dtype}")
     elif k_cache.dtype == torch.float8_e4m3fn:
-        if k_cache.dim() == 4 and k_cache.shape[2] != 1 or k_cache.dim() not in (3, 4):
+        if len(shape) not in (3, 4) or (len(shape) == 4 and shape[2] != 1):
             raise ValueError(f"{fn}: an e4m3 cache is (num_pages, page, dim) or (num_pages, page, 1, dim)")
-        num_pages, page, dim = k_cache.shape[0], k_cache.shape[1], k_cache.shape[-1]
+        num_pages, page, dim = shape[0], shape[1], shape[-1]
         heads, group, fmt = 1, dim, N.TL_E4M3
-        for name, x, cache, scale in sides:
-            if cache.dtype != torch.float8_e4m3fn or cache.shape != k_cache.shape or scale.dtype != torch.float32 \
-                    or tuple(scale.shape) != (num_pages, page):
-                raise ValueError(f"{fn}: {name}_cache must be {tuple(k_cache.shape)} e4m3 and {name}_scale ({num_pages}, {page}) float32")
-            if x.dim() == 3 and x.shape[1] == 1:
-                strides.append(_rows(x, (1, dim), dtype, f"{fn}: {name}"))
-            else:
-                strides.append(_rows(x, (dim,), dtype, f"{fn}: {name}"))
+        if tuple(sshape) != (num_pages, page) or k_scale.dtype != torch.float32:
+            raise ValueError(f"{fn}: k_scale must be ({num_pages}, {page}) float32")
     else:
         raise ValueError(f"{fn}: the cache must be uint8 (4-bit codes) or float8_e4m3fn, not {k_cache.dtype}")
-    if len(strides) == 1:
-        strides.append(0)
-    s = _prepare(slots, k_cache, k_scale, v_cache, v_scale, k[:1], v[:1] if v is not None else None)
+    k_stride, v_stride = _token_rows(k, tokens, heads, dim, dtype, "k"), 0
+    if both:
+        if v_cache.dtype != k_cache.dtype or v_cache.shape != shape or v_scale.dtype != k_scale.dtype or v_scale.shape != sshape:
+            raise ValueError(f"{fn}: v_cache and v_scale must be like k_cache and k_scale")
+        v_stride = _token_rows(v, tokens, heads, dim, dtype, "v")
+    _dense(fn, slots, k_cache, k_scale, v_cache, v_scale)
+    s = _stream_of((slots, k, k_cache, k_scale, v, v_cache, v_scale))
     lib = N.load()
-    if fn == "kv_cache_write":
-        rc = lib.tl_b200_kv_cache_write(_ptr(slots), _ptr(k), _ptr(k_cache), _ptr(k_scale), _ptr(v), _ptr(v_cache), _ptr(v_scale), tokens,
-                                        strides[0], strides[1], heads, dim, group, num_pages, page, fmt, dtype_code(dtype), s)
+    sizes = (tokens, k_stride, v_stride, heads, dim, group, num_pages, page, fmt, _DTYPES[dtype], s)
+    kp, kcp, ksp = k.data_ptr(), k_cache.data_ptr(), k_scale.data_ptr()
+    vp, vcp, vsp = (v.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr()) if both else (None, None, None)
+    if write:
+        rc = lib.tl_b200_kv_cache_write(slots.data_ptr(), kp, kcp, ksp, vp, vcp, vsp, *sizes)
     else:
-        rc = lib.tl_b200_kv_cache_read(_ptr(slots), _ptr(k_cache), _ptr(k_scale), _ptr(k), _ptr(v_cache), _ptr(v_scale), _ptr(v), tokens,
-                                       strides[0], strides[1], heads, dim, group, num_pages, page, fmt, dtype_code(dtype), s)
-    return N.check(rc, "tl_b200_" + fn)
+        rc = lib.tl_b200_kv_cache_read(slots.data_ptr(), kcp, ksp, kp, vcp, vsp, vp, *sizes)
+    return N.check(rc, entry)
 
 
 def kv_cache_write(slots: torch.Tensor, k: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor, v: torch.Tensor | None = None,
@@ -551,20 +574,20 @@ def kv_cache_write(slots: torch.Tensor, k: torch.Tensor, k_cache: torch.Tensor, 
     (32, 64 or 128; dim 64, 128 or 256).  e4m3 cache (the one mla_decode_paged reads): k (tokens, dim); cache
     (num_pages, page, dim) e4m3; scale (num_pages, page) float32.  k and v may be slices of a wider projection: only the
     columns of a token have to be contiguous.  Keys and values go in one launch when both are given."""
-    return _cache_call("kv_cache_write", slots, k, k_cache, k_scale, v, v_cache, v_scale)
+    return _cache_call("kv_cache_write", "tl_b200_kv_cache_write", slots, k, k_cache, k_scale, v, v_cache, v_scale, True)
 
 
 def kv_cache_read(slots: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor, k: torch.Tensor, v_cache: torch.Tensor | None = None,
                   v_scale: torch.Tensor | None = None, v: torch.Tensor | None = None) -> int:
     """Read rows of a quantised cache back in 16 bits: k[t] = value of slot slots[t]; layouts as in kv_cache_write.  Rows
     whose slot lies outside the cache are left as they are; a slot may be named more than once."""
-    return _cache_call("kv_cache_read", slots, k, k_cache, k_scale, v, v_cache, v_scale)
+    return _cache_call("kv_cache_read", "tl_b200_kv_cache_read", slots, k, k_cache, k_scale, v, v_cache, v_scale, False)
 
 
 _int4_workspaces: dict = {}
 
 
-def _int4_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+def _int4_workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """Scratch of attn_decode_paged_int4, kept apart from the other operators': its counters have to be zero between calls.
     One buffer per (device, stream), as in _workspace; a call that is being captured gets one of its own from the graph's
     pool, so that two graphs never share counters, however their replays overlap."""
@@ -572,7 +595,7 @@ def _int4_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
         buf[:N.ATTN_INT4_ZERO_BYTES].zero_()
         return buf
-    key = (device, torch.cuda.current_stream(device).cuda_stream)
+    key = (device.index, stream)
     buf = _int4_workspaces.get(key)
     if buf is None or buf.numel() < nbytes:
         buf = _int4_workspaces[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
@@ -587,33 +610,36 @@ def attn_decode_paged_int4(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torc
     (num_pages, h_kv, page, groups, 2) of q's dtype, block_table (B, max_pages) int32, cache_seqlens (B,) int32 (the new
     tokens included), out (B, s_q, h_q, D).  Query token i sees the keys before len - s_q + i + 1; a row that sees none
     is zero.  D 64, 128 or 256."""
-    if q.dim() != 4 or out.shape != q.shape or out.dtype != q.dtype or q.dtype not in (torch.bfloat16, torch.float16):
+    qshape, dtype = q.shape, q.dtype
+    if len(qshape) != 4 or out.shape != qshape or out.dtype != dtype or dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("attn_decode_paged_int4: q and out must be (B, s_q, h_q, D) bfloat16 or float16")
-    b, s_q, h_q, d = q.shape
-    if k_cache.dim() != 4 or k_cache.dtype != torch.uint8 or k_cache.shape[3] * 2 != d or v_cache.shape != k_cache.shape \
-            or v_cache.dtype != torch.uint8:
+    b, s_q, h_q, d = qshape
+    cshape, sshape = k_cache.shape, k_scale.shape
+    if len(cshape) != 4 or k_cache.dtype != torch.uint8 or cshape[3] * 2 != d or v_cache.shape != cshape or v_cache.dtype != torch.uint8:
         raise ValueError("attn_decode_paged_int4: caches must be (num_pages, h_kv, page, D / 2) uint8")
-    num_pages, h_kv, page, _ = k_cache.shape
-    if k_scale.dim() != 5 or tuple(k_scale.shape[:3]) != (num_pages, h_kv, page) or k_scale.shape[4] != 2 or k_scale.shape[3] < 1 \
-            or d % k_scale.shape[3] or v_scale.shape != k_scale.shape or k_scale.dtype != q.dtype or v_scale.dtype != q.dtype:
+    num_pages, h_kv, page, _ = cshape
+    if len(sshape) != 5 or sshape[:3] != cshape[:3] or sshape[4] != 2 or sshape[3] < 1 or d % sshape[3] or v_scale.shape != sshape \
+            or k_scale.dtype != dtype or v_scale.dtype != dtype:
         raise ValueError("attn_decode_paged_int4: scales must be (num_pages, h_kv, page, groups, 2) of q's dtype")
     if h_kv < 1 or h_q % h_kv:
         raise ValueError("attn_decode_paged_int4: h_q must be a multiple of h_kv")
-    if block_table.dtype != torch.int32 or cache_seqlens.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != b \
+    tshape = block_table.shape
+    if block_table.dtype != torch.int32 or cache_seqlens.dtype != torch.int32 or len(tshape) != 2 or tshape[0] != b \
             or cache_seqlens.numel() != b:
         raise ValueError("attn_decode_paged_int4: block_table (B, max_pages) and cache_seqlens (B,) must be int32")
-    if q.numel() and not q[:1, :1].is_contiguous():
+    sb, ss, sh, sd = q.stride()
+    if sd != 1 or (h_q > 1 and sh != d):
         raise ValueError("attn_decode_paged_int4: the heads of a token must be contiguous")
-    if softmax_scale is None:
-        softmax_scale = d ** -0.5
-    s = _prepare(k_cache, k_scale, v_cache, v_scale, block_table, cache_seqlens, out, q[:1, :1])
+    _dense("attn_decode_paged_int4", k_cache, k_scale, v_cache, v_scale, block_table, cache_seqlens, out)
+    s = _stream_of((q, k_cache, k_scale, v_cache, v_scale, block_table, cache_seqlens, out))
     lib = N.load()
-    nbytes = int(lib.tl_b200_attn_decode_paged_int4_workspace_bytes(b, s_q, h_q, h_kv, d))
-    ws = _int4_workspace(q.device, nbytes)
+    nbytes = lib.tl_b200_attn_decode_paged_int4_workspace_bytes(b, s_q, h_q, h_kv, d)
+    ws = _int4_workspace(q.device, s, nbytes)
     return N.check(lib.tl_b200_attn_decode_paged_int4(
-        _ptr(q), _ptr(k_cache), _ptr(k_scale), _ptr(v_cache), _ptr(v_scale), _ptr(block_table), _ptr(cache_seqlens), _ptr(out), b, s_q, h_q,
-        h_kv, d, d // k_scale.shape[3], q.stride(0) if b > 1 else 0, q.stride(1) if s_q > 1 else 0, page, block_table.shape[1], num_pages,
-        float(softmax_scale), dtype_code(q.dtype), _ptr(ws), nbytes, s), "tl_b200_attn_decode_paged_int4")
+        q.data_ptr(), k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
+        cache_seqlens.data_ptr(), out.data_ptr(), b, s_q, h_q, h_kv, d, d // sshape[3], sb if b > 1 else 0, ss if s_q > 1 else 0, page,
+        tshape[1], num_pages, d ** -0.5 if softmax_scale is None else softmax_scale, _DTYPES[dtype], ws.data_ptr(), nbytes, s),
+        "tl_b200_attn_decode_paged_int4")
 
 
 _ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
@@ -624,24 +650,26 @@ def gemm_epilogue(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, bias: torch
     """c = act(a @ b + bias) + residual (b is (K, N)), or with b.T (b is (N, K), transpose_b=True); fp32 accumulation and
     epilogue, one rounding.  bias (N,) and residual (M, N) share a's dtype, c has it or float32; residual may be c itself.
     activation: None, "relu", "gelu" (erf), "gelu_tanh" or "silu"."""
-    if a.dim() != 2 or b.dim() != 2 or c.dim() != 2:
+    ashape, bshape, cshape, dtype = a.shape, b.shape, c.shape, a.dtype
+    if len(ashape) != 2 or len(bshape) != 2 or len(cshape) != 2:
         raise ValueError("gemm_epilogue: a, b, c must be 2-D")
-    m, k = a.shape
-    n, kb = (b.shape[0], b.shape[1]) if transpose_b else (b.shape[1], b.shape[0])
+    m, k = ashape
+    n, kb = bshape if transpose_b else (bshape[1], bshape[0])
     if kb != k:
         raise ValueError("gemm K shape check failed")          # message of ppl_gemm's assert
-    if tuple(c.shape) != (m, n):
+    if cshape[0] != m or cshape[1] != n:
         raise ValueError(f"gemm_epilogue: c must be ({m}, {n})")
-    if a.dtype not in (torch.float16, torch.bfloat16, torch.float32) or b.dtype != a.dtype or c.dtype not in (a.dtype, torch.float32):
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32) or b.dtype != dtype or c.dtype not in (dtype, torch.float32):
         raise ValueError("gemm_epilogue: a and b must share float16, bfloat16 or float32; c has that dtype or float32")
-    if bias is not None and (bias.numel() != n or bias.dtype != a.dtype):
+    if bias is not None and (bias.numel() != n or bias.dtype != dtype):
         raise ValueError(f"gemm_epilogue: bias must hold {n} elements of a's dtype")
-    if residual is not None and (residual.shape != c.shape or residual.dtype != a.dtype):
+    if residual is not None and (residual.shape != cshape or residual.dtype != dtype):
         raise ValueError(f"gemm_epilogue: residual must be ({m}, {n}) of a's dtype")
     try:
         act = _ACTIVATIONS[activation]
     except (KeyError, TypeError):
         raise ValueError(f"gemm_epilogue: unknown activation {activation!r}") from None
-    s = _prepare(a, b, c, bias, residual)
-    return N.check(N.load().tl_b200_gemm_epilogue(_ptr(a), _ptr(b), _ptr(bias), _ptr(residual), _ptr(c), m, n, k, 1 if transpose_b else 0, act,
-                                                 dtype_code(a.dtype), dtype_code(c.dtype), s), "tl_b200_gemm_epilogue")
+    _dense("gemm_epilogue", a, b, c, bias, residual)
+    s = _stream_of((a, b, c, bias, residual))
+    return N.check(N.load().tl_b200_gemm_epilogue(a.data_ptr(), b.data_ptr(), _ptr(bias), _ptr(residual), c.data_ptr(), m, n, k,
+                                                 1 if transpose_b else 0, act, _DTYPES[dtype], _DTYPES[c.dtype], s), "tl_b200_gemm_epilogue")
