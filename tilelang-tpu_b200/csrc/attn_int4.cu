@@ -10,23 +10,28 @@
 //
 // Layout.  The MMAs are the warp-level m16n8k16 ones: at most 8 or 16 query rows share a key, so a 128-row tensor-memory
 // tile would be 90% padding, and codes have to pass through registers to be widened anyway.  Keys (and columns of V) are
-// the 16 rows, queries the 8 columns:  S^T = K Q^T  and  O^T = V^T P^T.  Widening folds into the operand layouts:
-//   * K: a lane holds whole 32-bit words of a key; (word >> 4i) & 0x000f000f are columns i and i + 4 of the word, one
-//     register of the A operand.  The columns of Q are permuted likewise when they are loaded, once a sequence.
-//   * V: a register of the A operand is one column of two neighbouring tokens: one byte permute joins half words of the two
-//     before they are widened.
+// the 16 rows, queries the 8 columns:  S^T = K Q^T  and  O^T = V^T P^T, both in fp16.  Widening is one AND per pair of
+// codes: a nibble in the low bits of an fp16 number is the subnormal c 2^-24 (the next nibble 16 c 2^-24), which the tensor
+// core multiplies exactly; the powers of two are taken back outside the loop.
+//   * K: a lane holds whole 32-bit words of a key; word & 0x000f000f are columns 0 and 4 of the word, one register of the A
+//     operand.  The columns of Q are permuted (and those of odd nibbles divided by 16) when they are loaded, once a
+//     sequence; a power of two per query tile brings Q into fp16's range, and what falls below it is 2^-35 of its largest.
+//   * V: a register of the A operand is one column of two neighbouring tokens: one byte permute joins half words of the two.
 //   * Steps and minima never touch the codes:  q . k = s (q . c) + lo sum(q) per group, and the value's step multiplies p
-//     (held in fp16 with a power-of-two factor per warp that keeps p s in range), its minimum adds p lo in fp32.
+//     (rounded to fp16 with a power-of-two factor per warp that keeps p s in range: 2^-12 of each weight), its minimum
+//     adds p lo in fp32.  The weights' rounding should meet c - 8, not c, so 8 times the sum of the ROUNDED weights, from an
+//     MMA with ones, is taken off, and 8 s goes to the minimum.
 // Every group of columns has its own MMAs, so a group's step can multiply the score or the weight.
 //
 // Work.  Sequences are cut into units of 128 tokens; the list of all (sequence, kv head, query tile, unit) is dealt out in
 // equal contiguous ranges to the CTAs, whatever the lengths.  A warp takes 16 tokens of every unit through its own ring of
-// cp.async stages, which runs ahead across the ends of sequences.  The eight warps' results are joined in shared memory at
-// the end of a segment; a segment that CTAs share leaves fp32 partial sums, and the CTA that arrives last adds them up in
+// cp.async stages, which runs ahead across the ends of sequences.  The eight warps' results are joined in shared memory,
+// a few rows at a time, at the end of a segment; a segment that CTAs share leaves fp32 partial sums, and the CTA that arrives last adds them up in
 // their fixed order, so the result does not depend on who that is.
 #include "sm100.cuh"
 #include "mla_common.cuh"
 
+#include <cfloat>
 #include <type_traits>
 
 namespace tl {
@@ -36,7 +41,7 @@ struct AttnInt4Params {
   const void* q;
   int64_t q_sb, q_ss;                  // elements from one sequence / query token to the next
   const uint8_t *k_codes, *v_codes;
-  const uint32_t *k_scale, *v_scale;   // (step, minimum) pairs of the 16-bit type
+  const uint8_t *k_scale, *v_scale;    // (step, minimum) pairs of the 16-bit type
   const int *table, *lens;
   void* out;
   int batch, s_q, h_q, h_kv, per, page_size, max_pages, num_pages, len_cap;
@@ -54,8 +59,9 @@ template <int DIM, int GROUP, int NT> struct I4Cfg {
   static constexpr int kCodes = 16 * DIM / 2;                          // codes of 16 tokens
   static constexpr int kStage = 2 * kCodes + 2 * 16 * 4 * kGroups + 16; // K, V, their scales, the mask of live tokens
   static constexpr int kRows = 8 * NT;
+  static constexpr int kJoinRows = 4 * NT;                              // rows joined at a time
   static constexpr int kPitch = DIM + 4;                                // floats of a row of the join buffer
-  static constexpr int kJoin = kWarps * kRows * (kPitch + 2) * 4;       // partial rows, maxima and sums of the eight warps
+  static constexpr int kJoin = kWarps * (kJoinRows * kPitch + 2 * kRows) * 4;   // partial rows, maxima and sums of the eight warps
   static constexpr int kCtas = DIM * NT <= 128 ? 2 : 1;                 // resident per SM: registers and shared memory
   static constexpr int kFit = ((227 * 1024 / kCtas) - 1024 - kJoin - 128) / (kWarps * kStage);
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
@@ -81,54 +87,23 @@ template <int WORDS> __device__ __forceinline__ void lds_words(uint32_t addr, ui
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
 }
 
-template <typename T> __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-template <uint32_t MASK, uint32_t OR> __device__ __forceinline__ uint32_t and_or(uint32_t v) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "n"(MASK), "n"(OR));      // (v & MASK) | OR
-  return r;
-}
-__device__ __forceinline__ uint32_t hfma2_bits(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
-
-// Four nibbles of each half of `r` as fp16 pairs of code - 8, exactly: 0x6400 | c is 1024 + c and 0x6400 | 16 c is 1024 + 16 c.
-__device__ __forceinline__ void widen4_f16(uint32_t r, uint32_t (&u)[4]) {
-  constexpr uint32_t kOne = 0x3c003c00u, kSixteenth = 0x2c002c00u, kM1032 = 0xe408e408u, kM72 = 0xd480d480u;
+// Four nibbles of each half of `r` as fp16 pairs: c, 16 c, c, 16 c, each times 2^-24 (subnormal, exact).
+__device__ __forceinline__ void widen4(uint32_t r, uint32_t (&u)[4]) {
   const uint32_t h = r >> 8;
-  u[0] = hfma2_bits(and_or<0x000f000fu, 0x64006400u>(r), kOne, kM1032);
-  u[1] = hfma2_bits(and_or<0x00f000f0u, 0x64006400u>(r), kSixteenth, kM72);
-  u[2] = hfma2_bits(and_or<0x000f000fu, 0x64006400u>(h), kOne, kM1032);
-  u[3] = hfma2_bits(and_or<0x00f000f0u, 0x64006400u>(h), kSixteenth, kM72);
-}
-// The same for keys.  bf16 has seven mantissa bits: 0x4300 | c is 128 + c, and the 128 is taken back once per score (its
-// share of the fp32 sum is 2^-24 of 144 sum |q|, far below the score's own rounding); fp16 as above.
-template <typename T> struct KeyOffset { static constexpr float value = -8.f; };
-template <> struct KeyOffset<__nv_bfloat16> { static constexpr float value = 128.f; };
-template <typename T> __device__ __forceinline__ void widen4_key(uint32_t r, uint32_t (&u)[4]) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    u[0] = and_or<0x000f000fu, 0x43004300u>(r);
-    u[1] = and_or<0x000f000fu, 0x43004300u>(r >> 4);
-    u[2] = and_or<0x000f000fu, 0x43004300u>(r >> 8);
-    u[3] = and_or<0x000f000fu, 0x43004300u>(r >> 12);
-  } else {
-    widen4_f16(r, u);
-  }
+  u[0] = r & 0x000f000fu;
+  u[1] = r & 0x00f000f0u;
+  u[2] = h & 0x000f000fu;
+  u[3] = h & 0x00f000f0u;
 }
 template <typename T> __device__ __forceinline__ float2 widen_scale(uint32_t w) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -170,8 +145,8 @@ attn_int4_kernel(const AttnInt4Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
   uint8_t* tail = smem + kWarps * ST * Cfg::kStage;
-  float* join = reinterpret_cast<float*>(tail);                  // [warps][rows][pitch]
-  float* join_m = join + kWarps * Cfg::kRows * Cfg::kPitch;      // [warps][rows]
+  float* join = reinterpret_cast<float*>(tail);                  // [warps][join rows][pitch]
+  float* join_m = join + kWarps * Cfg::kJoinRows * Cfg::kPitch;  // [warps][rows]
   float* join_l = join_m + kWarps * Cfg::kRows;
   int* shared_int = reinterpret_cast<int*>(join_l + kWarps * Cfg::kRows);
   const uint32_t ring = smem_u32(smem) + warp * ST * Cfg::kStage;
@@ -230,54 +205,80 @@ attn_int4_kernel(const AttnInt4Params p) {
     __syncthreads();                                                     // `found` lies in the join buffer
   }
 
-  // ---- loads: 16 tokens of unit `w` into a stage; one commit group each, empty ones included ---------------------------
+  // ---- loads: the 16 tokens of a warp in a unit go into a stage; one commit group each, empty ones included -------------
   const bool tile_in_page = p.page_size % 16 == 0;
-  auto load = [&](const UnitIter& w, int stage, int first_page) {
+  const uint8_t* k_lane = p.k_codes + lane * 16;                           // the codes of 16 tokens of a page are contiguous
+  const uint8_t* v_lane = p.v_codes + lane * 16;
+  const uint8_t* s_lane = (lane < 16 ? p.k_scale : p.v_scale) + lane % 16 * (4 * NG);
+  uint32_t k_dst[DIM / 64], v_dst[DIM / 64];
+#pragma unroll
+  for (int i = 0; i < DIM / 64; ++i) {
+    const int id = lane + 32 * i, row = id / kChunks, c = id % kChunks;
+    const int kf = (row / kLines * (GROUP / 32)) % kChunks;
+    const int rho = (row >> 1 & 3) | (row & 1) << 2 | (row & 8), vf = (rho / kLines * 2) % kChunks;
+    k_dst[i] = row * (DIM / 2) + (c ^ kf) * 16;
+    v_dst[i] = Cfg::kCodes + rho * (DIM / 2) + (c ^ vf) * 16;
+  }
+  const uint32_t s_dst = 2 * Cfg::kCodes + lane * (4 * NG);
+  auto load_scale = [&](uint32_t at, const uint8_t* from) {
+    if constexpr (NG <= 2) cp_async_small<4 * NG>(at + s_dst, from);
+    else
+#pragma unroll
+      for (int i = 0; i < NG / 4; ++i) cp_async16(at + s_dst + 16 * i, from + 16 * i);
+  };
+  auto load = [&](const UnitIter& w, int stage, int page) {
     const uint32_t at = ring + stage * Cfg::kStage;
     const int t0 = w.u * kUnit + warp * 16;
-    const int* row_of_table = p.table + (int64_t)w.b * p.max_pages;
-    const int my = lane % 16;                                            // the token whose scales this lane loads
-    int64_t base = 0;                                                    // cache row of token t0 (of token `my` when pages end inside)
-    bool live = t0 + my < w.len;
+    uint32_t mask;
     if (tile_in_page) {
-      live = live && mla_page_ok(first_page, p.num_pages);
-      base = ((int64_t)first_page * p.h_kv + w.h) * p.page_size + (t0 - (int)p.page_div(t0) * p.page_size);
-    } else if (live) {
-      const int pg = (int)p.page_div(t0 + my), page = __ldg(row_of_table + pg);
-      live = mla_page_ok(page, p.num_pages);
-      base = ((int64_t)page * p.h_kv + w.h) * p.page_size + (t0 + my - pg * p.page_size);
-    }
-    const uint32_t mask = __ballot_sync(0xffffffffu, live) & 0xffffu;
+      const uint32_t off = (uint32_t)t0 - p.page_div((uint32_t)t0) * (uint32_t)p.page_size;
+      const uint32_t row0 = ((uint32_t)page * p.h_kv + w.h) * (uint32_t)p.page_size + off;      // rows of the cache are fewer than 2^32
+      const int live = mla_page_ok(page, p.num_pages) ? min(max(w.len - t0, 0), 16) : 0;
+      mask = (1u << live) - 1u;
+      const uint8_t *k = k_lane + (uint64_t)row0 * (DIM / 2), *v = v_lane + (uint64_t)row0 * (DIM / 2), *sc = s_lane + (uint64_t)row0 * (4 * NG);
+      if (live == 16) {
 #pragma unroll
-    for (int i = 0; i < DIM / 64; ++i) {
-      const int id = lane + 32 * i, row = id / kChunks, c = id % kChunks;
-      int64_t src;
-      if (tile_in_page) {
-        src = base + row;
-      } else {
-        src = __shfl_sync(0xffffffffu, base, row);
-      }
-      if (mask >> row & 1) {
-        const int kf = (row / kLines * (GROUP / 32)) % kChunks;
-        const int rho = (row >> 1 & 3) | (row & 1) << 2 | (row & 8), vf = (rho / kLines * 2) % kChunks;
-        cp_async16(at + row * (DIM / 2) + (c ^ kf) * 16, p.k_codes + src * (DIM / 2) + c * 16);
-        cp_async16(at + Cfg::kCodes + rho * (DIM / 2) + (c ^ vf) * 16, p.v_codes + src * (DIM / 2) + c * 16);
-      }
-    }
-    if (live) {
-      const int64_t src = tile_in_page ? base + my : base;
-      const uint32_t* from = (lane < 16 ? p.k_scale : p.v_scale) + src * NG;
-      const uint32_t to = at + 2 * Cfg::kCodes + lane * (4 * NG);
-      if constexpr (NG <= 2) cp_async_small<4 * NG>(to, from);
-      else
+        for (int i = 0; i < DIM / 64; ++i) cp_async16(at + k_dst[i], k + 512 * i);
+        load_scale(at, sc);
 #pragma unroll
-        for (int i = 0; i < NG / 4; ++i) cp_async16(to + 16 * i, from + 4 * i);
+        for (int i = 0; i < DIM / 64; ++i) cp_async16(at + v_dst[i], v + 512 * i);
+      } else if (live > 0) {
+#pragma unroll
+        for (int i = 0; i < DIM / 64; ++i)
+          if ((lane + 32 * i) / kChunks < live) {
+            cp_async16(at + k_dst[i], k + 512 * i);
+            cp_async16(at + v_dst[i], v + 512 * i);
+          }
+        if (lane % 16 < live) load_scale(at, sc);
+      }
+    } else {                                          // pages end inside the tile: a table entry per token
+      const int my = t0 + lane % 16;
+      bool live = my < w.len;
+      uint32_t row = 0;
+      if (live) {
+        const uint32_t pg = p.page_div((uint32_t)my);
+        const int id = __ldg(p.table + (int64_t)w.b * p.max_pages + pg);
+        live = mla_page_ok(id, p.num_pages);
+        row = ((uint32_t)id * p.h_kv + w.h) * (uint32_t)p.page_size + ((uint32_t)my - pg * (uint32_t)p.page_size);
+      }
+      mask = __ballot_sync(0xffffffffu, live) & 0xffffu;
+#pragma unroll
+      for (int i = 0; i < DIM / 64; ++i) {
+        const int r = (lane + 32 * i) / kChunks;      // k_lane points at this lane's chunk of row lane / kChunks
+        const uint32_t from = __shfl_sync(0xffffffffu, row, r);
+        if (mask >> r & 1) {
+          const int64_t o = (int64_t)from * (DIM / 2) - (lane / kChunks) * (DIM / 2);
+          cp_async16(at + k_dst[i], k_lane + o);
+          cp_async16(at + v_dst[i], v_lane + o);
+        }
+      }
+      if (live) load_scale(at, s_lane + (int64_t)row * (4 * NG) - lane % 16 * (4 * NG));
     }
-    if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 2 * Cfg::kCodes + 128 * NG), "r"(mask) : "memory");
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 2 * Cfg::kCodes + 128 * NG), "r"(mask) : "memory");   // every lane, the same word
   };
   auto page_at = [&](const UnitIter& w) {            // page id of the first token of this warp's tile (0 where it has none)
     const int t0 = w.u * kUnit + warp * 16;
-    return tile_in_page && t0 < w.len ? __ldg(p.table + (int64_t)w.b * p.max_pages + p.page_div(t0)) : 0;
+    return tile_in_page && t0 < w.len ? __ldg(p.table + (int64_t)w.b * p.max_pages + p.page_div((uint32_t)t0)) : 0;
   };
 
   int64_t to_load = end - start, left = to_load;
@@ -296,55 +297,79 @@ attn_int4_kernel(const AttnInt4Params p) {
   int stage = 0;
   while (left > 0) {
     const int rows = min(Cfg::kRows, p.rows - it.qt * Cfg::kRows);
-    // the columns of Q as the B operand, permuted like the columns of the widened keys
+    // the columns of Q as the B operand: permuted like the columns of the widened keys, times a power of two that brings the
+    // largest (finite) one to 2^14, odd nibbles' columns divided by 16
     uint32_t qf[NT][DIM / 16][2];
-    float qsum[NG][NT][2];                            // scale * sum of q over the group, for queries 2j and 2j + 1
+    float qsum[NG][NT][2], to_score;                  // scale * sum of q over the group for queries 2j, 2j + 1; scale of the dot products
     int limit[NT][2];                                 // keys that queries 2j and 2j + 1 see
+    {
+      uint4 raw[NT][DIM / 32];
+      float big = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = nt * 8 + g, row = it.qt * Cfg::kRows + r;
-      const bool ok = r < rows;
-      const int qi = ok ? row / p.per : 0;
-      const T* src = reinterpret_cast<const T*>(p.q) + it.b * p.q_sb + qi * p.q_ss + ((int64_t)it.h * p.per + (ok ? row - qi * p.per : 0)) * DIM;
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = nt * 8 + g, row = it.qt * Cfg::kRows + r;
+        const bool ok = r < rows;
+        const int qi = ok ? row / p.per : 0;
+        const T* src = reinterpret_cast<const T*>(p.q) + it.b * p.q_sb + qi * p.q_ss + ((int64_t)it.h * p.per + (ok ? row - qi * p.per : 0)) * DIM;
 #pragma unroll
-      for (int gg = 0; gg < NG; ++gg)
-#pragma unroll
-        for (int x = 0; x < GROUP / 32; ++x) {
-          const uint4 v = ok ? __ldg(reinterpret_cast<const uint4*>(src + gg * GROUP + (j * (GROUP / 32) + x) * 8)) : make_uint4(0, 0, 0, 0);
-          uint32_t(&f0)[2] = qf[nt][gg * MG + 2 * x], (&f1)[2] = qf[nt][gg * MG + 2 * x + 1];
-          f0[0] = __byte_perm(v.x, v.z, 0x5410);      // columns 0 and 4 of the word
-          f0[1] = __byte_perm(v.x, v.z, 0x7632);      // 1 and 5
-          f1[0] = __byte_perm(v.y, v.w, 0x5410);
-          f1[1] = __byte_perm(v.y, v.w, 0x7632);
+        for (int x = 0; x < DIM / 32; ++x) {
+          const int col = x / (GROUP / 32) * GROUP + (j * (GROUP / 32) + x % (GROUP / 32)) * 8;
+          raw[nt][x] = ok ? __ldg(reinterpret_cast<const uint4*>(src + col)) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-      for (int gg = 0; gg < NG; ++gg) {               // sums of q: an MMA with keys of ones
-        constexpr uint32_t one = std::is_same<T, __nv_bfloat16>::value ? 0x3f803f80u : 0x3c003c00u;
-        const uint32_t ones[4] = {one, one, one, one};
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < MG; ++ks) mma16816<T>(d, ones, qf[nt][gg * MG + ks][0], qf[nt][gg * MG + ks][1]);
-        qsum[gg][nt][0] = d[0] * p.scale_log2;
-        qsum[gg][nt][1] = d[1] * p.scale_log2;
+        for (int e = 0; e < 2; ++e) limit[nt][e] = it.len - p.s_q + (it.qt * Cfg::kRows + nt * 8 + 2 * j + e) / p.per + 1;
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int rr = it.qt * Cfg::kRows + nt * 8 + 2 * j + e;
-        limit[nt][e] = it.len - p.s_q + rr / p.per + 1;
-      }
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < DIM / 32; ++x) {
+          const uint32_t w[4] = {raw[nt][x].x, raw[nt][x].y, raw[nt][x].z, raw[nt][x].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = widen_scale<T>(w[e]);
+            big = fmaxf(big, fabsf(f.x) < INFINITY ? fabsf(f.x) : 0.f);
+            big = fmaxf(big, fabsf(f.y) < INFINITY ? fabsf(f.y) : 0.f);
+          }
+        }
+      big = warp_max(big);
+      const int up = min(14 - ((int)(__float_as_uint(big) >> 23) - 127), 120);         // big < 2^128, so up >= -113
+      const float mul = __uint_as_float((uint32_t)(127 + up) << 23), mul16 = mul * 0.0625f;
+      to_score = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23) * 0x1p24f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < DIM / 32; ++x) {
+          const float2 e01 = widen_scale<T>(raw[nt][x].x), e23 = widen_scale<T>(raw[nt][x].y), e45 = widen_scale<T>(raw[nt][x].z),
+                       e67 = widen_scale<T>(raw[nt][x].w);
+          qf[nt][2 * x][0] = pack_f16(e01.x * mul, e45.x * mul);
+          qf[nt][2 * x][1] = pack_f16(e01.y * mul16, e45.y * mul16);
+          qf[nt][2 * x + 1][0] = pack_f16(e23.x * mul, e67.x * mul);
+          qf[nt][2 * x + 1][1] = pack_f16(e23.y * mul16, e67.y * mul16);
+        }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int gg = 0; gg < NG; ++gg) {             // sums of q: an MMA with keys whose widened codes are 1 and 16
+          const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u};
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < MG; ++ks) mma16816(d, ones, qf[nt][gg * MG + ks][0], qf[nt][gg * MG + ks][1]);
+          qsum[gg][nt][0] = d[0] * (to_score * 0x1p-24f);
+          qsum[gg][nt][1] = d[1] * (to_score * 0x1p-24f);
+        }
     }
     const int all_see = it.len - p.s_q + 1;           // tokens before this one are seen by every query
 
-    float acc[MT][NT][4], low[NG][NT][2], m[NT][2], l[NT][2];
-    float f = 0.f;                                    // the weights are p * step * f; 0: no step seen yet
+    float acc[MT][NT][4], wsum[NG][NT][4], low[NG][NT][2], m[NT][2], l[NT][2];
+    float f = 0.f, most = 0.f;                        // the weights are p * step * f, steps up to `most`; 0: none seen yet
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        m[nt][e] = -INFINITY;
+        m[nt][e] = -FLT_MAX;                          // finite, so that a score of -inf weighs 0 and not NaN
         l[nt][e] = 0.f;
 #pragma unroll
-        for (int gg = 0; gg < NG; ++gg) low[gg][nt][e] = 0.f;
+        for (int gg = 0; gg < NG; ++gg) low[gg][nt][e] = wsum[gg][nt][e] = wsum[gg][nt][2 + e] = 0.f;
       }
 #pragma unroll
       for (int t = 0; t < MT; ++t)
@@ -367,14 +392,10 @@ attn_int4_kernel(const AttnInt4Params p) {
       const int t0 = it.u * kUnit + warp * 16;
       uint32_t mask[1];
       lds_words(at + 2 * Cfg::kCodes + 128 * NG, mask);
-      if (mask[0]) {                                  // uniform in the warp
-        const bool live0 = mask[0] >> g & 1, live1 = mask[0] >> (g + 8) & 1;
+      if (mask[0]) {                                  // uniform in the warp, like `full`
+        const bool full = mask[0] == 0xffffu && t0 + 16 <= all_see;       // every query sees every token
         // ---- S^T = K Q^T, log2 domain -------------------------------------------------------------------------------------
         float sc[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[nt][e] = 0.f;
 #pragma unroll
         for (int gg = 0; gg < NG; ++gg) {
           constexpr int W = GROUP / 32;
@@ -393,30 +414,30 @@ attn_int4_kernel(const AttnInt4Params p) {
 #pragma unroll
           for (int x = 0; x < W; ++x) {
             uint32_t u0[4], u1[4];
-            widen4_key<T>(w0[x], u0);
-            widen4_key<T>(w1[x], u1);
+            widen4(w0[x], u0);
+            widen4(w1[x], u1);
             const uint32_t a0[4] = {u0[0], u1[0], u0[1], u1[1]}, a1[4] = {u0[2], u1[2], u0[3], u1[3]};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma16816<T>(d[nt], a0, qf[nt][gg * MG + 2 * x][0], qf[nt][gg * MG + 2 * x][1]);
-              mma16816<T>(d[nt], a1, qf[nt][gg * MG + 2 * x + 1][0], qf[nt][gg * MG + 2 * x + 1][1]);
+              mma16816(d[nt], a0, qf[nt][gg * MG + 2 * x][0], qf[nt][gg * MG + 2 * x][1]);
+              mma16816(d[nt], a1, qf[nt][gg * MG + 2 * x + 1][0], qf[nt][gg * MG + 2 * x + 1][1]);
             }
           }
           uint32_t s0[1], s1[1];
           lds_words(at + 2 * Cfg::kCodes + (g * NG + gg) * 4, s0);
           lds_words(at + 2 * Cfg::kCodes + ((g + 8) * NG + gg) * 4, s1);
           const float2 k0 = widen_scale<T>(s0[0]), k1 = widen_scale<T>(s1[0]);
-          const float a0 = k0.x * p.scale_log2, a1 = k1.x * p.scale_log2;
-          const float b0 = fmaf(-KeyOffset<T>::value, k0.x, k0.y), b1 = fmaf(-KeyOffset<T>::value, k1.x, k1.y);
+          const float a0 = k0.x * to_score, a1 = k1.x * to_score;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              sc[nt][e] += fmaf(a0, d[nt][e], b0 * qsum[gg][nt][e]);
-              sc[nt][2 + e] += fmaf(a1, d[nt][2 + e], b1 * qsum[gg][nt][e]);
+              const float lo0 = k0.y * qsum[gg][nt][e], lo1 = k1.y * qsum[gg][nt][e];
+              sc[nt][e] = fmaf(a0, d[nt][e], gg ? sc[nt][e] + lo0 : lo0);
+              sc[nt][2 + e] = fmaf(a1, d[nt][2 + e], gg ? sc[nt][2 + e] + lo1 : lo1);
             }
         }
-        // ---- the values' steps, and whether the running maximum or the factor f has to move ------------------------------
+        // ---- the values' steps and minima; what is not seen --------------------------------------------------------------
         float2 v0[NG], v1[NG];
         float big = 0.f;
 #pragma unroll
@@ -424,31 +445,46 @@ attn_int4_kernel(const AttnInt4Params p) {
           uint32_t s0[1], s1[1];
           lds_words(at + 2 * Cfg::kCodes + 64 * NG + (g * NG + gg) * 4, s0);
           lds_words(at + 2 * Cfg::kCodes + 64 * NG + ((g + 8) * NG + gg) * 4, s1);
-          v0[gg] = live0 ? widen_scale<T>(s0[0]) : make_float2(0.f, 0.f);        // a stage's rows behind the last token hold anything
-          v1[gg] = live1 ? widen_scale<T>(s1[0]) : make_float2(0.f, 0.f);
-          v0[gg].y = fmaf(8.f, v0[gg].x, v0[gg].y);                              // the middle of the range: codes are widened to c - 8
-          v1[gg].y = fmaf(8.f, v1[gg].x, v1[gg].y);
-          big = fmaxf(big, fmaxf(fabsf(v0[gg].x), fabsf(v1[gg].x)));
+          v0[gg] = widen_scale<T>(s0[0]);
+          v1[gg] = widen_scale<T>(s1[0]);
         }
-        bool see[NT][4];
-        bool grow = big * f > 64.f || (f == 0.f && big > 0.f);
-        const bool tail_tile = t0 + 16 > all_see;     // uniform
+        uint32_t see = 0xffffffffu;                   // bit 4 nt + e: query 2j + (e & 1) sees token g + 8 (e >> 1)
+        if (!full) {
+          const bool live0 = mask[0] >> g & 1, live1 = mask[0] >> (g + 8) & 1;
+          see = 0;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool ok = (e < 2 ? live0 : live1) && t0 + g + (e < 2 ? 0 : 8) < limit[nt][e & 1];
+              sc[nt][e] = ok ? sc[nt][e] : -INFINITY;
+              see |= (ok ? 1u : 0u) << (4 * nt + e);
+            }
+#pragma unroll
+          for (int gg = 0; gg < NG; ++gg) {           // rows behind the last token hold anything
+            v0[gg] = live0 ? v0[gg] : make_float2(0.f, 0.f);
+            v1[gg] = live1 ? v1[gg] : make_float2(0.f, 0.f);
+          }
+        }
+#pragma unroll
+        for (int gg = 0; gg < NG; ++gg) {
+          big = fmaxf(big, fmaxf(fabsf(v0[gg].x), fabsf(v1[gg].x)));
+          v0[gg].y = fmaf(8.f, v0[gg].x, v0[gg].y);   // the middle of the range: the weights' rounding meets c - 8
+          v1[gg].y = fmaf(8.f, v1[gg].x, v1[gg].y);
+        }
+        // ---- whether the running maximum or the factor f has to move -----------------------------------------------------
+        // the maximum may lag by 2^8: p stays below 256, and sums are exact whatever the reference is
+        float over = 0.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            see[nt][e] = e < 2 ? live0 : live1;
-            if (tail_tile) see[nt][e] = see[nt][e] && t0 + g + (e < 2 ? 0 : 8) < limit[nt][e & 1];
-            // the maximum may lag by 2^8: p stays below 256, and sums are exact whatever the reference is
-            grow = grow || (see[nt][e] && sc[nt][e] > m[nt][e & 1] + 8.f);
-          }
-        if (__any_sync(0xffffffffu, grow)) {
+          for (int e = 0; e < 4; ++e) over = fmaxf(over, sc[nt][e] - m[nt][e & 1]);
+        if (__any_sync(0xffffffffu, over > 8.f || big > most)) {
           float top[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              top[nt][e] = fmaxf(see[nt][e] ? sc[nt][e] : -INFINITY, see[nt][2 + e] ? sc[nt][2 + e] : -INFINITY);
+            for (int e = 0; e < 2; ++e) top[nt][e] = fmaxf(sc[nt][e], sc[nt][2 + e]);
 #pragma unroll
           for (int o = 4; o < 32; o *= 2) {
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
@@ -458,38 +494,44 @@ attn_int4_kernel(const AttnInt4Params p) {
               for (int e = 0; e < 2; ++e) top[nt][e] = fmaxf(top[nt][e], __shfl_xor_sync(0xffffffffu, top[nt][e], o));
           }
           float ratio = 1.f;                          // what the factor f changes by
-          if (big * f > 64.f || (f == 0.f && big > 0.f)) {
-            // f = 2^(4 - exponent): the largest step times f lies in [16, 32); exponents of f stay normal
+          if (big > most) {
+            // f = 2^(4 - exponent): the largest step times f lies in [16, 32), and steps up to four times as large need no
+            // change; exponents of f stay normal
             const int ex = max((int)(__float_as_uint(big) >> 23) - 127, -112);
             const float f_new = __uint_as_float((uint32_t)(127 + 4 - min(ex, 127)) << 23);
             ratio = f == 0.f ? 0.f : f_new / f;
             f = f_new;
+            most = 64.f / f_new;                      // infinity at the upper end
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float m_new = fmaxf(m[nt][e], top[nt][e]);
-              const float alpha = m[nt][e] == -INFINITY ? 0.f : ex2_approx(m[nt][e] - m_new);
+              const float m_new = fmaxf(m[nt][e], top[nt][e]), alpha = ex2_approx(m[nt][e] - m_new), both = alpha * ratio;
               m[nt][e] = m_new;
               l[nt][e] *= alpha;
 #pragma unroll
-              for (int gg = 0; gg < NG; ++gg) low[gg][nt][e] *= alpha;
+              for (int gg = 0; gg < NG; ++gg) {
+                low[gg][nt][e] *= alpha;
+                wsum[gg][nt][e] *= both;
+                wsum[gg][nt][2 + e] *= both;
+              }
 #pragma unroll
               for (int t = 0; t < MT; ++t) {
-                acc[t][nt][e] *= alpha * ratio;
-                acc[t][nt][2 + e] *= alpha * ratio;
+                acc[t][nt][e] *= both;
+                acc[t][nt][2 + e] *= both;
               }
             }
         }
-        // ---- p, its sum, the minima's share --------------------------------------------------------------------------------
+        // ---- p and its sum ---------------------------------------------------------------------------------------------------
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            sc[nt][e] = see[nt][e] ? ex2_approx(sc[nt][e] - m[nt][e & 1]) : 0.f;
-            l[nt][e & 1] += sc[nt][e];
-          }
+          for (int e = 0; e < 4; ++e) sc[nt][e] = ex2_approx(sc[nt][e] - m[nt][e & 1]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) l[nt][e] += sc[nt][e] + sc[nt][2 + e];
         // ---- O^T += V^T P^T, group by group ----------------------------------------------------------------------------------
 #pragma unroll
         for (int gg = 0; gg < NG; ++gg) {
@@ -498,19 +540,21 @@ attn_int4_kernel(const AttnInt4Params p) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float w[4] = {sc[nt][0] * f0, sc[nt][1] * f0, sc[nt][2] * f1, sc[nt][3] * f1};
-            if (!tail_tile) {
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                low[gg][nt][e] = fmaf(sc[nt][e], v0[gg].y, fmaf(sc[nt][2 + e], v1[gg].y, low[gg][nt][e]));
-            } else {                                  // a value that a query does not see may be NaN, which 0 does not cancel
+            float lo[4] = {sc[nt][0] * v0[gg].y, sc[nt][1] * v0[gg].y, sc[nt][2] * v1[gg].y, sc[nt][3] * v1[gg].y};
+            if (!full) {                              // a value that a query does not see may be NaN, which 0 does not cancel
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                w[e] = see[nt][e] ? w[e] : 0.f;
-                low[gg][nt][e & 1] += see[nt][e] ? sc[nt][e] * (e < 2 ? v0[gg].y : v1[gg].y) : 0.f;
+                const bool ok = see >> (4 * nt + e) & 1;
+                w[e] = ok ? w[e] : 0.f;
+                lo[e] = ok ? lo[e] : 0.f;
               }
             }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) low[gg][nt][e] += lo[e] + lo[2 + e];
             pb[nt][0] = movmatrix_trans(pack_f16(w[0], w[1]));
             pb[nt][1] = movmatrix_trans(pack_f16(w[2], w[3]));
+            const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+            mma16816(wsum[gg][nt], ones, pb[nt][0], pb[nt][1]);
           }
           // words of tokens 2j, 2j + 1, 2j + 8, 2j + 9: rows j, j + 4, j + 8, j + 12 of the stage
           constexpr int W = GROUP >= 64 ? GROUP / 64 : 1;
@@ -527,14 +571,14 @@ attn_int4_kernel(const AttnInt4Params p) {
             for (int half = 0; half < (GROUP >= 64 ? 2 : 1); ++half) {
               const uint32_t sel = GROUP >= 64 ? (half ? 0x7632u : 0x5410u) : ((g & 1) ? 0x7632u : 0x5410u);
               uint32_t ua[4], ub[4];
-              widen4_f16(__byte_perm(w[0][x], w[1][x], sel), ua);
-              widen4_f16(__byte_perm(w[2][x], w[3][x], sel), ub);
+              widen4(__byte_perm(w[0][x], w[1][x], sel), ua);
+              widen4(__byte_perm(w[2][x], w[3][x], sel), ub);
               const int t = gg * MG + (GROUP >= 64 ? 4 * x + 2 * half : 0);
               const uint32_t a0[4] = {ua[0], ua[1], ub[0], ub[1]}, a1[4] = {ua[2], ua[3], ub[2], ub[3]};
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                mma16816<__half>(acc[t][nt], a0, pb[nt][0], pb[nt][1]);
-                mma16816<__half>(acc[t + 1][nt], a1, pb[nt][0], pb[nt][1]);
+                mma16816(acc[t][nt], a0, pb[nt][0], pb[nt][1]);
+                mma16816(acc[t + 1][nt], a1, pb[nt][0], pb[nt][1]);
               }
             }
         }
@@ -561,6 +605,7 @@ attn_int4_kernel(const AttnInt4Params p) {
         for (int e = 0; e < 2; ++e) join_m[warp * Cfg::kRows + nt * 8 + 2 * j + e] = m[nt][e];
     __syncthreads();
     const float inv_f = f == 0.f ? 0.f : 1.f / f;
+    float part[NT][2];                                // this warp's weight in the joint result
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -569,21 +614,9 @@ attn_int4_kernel(const AttnInt4Params p) {
         float top = join_m[r];
 #pragma unroll
         for (int w = 1; w < kWarps; ++w) top = fmaxf(top, join_m[w * Cfg::kRows + r]);
-        const float a = m[nt][e] == -INFINITY && l[nt][e] == 0.f ? 0.f : ex2_approx(m[nt][e] - top);
-        if (g == 0) join_l[warp * Cfg::kRows + r] = l[nt][e] * a;
-        float* dst = join + (warp * Cfg::kRows + r) * Cfg::kPitch;
-#pragma unroll
-        for (int gg = 0; gg < NG; ++gg)
-#pragma unroll
-          for (int t = 0; t < MG; ++t) {
-            const int d = gg * GROUP + g * (GROUP / 8) + 2 * t;
-            *reinterpret_cast<float2*>(dst + d) = make_float2((acc[gg * MG + t][nt][e] * inv_f + low[gg][nt][e]) * a,
-                                                              (acc[gg * MG + t][nt][2 + e] * inv_f + low[gg][nt][e]) * a);
-          }
+        part[nt][e] = ex2_approx(m[nt][e] - top);
+        if (g == 0) join_l[warp * Cfg::kRows + r] = l[nt][e] * part[nt][e];
       }
-    __syncthreads();
-
-    // ---- the segment's rows: to the output, or to the partial sums --------------------------------------------------------
     const int64_t seg_first = seq_base + ((int64_t)seg.h * p.q_tiles + seg.qt) * seg.units, seg_end = seg_first + seg.units;
     const bool whole = seg_first >= start && seg_end <= end;
     auto store_out = [&](int r, int d, float4 v) {
@@ -595,27 +628,52 @@ attn_int4_kernel(const AttnInt4Params p) {
     };
     constexpr int kSlot = Cfg::kRows * (DIM + 2);      // floats of one partial result: rows, maxima, sums
     float* slot = p.partial + ((int64_t)blockIdx.x * 2 + (seg_first + seg.u > start ? 1 : 0)) * kSlot;
-    for (int i = threadIdx.x; i < rows * (DIM / 4); i += 32 * kWarps) {
-      const int r = i / (DIM / 4), d = i % (DIM / 4) * 4;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      float sum = 0.f, top = join_m[r];
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += Cfg::kJoinRows) {
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float4 a = *reinterpret_cast<const float4*>(join + (w * Cfg::kRows + r) * Cfg::kPitch + d);
-        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
-        sum += join_l[w * Cfg::kRows + r];
-        top = fmaxf(top, join_m[w * Cfg::kRows + r]);
-      }
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        store_out(r, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-      } else {
-        __stcg(reinterpret_cast<float4*>(slot + r * DIM + d), v);
-        if (d == 0) {
-          __stcg(slot + Cfg::kRows * DIM + r, top);
-          __stcg(slot + Cfg::kRows * (DIM + 1) + r, sum);
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = nt * 8 + 2 * j + e - r0;
+          if (r >= 0 && r < Cfg::kJoinRows) {
+            float* dst = join + (warp * Cfg::kJoinRows + r) * Cfg::kPitch;
+#pragma unroll
+            for (int gg = 0; gg < NG; ++gg)
+#pragma unroll
+              for (int t = 0; t < MG; ++t) {
+                const int d = gg * GROUP + g * (GROUP / 8) + 2 * t;
+                const float a0 = fmaf(acc[gg * MG + t][nt][e], 0x1p24f, -8.f * wsum[gg][nt][e]);
+                const float a1 = fmaf(acc[gg * MG + t][nt][2 + e], 0x1p20f, -8.f * wsum[gg][nt][e]);
+                *reinterpret_cast<float2*>(dst + d) =
+                    make_float2(fmaf(a0, inv_f, low[gg][nt][e]) * part[nt][e], fmaf(a1, inv_f, low[gg][nt][e]) * part[nt][e]);
+              }
+          }
+        }
+      __syncthreads();
+      // the segment's rows: to the output, or to the partial sums
+      for (int i = threadIdx.x; i < min(rows - r0, Cfg::kJoinRows) * (DIM / 4); i += 32 * kWarps) {
+        const int rj = i / (DIM / 4), r = r0 + rj, d = i % (DIM / 4) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f, top = join_m[r];
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 a = *reinterpret_cast<const float4*>(join + (w * Cfg::kJoinRows + rj) * Cfg::kPitch + d);
+          v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+          sum += join_l[w * Cfg::kRows + r];
+          top = fmaxf(top, join_m[w * Cfg::kRows + r]);
+        }
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          store_out(r, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        } else {
+          __stcg(reinterpret_cast<float4*>(slot + r * DIM + d), v);
+          if (d == 0) {
+            __stcg(slot + Cfg::kRows * DIM + r, top);
+            __stcg(slot + Cfg::kRows * (DIM + 1) + r, sum);
+          }
         }
       }
+      __syncthreads();                                 // the join buffer is free again
     }
     if (!whole) {
       // CTAs c0 .. c1 share the segment; the last to arrive adds up their partial sums
@@ -634,7 +692,7 @@ attn_int4_kernel(const AttnInt4Params p) {
         };
         for (int i = threadIdx.x; i < rows * (DIM / 4); i += 32 * kWarps) {
           const int r = i / (DIM / 4), d = i % (DIM / 4) * 4;
-          float top = -INFINITY;
+          float top = -FLT_MAX;
           for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(slot_of(c) + Cfg::kRows * DIM + r));
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
           float sum = 0.f;
@@ -642,7 +700,7 @@ attn_int4_kernel(const AttnInt4Params p) {
           for (int c = c0; c <= c1; ++c) {
             const float* s = slot_of(c);
             const float mc = __ldcg(s + Cfg::kRows * DIM + r), lc = __ldcg(s + Cfg::kRows * (DIM + 1) + r);
-            const float a = mc == -INFINITY && lc == 0.f ? 0.f : ex2_approx(mc - top);
+            const float a = ex2_approx(mc - top);
             const float4 x = __ldcg(reinterpret_cast<const float4*>(s + r * DIM + d));
             v.x = fmaf(x.x, a, v.x); v.y = fmaf(x.y, a, v.y); v.z = fmaf(x.z, a, v.z); v.w = fmaf(x.w, a, v.w);
             sum = fmaf(lc, a, sum);
@@ -653,7 +711,7 @@ attn_int4_kernel(const AttnInt4Params p) {
       }
     }
     if (left > 0 && it.b != seg.b) seq_base += (int64_t)seg.units * p.h_kv * p.q_tiles;
-    __syncthreads();                                   // the join buffer is free again
+    __syncthreads();                                   // shared_int and the maxima are free again
   }
   cp_async_wait<0>();
 }
@@ -731,7 +789,8 @@ extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache
   TL_REQUIRE(h_q % h_kv == 0, "attn_decode_paged_int4: h_q must be a multiple of h_kv");
   TL_REQUIRE(batch < (1 << 24) && s_q < (1 << 24) && h_q <= 65536 && batch * s_q * h_q < (1ll << 31),
              "attn_decode_paged_int4: size too large");
-  TL_REQUIRE(num_pages < (1ll << 31) && page_size < (1ll << 31) && num_pages * page_size < (1ll << 31) && max_pages_per_seq < (1ll << 31),
+  TL_REQUIRE(num_pages < (1ll << 31) && page_size < (1ll << 31) && num_pages * page_size < (1ll << 31) && max_pages_per_seq < (1ll << 31) &&
+                 num_pages * page_size * h_kv < (1ll << 32),            // 2^32 rows of 32 bytes and their values are over 256 GB
              "attn_decode_paged_int4: cache too large");
   if (batch == 0 || s_q == 0) return TL_B200_OK;
   const bool keys = num_pages > 0 && max_pages_per_seq > 0;
@@ -746,7 +805,7 @@ extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache
   AttnInt4Params p;
   p.q = q; p.q_sb = q_stride_batch; p.q_ss = q_stride_token;
   p.k_codes = (const uint8_t*)k_cache; p.v_codes = (const uint8_t*)v_cache;
-  p.k_scale = (const uint32_t*)k_scale; p.v_scale = (const uint32_t*)v_scale;
+  p.k_scale = (const uint8_t*)k_scale; p.v_scale = (const uint8_t*)v_scale;
   p.table = block_table; p.lens = cache_seqlens; p.out = out;
   p.batch = (int)batch; p.s_q = (int)s_q; p.h_q = (int)h_q; p.h_kv = (int)h_kv; p.per = (int)(h_q / h_kv);
   p.page_size = (int)page_size; p.max_pages = (int)max_pages_per_seq; p.num_pages = (int)num_pages;
