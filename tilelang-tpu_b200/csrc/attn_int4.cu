@@ -63,10 +63,11 @@ template <int DIM, int GROUP, int NT> struct I4Cfg {
   static constexpr int kPitch = DIM + 4;                                // floats of a row of the join buffer
   static constexpr int kJoin = kWarps * (kJoinRows * kPitch + 2 * kRows) * 4;   // partial rows, maxima and sums of the eight warps
   static constexpr int kCtas = DIM * NT <= 128 ? 2 : 1;                 // resident per SM: registers and shared memory
-  static constexpr int kFit = ((227 * 1024 / kCtas) - 1024 - kJoin - 128) / (kWarps * kStage);
+  static constexpr int kFit = ((227 * 1024 / kCtas) - 1024 - kJoin - 256) / (kWarps * kStage);
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
-  static constexpr int kSmem = kWarps * kStages * kStage + kJoin + 128;
+  static constexpr int kSmem = kWarps * kStages * kStage + kJoin + 256;
   static_assert(kStages >= 3, "ring too short");
+  static_assert(kWarps * kJoinRows * kPitch >= 5 * 32 * kWarps, "the join buffer serves the merge of partial sums too");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -148,12 +149,18 @@ attn_int4_kernel(const AttnInt4Params p) {
   float* join = reinterpret_cast<float*>(tail);                  // [warps][join rows][pitch]
   float* join_m = join + kWarps * Cfg::kJoinRows * Cfg::kPitch;  // [warps][rows]
   float* join_l = join_m + kWarps * Cfg::kRows;
-  int* shared_int = reinterpret_cast<int*>(join_l + kWarps * Cfg::kRows);
+  // what only the ends of segments need stays in shared memory
+  struct Shared {
+    int64_t sums[kWarps];
+    int64_t total, ctas, start, end, seq_base;         // seq_base: first unit of sequence it.b
+    int first_b, last;
+  };
+  Shared& sh = *reinterpret_cast<Shared*>(join_l + kWarps * Cfg::kRows);
   const uint32_t ring = smem_u32(smem) + warp * ST * Cfg::kStage;
 
   // ---- this CTA's range of the list --------------------------------------------------------------------------------
-  int64_t total, ctas, start, end, seq_base;         // seq_base: first unit of sequence it.b
   UnitIter it;
+  int left;                                            // units of this CTA still to do
   {
     const int64_t per_unit = (int64_t)p.h_kv * p.q_tiles;
     const int chunk = (p.batch + 32 * kWarps - 1) / (32 * kWarps);
@@ -166,21 +173,17 @@ attn_int4_kernel(const AttnInt4Params p) {
       const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    int64_t* warp_sum64 = reinterpret_cast<int64_t*>(shared_int);        // 8 sums, then the found position in two more
-    int64_t* found = reinterpret_cast<int64_t*>(join);
-    if (lane == 31) warp_sum64[warp] = incl;
+    if (lane == 31) sh.sums[warp] = incl;
     __syncthreads();
-    int64_t before = 0;
-    total = 0;
+    int64_t before = 0, total = 0;
     for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += warp_sum64[w];
-      total += warp_sum64[w];
+      if (w < warp) before += sh.sums[w];
+      total += sh.sums[w];
     }
     total *= per_unit;
-    ctas = total < gridDim.x ? total : gridDim.x;                        // every one of them has a unit
+    const int64_t ctas = total < gridDim.x ? total : gridDim.x;          // every one of them has a unit
     if (blockIdx.x >= ctas) return;                                      // the whole CTA
-    start = (int64_t)blockIdx.x * total / ctas;
-    end = ((int64_t)blockIdx.x + 1) * total / ctas;
+    const int64_t start = (int64_t)blockIdx.x * total / ctas, end = ((int64_t)blockIdx.x + 1) * total / ctas;
     int64_t base = before + incl - mine;
     if (base * per_unit <= start && start < (base + mine) * per_unit) {  // exactly one thread
       int b = b0, units = 0;
@@ -189,20 +192,23 @@ attn_int4_kernel(const AttnInt4Params p) {
         if (start < (base + units) * per_unit) break;
         base += units;
       }
-      found[0] = b;
-      found[1] = base * per_unit;
+      sh.first_b = b;
+      sh.seq_base = base * per_unit;
+      sh.total = total;
+      sh.ctas = ctas;
+      sh.start = start;
+      sh.end = end;
     }
     __syncthreads();
-    it.b = (int)found[0];
-    seq_base = found[1];
+    left = (int)(end - start);                                           // the host checks that it fits
+    it.b = sh.first_b;
     it.len = mla_len(p.lens, it.b, p.len_cap);
     it.units = units_of(it.len);
-    const int64_t off = start - seq_base;
+    const int64_t off = start - sh.seq_base;
     const int seg = (int)(off / it.units);
     it.u = (int)(off - (int64_t)seg * it.units);
     it.h = seg / p.q_tiles;
     it.qt = seg - it.h * p.q_tiles;
-    __syncthreads();                                                     // `found` lies in the join buffer
   }
 
   // ---- loads: the 16 tokens of a warp in a unit go into a stage; one commit group each, empty ones included -------------
@@ -281,7 +287,7 @@ attn_int4_kernel(const AttnInt4Params p) {
     return tile_in_page && t0 < w.len ? __ldg(p.table + (int64_t)w.b * p.max_pages + p.page_div((uint32_t)t0)) : 0;
   };
 
-  int64_t to_load = end - start, left = to_load;
+  int to_load = left;
   UnitIter ahead = it;
   int next_page = page_at(ahead);
 #pragma unroll 1
@@ -377,9 +383,8 @@ attn_int4_kernel(const AttnInt4Params p) {
         for (int e = 0; e < 4; ++e) acc[t][nt][e] = 0.f;
     }
 
-    const UnitIter seg = it;                          // its u is the first unit of this CTA's share
-    bool more = true;
-    while (more) {
+    const int first_u = it.u;                         // the first unit of this CTA's share of the segment
+    while (true) {
       cp_async_wait<ST - 2>();
       __syncwarp();                                   // every lane's copies have landed, and every lane has left the stage refilled below
       if (to_load > 0) {
@@ -584,7 +589,8 @@ attn_int4_kernel(const AttnInt4Params p) {
         }
       }
       --left;
-      more = !advance(it, p) && left > 0;
+      if (left == 0 || it.u + 1 == it.units) break;
+      ++it.u;
     }
 
     // ---- join the warps ---------------------------------------------------------------------------------------------------
@@ -617,17 +623,17 @@ attn_int4_kernel(const AttnInt4Params p) {
         part[nt][e] = ex2_approx(m[nt][e] - top);
         if (g == 0) join_l[warp * Cfg::kRows + r] = l[nt][e] * part[nt][e];
       }
-    const int64_t seg_first = seq_base + ((int64_t)seg.h * p.q_tiles + seg.qt) * seg.units, seg_end = seg_first + seg.units;
-    const bool whole = seg_first >= start && seg_end <= end;
+    const int64_t seg_first = sh.seq_base + ((int64_t)it.h * p.q_tiles + it.qt) * it.units, seg_end = seg_first + it.units;
+    const bool whole = seg_first >= sh.start && seg_end <= sh.end;
     auto store_out = [&](int r, int d, float4 v) {
-      const int row = seg.qt * Cfg::kRows + r, qi = row / p.per;
-      T* dst = reinterpret_cast<T*>(p.out) + (((int64_t)seg.b * p.s_q + qi) * p.h_q + (int64_t)seg.h * p.per + (row - qi * p.per)) * DIM + d;
+      const int row = it.qt * Cfg::kRows + r, qi = row / p.per;
+      T* dst = reinterpret_cast<T*>(p.out) + (((int64_t)it.b * p.s_q + qi) * p.h_q + (int64_t)it.h * p.per + (row - qi * p.per)) * DIM + d;
       union { uint2 raw; T e[4]; } o;
       o.e[0] = from_f32<T>(v.x); o.e[1] = from_f32<T>(v.y); o.e[2] = from_f32<T>(v.z); o.e[3] = from_f32<T>(v.w);
       *reinterpret_cast<uint2*>(dst) = o.raw;
     };
     constexpr int kSlot = Cfg::kRows * (DIM + 2);      // floats of one partial result: rows, maxima, sums
-    float* slot = p.partial + ((int64_t)blockIdx.x * 2 + (seg_first + seg.u > start ? 1 : 0)) * kSlot;
+    float* slot = p.partial + ((int64_t)blockIdx.x * 2 + (seg_first + first_u > sh.start ? 1 : 0)) * kSlot;
 #pragma unroll 1
     for (int r0 = 0; r0 < rows; r0 += Cfg::kJoinRows) {
 #pragma unroll
@@ -677,41 +683,74 @@ attn_int4_kernel(const AttnInt4Params p) {
     }
     if (!whole) {
       // CTAs c0 .. c1 share the segment; the last to arrive adds up their partial sums
+      const int64_t total = sh.total, ctas = sh.ctas;
       const int c0 = (int)(((seg_first + 1) * ctas - 1) / total), c1 = (int)((seg_end * ctas - 1) / total);
       int* counter = p.counters + c0;                // only one shared segment begins in a CTA's range: its last
       __threadfence();
       __syncthreads();
-      if (threadIdx.x == 0) shared_int[0] = atomicAdd(counter, 1) == c1 - c0;
+      if (threadIdx.x == 0) sh.last = atomicAdd(counter, 1) == c1 - c0;
       __syncthreads();
-      if (shared_int[0]) {
+      if (sh.last) {
         __threadfence();
         if (threadIdx.x == 0) *counter = 0;            // ready for the next call
-        auto slot_of = [&](int c) {                    // a CTA's first segment is in its slot 0, its last in slot 1
-          const int64_t c_start = (int64_t)c * total / ctas;
-          return p.partial + ((int64_t)c * 2 + (seg_first > c_start ? 1 : 0)) * kSlot;
-        };
-        for (int i = threadIdx.x; i < rows * (DIM / 4); i += 32 * kWarps) {
-          const int r = i / (DIM / 4), d = i % (DIM / 4) * 4;
+        // the segment is the last of CTA c0 (slot 1 unless it is its first as well) and the first of all others (slot 0)
+        const float* slots = p.partial + (int64_t)c0 * 2 * kSlot;
+        const int in_c0 = seg_first > (int64_t)c0 * total / ctas ? kSlot : 0, count = c1 - c0 + 1;
+        auto slot_of = [&](int c) { return slots + (c == 0 ? in_c0 : (int64_t)c * 2 * kSlot); };
+        constexpr int kRowThreads = DIM / 4 < 32 ? DIM / 4 : 32;         // neighbouring lanes with one row
+        const int items = rows * (DIM / 4), teams = 32 * kWarps > items ? 32 * kWarps / items : 1;
+        float4* team_v = reinterpret_cast<float4*>(join);               // [teams][items], at most 256
+        float* team_l = join + 4 * 32 * kWarps;
+        for (int i0 = 0; i0 < items; i0 += 32 * kWarps) {                // one round, unless a tile has more than 256 items
+          const int team = items < 32 * kWarps ? threadIdx.x / items : 0, i = items < 32 * kWarps ? threadIdx.x % items : i0 + threadIdx.x;
+          const bool on = team < teams && i < items;
+          const int r = on ? i / (DIM / 4) : 0, d = i % (DIM / 4) * 4;
           float top = -FLT_MAX;
-          for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(slot_of(c) + Cfg::kRows * DIM + r));
+          for (int c = lane % kRowThreads; c < count; c += kRowThreads) top = fmaxf(top, __ldcg(slot_of(c) + Cfg::kRows * DIM + r));
+#pragma unroll
+          for (int o = 1; o < kRowThreads; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
           float sum = 0.f;
-#pragma unroll 4
-          for (int c = c0; c <= c1; ++c) {
-            const float* s = slot_of(c);
-            const float mc = __ldcg(s + Cfg::kRows * DIM + r), lc = __ldcg(s + Cfg::kRows * (DIM + 1) + r);
-            const float a = ex2_approx(mc - top);
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(s + r * DIM + d));
-            v.x = fmaf(x.x, a, v.x); v.y = fmaf(x.y, a, v.y); v.z = fmaf(x.z, a, v.z); v.w = fmaf(x.w, a, v.w);
-            sum = fmaf(lc, a, sum);
+          if (on) {
+#pragma unroll 8
+            for (int c = team; c < count; c += teams) {
+              const float* s = slot_of(c);
+              const float mc = __ldcg(s + Cfg::kRows * DIM + r), lc = __ldcg(s + Cfg::kRows * (DIM + 1) + r);
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(s + r * DIM + d));
+              const float a = ex2_approx(mc - top);
+              v.x = fmaf(x.x, a, v.x); v.y = fmaf(x.y, a, v.y); v.z = fmaf(x.z, a, v.z); v.w = fmaf(x.w, a, v.w);
+              sum = fmaf(lc, a, sum);
+            }
           }
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          store_out(r, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+          if (teams > 1) {                             // in a fixed order
+            if (on) {
+              team_v[team * items + i] = v;
+              team_l[team * items + i] = sum;
+            }
+            __syncthreads();
+            if (on && team == 0)
+              for (int t = 1; t < teams; ++t) {
+                const float4 x = team_v[t * items + i];
+                v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+                sum += team_l[t * items + i];
+              }
+          }
+          if (on && team == 0) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            store_out(r, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+          }
         }
       }
     }
-    if (left > 0 && it.b != seg.b) seq_base += (int64_t)seg.units * p.h_kv * p.q_tiles;
-    __syncthreads();                                   // shared_int and the maxima are free again
+    __syncthreads();                                   // sh, the maxima and the join buffer are free again
+    if (left > 0) {
+      const int b = it.b;
+      const int64_t next = (int64_t)it.units * p.h_kv * p.q_tiles;
+      advance(it, p);
+      if (it.b != b) {                                 // read again only behind the barriers of the next segment's end
+        if (threadIdx.x == 0) sh.seq_base += next;
+      }
+    }
   }
   cp_async_wait<0>();
 }
@@ -814,6 +853,8 @@ extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache
   p.rows = (int)(s_q * (h_q / h_kv)); p.q_tiles = plan.q_tiles;
   p.page_div = FastDiv((uint32_t)page_size);
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  TL_REQUIRE((batch * h_kv * plan.q_tiles) / plan.grid + 1 < (1ll << 31) / (p.len_cap / kUnit + 1),
+             "attn_decode_paged_int4: more units of work than a CTA counts");
   TL_REQUIRE(plan.grid * 4 <= TL_B200_ATTN_INT4_ZERO_BYTES, "attn_decode_paged_int4: more SMs than counters");
   p.counters = (int*)workspace;
   p.partial = (float*)((uint8_t*)workspace + TL_B200_ATTN_INT4_ZERO_BYTES);
