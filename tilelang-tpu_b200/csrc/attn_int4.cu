@@ -24,8 +24,9 @@
 // Every group of columns has its own MMAs, so a group's step can multiply the score or the weight.
 //
 // Work.  Sequences are cut into units of 128 tokens; the list of all (sequence, kv head, query tile, unit) is dealt out in
-// equal contiguous ranges to the CTAs, whatever the lengths.  A warp takes 16 tokens of every unit through its own ring of
-// cp.async stages, which runs ahead across the ends of sequences.  The eight warps' results are joined in shared memory,
+// equal contiguous ranges to the CTAs, whatever the lengths.  A unit is a stage of a ring that bulk copies fill, page by
+// page, across the ends of sequences; the warps take turns to issue them, so that no warp falls behind and none is idle.
+// Each of the eight warps takes 16 tokens of a unit.  Their results are joined in shared memory,
 // a few rows at a time, at the end of a segment; a segment that CTAs share leaves fp32 partial sums, and the CTA that arrives last adds them up in
 // their fixed order, so the result does not depend on who that is.
 #include "sm100.cuh"
@@ -50,34 +51,30 @@ struct AttnInt4Params {
   float scale_log2;
   int* counters;                       // one per CTA, zero between calls
   float* partial;                      // [2 * gridDim.x][kRows * (dim + 2)]
+  int* status;
 };
 
 constexpr int kWarps = 8, kUnit = 16 * kWarps;
 
 template <int DIM, int GROUP, int NT> struct I4Cfg {
   static constexpr int kGroups = DIM / GROUP;
-  static constexpr int kCodes = 16 * DIM / 2;                          // codes of 16 tokens
-  static constexpr int kStage = 2 * kCodes + 2 * 16 * 4 * kGroups + 16; // K, V, their scales, the mask of live tokens
+  static constexpr int kCodes = kUnit * DIM / 2;                        // a stage: codes of K and of V, their scales,
+  static constexpr int kScales = kUnit * 4 * kGroups;                   // a word of 16 live bits per warp
+  static constexpr int kMask = 2 * kCodes + 2 * kScales;
+  static constexpr int kStage = kMask + 4 * kWarps;
   static constexpr int kRows = 8 * NT;
   static constexpr int kJoinRows = 4 * NT;                              // rows joined at a time
   static constexpr int kPitch = DIM + 4;                                // floats of a row of the join buffer
   static constexpr int kJoin = kWarps * (kJoinRows * kPitch + 2 * kRows) * 4;   // partial rows, maxima and sums of the eight warps
   static constexpr int kCtas = DIM * NT <= 128 ? 2 : 1;                 // resident per SM: registers and shared memory
-  static constexpr int kFit = ((227 * 1024 / kCtas) - 1024 - kJoin - 256) / (kWarps * kStage);
+  static constexpr int kFit = ((227 * 1024 / kCtas) - 1024 - kJoin - 384) / kStage;
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
-  static constexpr int kSmem = kWarps * kStages * kStage + kJoin + 256;
-  static_assert(kStages >= 3, "ring too short");
+  static constexpr int kAhead = kStages - 2;                            // units in flight while one is worked on
+  static constexpr int kSmem = kStages * kStage + kJoin + 384;
+  static_assert(kStages >= 3 && kAhead <= kWarps, "ring");
+  static_assert(kStage % 16 == 0, "bulk copies are 16-byte aligned");
   static_assert(kWarps * kJoinRows * kPitch >= 5 * 32 * kWarps, "the join buffer serves the merge of partial sums too");
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-template <int N> __device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <int WORDS> __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[WORDS]) {
   if constexpr (WORDS == 4)
@@ -142,10 +139,9 @@ __global__ void __launch_bounds__(32 * kWarps, I4Cfg<DIM, GROUP, NT>::kCtas)
 attn_int4_kernel(const AttnInt4Params p) {
   using Cfg = I4Cfg<DIM, GROUP, NT>;
   constexpr int NG = Cfg::kGroups, ST = Cfg::kStages, MT = DIM / 16, MG = GROUP / 16;
-  constexpr int kLines = 256 / DIM, kChunks = DIM / 32;          // rows per 128 bytes of shared memory, 16-byte chunks per row
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
-  uint8_t* tail = smem + kWarps * ST * Cfg::kStage;
+  uint8_t* tail = smem + ST * Cfg::kStage;
   float* join = reinterpret_cast<float*>(tail);                  // [warps][join rows][pitch]
   float* join_m = join + kWarps * Cfg::kJoinRows * Cfg::kPitch;  // [warps][rows]
   float* join_l = join_m + kWarps * Cfg::kRows;
@@ -153,10 +149,22 @@ attn_int4_kernel(const AttnInt4Params p) {
   struct Shared {
     int64_t sums[kWarps];
     int64_t total, ctas, start, end, seq_base;         // seq_base: first unit of sequence it.b
-    int first_b, last;
+    uint64_t full[ST], empty[ST];                      // a unit has landed; all warps have left it
+    int first_b, last, abort;
   };
   Shared& sh = *reinterpret_cast<Shared*>(join_l + kWarps * Cfg::kRows);
-  const uint32_t ring = smem_u32(smem) + warp * ST * Cfg::kStage;
+  const uint32_t ring = smem_u32(smem), bar_full = smem_u32(sh.full), bar_empty = smem_u32(sh.empty);
+  // Row r of the 16-row operands is token r ^ (r >> 1 & 1) of the tile: with unswizzled rows of 64 bytes K is then read
+  // without bank conflicts and V with two-way ones.
+  const int tok = g ^ (g >> 1 & 1);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(bar_full + 8 * i, 1);
+      mbar_init(bar_empty + 8 * i, kWarps);
+    }
+    sh.abort = 0;
+    mbar_fence_init();
+  }
 
   // ---- this CTA's range of the list --------------------------------------------------------------------------------
   UnitIter it;
@@ -211,96 +219,98 @@ attn_int4_kernel(const AttnInt4Params p) {
     it.qt = seg - it.h * p.q_tiles;
   }
 
-  // ---- loads: the 16 tokens of a warp in a unit go into a stage; one commit group each, empty ones included -------------
-  const bool tile_in_page = p.page_size % 16 == 0;
-  const uint8_t* k_lane = p.k_codes + lane * 16;                           // the codes of 16 tokens of a page are contiguous
-  const uint8_t* v_lane = p.v_codes + lane * 16;
-  const uint8_t* s_lane = (lane < 16 ? p.k_scale : p.v_scale) + lane % 16 * (4 * NG);
-  uint32_t k_dst[DIM / 64], v_dst[DIM / 64];
-#pragma unroll
-  for (int i = 0; i < DIM / 64; ++i) {
-    const int id = lane + 32 * i, row = id / kChunks, c = id % kChunks;
-    const int kf = (row / kLines * (GROUP / 32)) % kChunks;
-    const int rho = (row >> 1 & 3) | (row & 1) << 2 | (row & 8), vf = (rho / kLines * 2) % kChunks;
-    k_dst[i] = row * (DIM / 2) + (c ^ kf) * 16;
-    v_dst[i] = Cfg::kCodes + rho * (DIM / 2) + (c ^ vf) * 16;
-  }
-  const uint32_t s_dst = 2 * Cfg::kCodes + lane * (4 * NG);
-  auto load_scale = [&](uint32_t at, const uint8_t* from) {
-    if constexpr (NG <= 2) cp_async_small<4 * NG>(at + s_dst, from);
-    else
-#pragma unroll
-      for (int i = 0; i < NG / 4; ++i) cp_async16(at + s_dst + 16 * i, from + 16 * i);
-  };
-  auto load = [&](const UnitIter& w, int stage, int page) {
-    const uint32_t at = ring + stage * Cfg::kStage;
-    const int t0 = w.u * kUnit + warp * 16;
-    uint32_t mask;
-    if (tile_in_page) {
-      const uint32_t off = (uint32_t)t0 - p.page_div((uint32_t)t0) * (uint32_t)p.page_size;
-      const uint32_t row0 = ((uint32_t)page * p.h_kv + w.h) * (uint32_t)p.page_size + off;      // rows of the cache are fewer than 2^32
-      const int live = mla_page_ok(page, p.num_pages) ? min(max(w.len - t0, 0), 16) : 0;
-      mask = (1u << live) - 1u;
-      const uint8_t *k = k_lane + (uint64_t)row0 * (DIM / 2), *v = v_lane + (uint64_t)row0 * (DIM / 2), *sc = s_lane + (uint64_t)row0 * (4 * NG);
-      if (live == 16) {
-#pragma unroll
-        for (int i = 0; i < DIM / 64; ++i) cp_async16(at + k_dst[i], k + 512 * i);
-        load_scale(at, sc);
-#pragma unroll
-        for (int i = 0; i < DIM / 64; ++i) cp_async16(at + v_dst[i], v + 512 * i);
-      } else if (live > 0) {
-#pragma unroll
-        for (int i = 0; i < DIM / 64; ++i)
-          if ((lane + 32 * i) / kChunks < live) {
-            cp_async16(at + k_dst[i], k + 512 * i);
-            cp_async16(at + v_dst[i], v + 512 * i);
+  // ---- loads: one warp fills a stage with a unit, a lane per page ------------------------------------------------------
+  const bool whole_rows = p.page_size % 4 == 0;         // pieces of pages are multiples of four rows: of 16 bytes of scales
+  auto issue = [&](const UnitIter& w, int stage) {
+    const uint32_t at = ring + stage * Cfg::kStage, full = bar_full + 8 * stage;
+    const int t0 = w.u * kUnit, t1 = min(t0 + kUnit, w.len);
+    const int* table = p.table + (int64_t)w.b * p.max_pages;
+    uint32_t* masks = reinterpret_cast<uint32_t*>(smem + stage * Cfg::kStage + Cfg::kMask);
+    if (whole_rows) {
+      const int first = (int)p.page_div((uint32_t)t0);                    // at most 32 pages: they hold four tokens or more
+      const int64_t edge = (int64_t)(first + lane) * p.page_size;         // first token of this lane's page
+      const int begin = (int)max((int64_t)t0, min(edge, (int64_t)t1)), end = (int)min((int64_t)t1, edge + p.page_size);
+      int page = -1;
+      if (begin < end) page = __ldg(table + first + lane);
+      const bool have = begin < end && mla_page_ok(page, p.num_pages);
+      const int rows = have ? (end - begin + 3) / 4 * 4 : 0;              // up to three rows behind the last token, of the same page
+      if (__all_sync(0xffffffffu, have || begin >= end) && t1 == t0 + kUnit) {
+        if (lane < kWarps) masks[lane] = 0xffffu;
+      } else {
+        if (lane < kWarps) masks[lane] = 0;
+        __syncwarp();
+        if (have)
+          for (int i = (begin - t0) / 16; i * 16 < end - t0; ++i) {
+            const int lo = max(begin - t0 - i * 16, 0), hi = min(end - t0 - i * 16, 16);
+            atomicOr(masks + i, (1u << hi) - (1u << lo));
           }
-        if (lane % 16 < live) load_scale(at, sc);
       }
-    } else {                                          // pages end inside the tile: a table entry per token
-      const int my = t0 + lane % 16;
-      bool live = my < w.len;
-      uint32_t row = 0;
-      if (live) {
-        const uint32_t pg = p.page_div((uint32_t)my);
-        const int id = __ldg(p.table + (int64_t)w.b * p.max_pages + pg);
-        live = mla_page_ok(id, p.num_pages);
-        row = ((uint32_t)id * p.h_kv + w.h) * (uint32_t)p.page_size + ((uint32_t)my - pg * (uint32_t)p.page_size);
+      const uint32_t all = __reduce_add_sync(0xffffffffu, (uint32_t)rows);
+      __syncwarp();
+      if (lane == 0) mbar_expect_tx(full, all * (DIM + 8 * NG));
+      __syncwarp();
+      if (have) {
+        // rows of the cache are fewer than 2^32
+        const uint32_t row = ((uint32_t)page * p.h_kv + w.h) * (uint32_t)p.page_size + (uint32_t)(begin - (int)edge);
+        const uint32_t n = (uint32_t)rows, to = (uint32_t)(begin - t0);
+        bulk_load(at + to * (DIM / 2), p.k_codes + (uint64_t)row * (DIM / 2), n * (DIM / 2), full);
+        bulk_load(at + 2 * Cfg::kCodes + to * (4 * NG), p.k_scale + (uint64_t)row * (4 * NG), n * (4 * NG), full);
+        bulk_load(at + Cfg::kCodes + to * (DIM / 2), p.v_codes + (uint64_t)row * (DIM / 2), n * (DIM / 2), full);
+        bulk_load(at + 2 * Cfg::kCodes + Cfg::kScales + to * (4 * NG), p.v_scale + (uint64_t)row * (4 * NG), n * (4 * NG), full);
       }
-      mask = __ballot_sync(0xffffffffu, live) & 0xffffu;
-#pragma unroll
-      for (int i = 0; i < DIM / 64; ++i) {
-        const int r = (lane + 32 * i) / kChunks;      // k_lane points at this lane's chunk of row lane / kChunks
-        const uint32_t from = __shfl_sync(0xffffffffu, row, r);
-        if (mask >> r & 1) {
-          const int64_t o = (int64_t)from * (DIM / 2) - (lane / kChunks) * (DIM / 2);
-          cp_async16(at + k_dst[i], k_lane + o);
-          cp_async16(at + v_dst[i], v_lane + o);
+    } else {                                              // any page size: a lane per token, by plain loads and stores
+      uint8_t* stage_ptr = smem + stage * Cfg::kStage;
+#pragma unroll 1
+      for (int i = 0; i < kUnit / 32; ++i) {
+        const int to = i * 32 + lane, t = t0 + to;
+        bool have = t < t1;
+        uint32_t row = 0;
+        if (have) {
+          const uint32_t pg = p.page_div((uint32_t)t);
+          const int page = __ldg(table + pg);
+          have = mla_page_ok(page, p.num_pages);
+          row = ((uint32_t)page * p.h_kv + w.h) * (uint32_t)p.page_size + ((uint32_t)t - pg * (uint32_t)p.page_size);
+        }
+        const uint32_t mask = __ballot_sync(0xffffffffu, have);
+        if (lane < 2) masks[2 * i + lane] = mask >> (16 * lane) & 0xffffu;
+        if (have) {
+          const uint4 *k = reinterpret_cast<const uint4*>(p.k_codes + (uint64_t)row * (DIM / 2)),
+                      *v = reinterpret_cast<const uint4*>(p.v_codes + (uint64_t)row * (DIM / 2));
+          for (int c = 0; c < DIM / 32; ++c) {
+            reinterpret_cast<uint4*>(stage_ptr + to * (DIM / 2))[c] = __ldg(k + c);
+            reinterpret_cast<uint4*>(stage_ptr + Cfg::kCodes + to * (DIM / 2))[c] = __ldg(v + c);
+          }
+          for (int c = 0; c < NG; ++c) {
+            reinterpret_cast<uint32_t*>(stage_ptr + 2 * Cfg::kCodes)[to * NG + c] = __ldg(reinterpret_cast<const uint32_t*>(p.k_scale) + (uint64_t)row * NG + c);
+            reinterpret_cast<uint32_t*>(stage_ptr + 2 * Cfg::kCodes + Cfg::kScales)[to * NG + c] =
+                __ldg(reinterpret_cast<const uint32_t*>(p.v_scale) + (uint64_t)row * NG + c);
+          }
         }
       }
-      if (live) load_scale(at, s_lane + (int64_t)row * (4 * NG) - lane % 16 * (4 * NG));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full);
     }
-    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 2 * Cfg::kCodes + 128 * NG), "r"(mask) : "memory");   // every lane, the same word
   };
-  auto page_at = [&](const UnitIter& w) {            // page id of the first token of this warp's tile (0 where it has none)
-    const int t0 = w.u * kUnit + warp * 16;
-    return tile_in_page && t0 < w.len ? __ldg(p.table + (int64_t)w.b * p.max_pages + p.page_div((uint32_t)t0)) : 0;
-  };
-
-  int to_load = left;
-  UnitIter ahead = it;
-  int next_page = page_at(ahead);
-#pragma unroll 1
-  for (int s = 0; s < ST - 1; ++s) {
-    if (to_load > 0) {
-      load(ahead, s, next_page);
-      if (--to_load > 0) { advance(ahead, p); next_page = page_at(ahead); }
+  // the unit `by` behind `it`
+  auto ahead_of = [&](UnitIter w, int by) {
+    w.u += by;
+    while (w.u >= w.units) {
+      const int over = w.u - w.units;
+      w.u = w.units - 1;
+      advance(w, p);
+      w.u = over;
     }
-    cp_async_commit();
-  }
+    return w;
+  };
+  volatile int* abort_flag = &sh.abort;
+  const int count = left;
+  if (warp < Cfg::kAhead && warp < count) issue(ahead_of(it, warp), warp);       // the ring is fresh: no wait
 
   // ---- segments -------------------------------------------------------------------------------------------------------
   int stage = 0;
+  uint32_t phase = 0;                                  // of the full barriers
+  int next_stage = Cfg::kAhead, next_phase = 1;        // where the unit kAhead further on goes, and the parity its empty barrier has by then
+  bool ok = true;
   while (left > 0) {
     const int rows = min(Cfg::kRows, p.rows - it.qt * Cfg::kRows);
     // the columns of Q as the B operand: permuted like the columns of the widened keys, times a power of two that brings the
@@ -385,18 +395,18 @@ attn_int4_kernel(const AttnInt4Params p) {
 
     const int first_u = it.u;                         // the first unit of this CTA's share of the segment
     while (true) {
-      cp_async_wait<ST - 2>();
-      __syncwarp();                                   // every lane's copies have landed, and every lane has left the stage refilled below
-      if (to_load > 0) {
-        load(ahead, stage == 0 ? ST - 1 : stage - 1, next_page);
-        if (--to_load > 0) { advance(ahead, p); next_page = page_at(ahead); }
+      if (left > Cfg::kAhead && (count - left + Cfg::kAhead) % kWarps == warp) {          // this warp's turn
+        ok = mbar_wait(bar_empty + 8 * next_stage, next_phase, abort_flag);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        issue(ahead_of(it, Cfg::kAhead), next_stage);
       }
-      cp_async_commit();
-      const uint32_t at = ring + stage * Cfg::kStage;
-      if (++stage == ST) stage = 0;
+      if (++next_stage == ST) { next_stage = 0; next_phase ^= 1; }
+      ok = mbar_wait(bar_full + 8 * stage, phase, abort_flag);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      const uint32_t at = ring + stage * Cfg::kStage + warp * 16 * (DIM / 2), at_scale = ring + stage * Cfg::kStage + 2 * Cfg::kCodes + warp * 16 * (4 * NG);
       const int t0 = it.u * kUnit + warp * 16;
       uint32_t mask[1];
-      lds_words(at + 2 * Cfg::kCodes + 128 * NG, mask);
+      lds_words(ring + stage * Cfg::kStage + Cfg::kMask + 4 * warp, mask);
       if (mask[0]) {                                  // uniform in the warp, like `full`
         const bool full = mask[0] == 0xffffu && t0 + 16 <= all_see;       // every query sees every token
         // ---- S^T = K Q^T, log2 domain -------------------------------------------------------------------------------------
@@ -406,10 +416,9 @@ attn_int4_kernel(const AttnInt4Params p) {
           constexpr int W = GROUP / 32;
           uint32_t w0[W], w1[W];
           {
-            const int b = gg * (GROUP / 2) + j * (GROUP / 8), c = b / 16, in = b % 16;       // byte in the row, chunk, byte in the chunk
-            const int f0 = (g / kLines * (GROUP / 32)) % kChunks, f1 = ((g + 8) / kLines * (GROUP / 32)) % kChunks;
-            lds_words(at + g * (DIM / 2) + (c ^ f0) * 16 + in, w0);
-            lds_words(at + (g + 8) * (DIM / 2) + (c ^ f1) * 16 + in, w1);
+            const int b = gg * (GROUP / 2) + j * (GROUP / 8);
+            lds_words(at + tok * (DIM / 2) + b, w0);
+            lds_words(at + (tok + 8) * (DIM / 2) + b, w1);
           }
           float d[NT][4];
 #pragma unroll
@@ -429,8 +438,8 @@ attn_int4_kernel(const AttnInt4Params p) {
             }
           }
           uint32_t s0[1], s1[1];
-          lds_words(at + 2 * Cfg::kCodes + (g * NG + gg) * 4, s0);
-          lds_words(at + 2 * Cfg::kCodes + ((g + 8) * NG + gg) * 4, s1);
+          lds_words(at_scale + (tok * NG + gg) * 4, s0);
+          lds_words(at_scale + ((tok + 8) * NG + gg) * 4, s1);
           const float2 k0 = widen_scale<T>(s0[0]), k1 = widen_scale<T>(s1[0]);
           const float a0 = k0.x * to_score, a1 = k1.x * to_score;
 #pragma unroll
@@ -448,20 +457,20 @@ attn_int4_kernel(const AttnInt4Params p) {
 #pragma unroll
         for (int gg = 0; gg < NG; ++gg) {
           uint32_t s0[1], s1[1];
-          lds_words(at + 2 * Cfg::kCodes + 64 * NG + (g * NG + gg) * 4, s0);
-          lds_words(at + 2 * Cfg::kCodes + 64 * NG + ((g + 8) * NG + gg) * 4, s1);
+          lds_words(at_scale + Cfg::kScales + (tok * NG + gg) * 4, s0);
+          lds_words(at_scale + Cfg::kScales + ((tok + 8) * NG + gg) * 4, s1);
           v0[gg] = widen_scale<T>(s0[0]);
           v1[gg] = widen_scale<T>(s1[0]);
         }
-        uint32_t see = 0xffffffffu;                   // bit 4 nt + e: query 2j + (e & 1) sees token g + 8 (e >> 1)
+        uint32_t see = 0xffffffffu;                   // bit 4 nt + e: query 2j + (e & 1) sees token tok + 8 (e >> 1)
         if (!full) {
-          const bool live0 = mask[0] >> g & 1, live1 = mask[0] >> (g + 8) & 1;
+          const bool live0 = mask[0] >> tok & 1, live1 = mask[0] >> (tok + 8) & 1;
           see = 0;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const bool ok = (e < 2 ? live0 : live1) && t0 + g + (e < 2 ? 0 : 8) < limit[nt][e & 1];
+              const bool ok = (e < 2 ? live0 : live1) && t0 + tok + (e < 2 ? 0 : 8) < limit[nt][e & 1];
               sc[nt][e] = ok ? sc[nt][e] : -INFINITY;
               see |= (ok ? 1u : 0u) << (4 * nt + e);
             }
@@ -561,14 +570,13 @@ attn_int4_kernel(const AttnInt4Params p) {
             const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
             mma16816(wsum[gg][nt], ones, pb[nt][0], pb[nt][1]);
           }
-          // words of tokens 2j, 2j + 1, 2j + 8, 2j + 9: rows j, j + 4, j + 8, j + 12 of the stage
+          // words of the tokens of operand rows 2j, 2j + 1, 2j + 8, 2j + 9
           constexpr int W = GROUP >= 64 ? GROUP / 64 : 1;
           uint32_t w[4][W];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int rho = j + 4 * i, vf = (rho / kLines * 2) % kChunks;
-            const int b = gg * (GROUP / 2) + (GROUP >= 64 ? g * (GROUP / 16) : (g >> 1) * 4), c = b / 16, in = b % 16;
-            lds_words(at + Cfg::kCodes + rho * (DIM / 2) + (c ^ vf) * 16 + in, w[i]);
+            const int row = ((2 * j + (i & 1)) ^ (j & 1)) + 8 * (i >> 1);
+            lds_words(at + Cfg::kCodes + row * (DIM / 2) + gg * (GROUP / 2) + (GROUP >= 64 ? g * (GROUP / 16) : (g >> 1) * 4), w[i]);
           }
 #pragma unroll
           for (int x = 0; x < W; ++x)
@@ -588,9 +596,18 @@ attn_int4_kernel(const AttnInt4Params p) {
             }
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_empty + 8 * stage);
+      if (++stage == ST) { stage = 0; phase ^= 1; }
       --left;
       if (left == 0 || it.u + 1 == it.units) break;
       ++it.u;
+    }
+    if (!ok) {
+      // a wait gave up: let the copies in flight land before the shared memory is released, report, leave
+      for (int i = 0; i < 64; ++i) __nanosleep(20000);
+      if (lane == 0 && p.status) *p.status = *abort_flag;
+      return;
     }
 
     // ---- join the warps ---------------------------------------------------------------------------------------------------
@@ -752,7 +769,6 @@ attn_int4_kernel(const AttnInt4Params p) {
       }
     }
   }
-  cp_async_wait<0>();
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
@@ -853,6 +869,7 @@ extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache
   p.rows = (int)(s_q * (h_q / h_kv)); p.q_tiles = plan.q_tiles;
   p.page_div = FastDiv((uint32_t)page_size);
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.status = device_status_word();
   TL_REQUIRE((batch * h_kv * plan.q_tiles) / plan.grid + 1 < (1ll << 31) / (p.len_cap / kUnit + 1),
              "attn_decode_paged_int4: more units of work than a CTA counts");
   TL_REQUIRE(plan.grid * 4 <= TL_B200_ATTN_INT4_ZERO_BYTES, "attn_decode_paged_int4: more SMs than counters");
