@@ -76,23 +76,26 @@ template <int DIM, int GROUP, int NT> struct I4Cfg {
   static_assert(kWarps * kJoinRows * kPitch >= 5 * 32 * kWarps, "the join buffer serves the merge of partial sums too");
 };
 
-template <int WORDS> __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[WORDS]) {
-  if constexpr (WORDS == 4)
-    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
-  else if constexpr (WORDS == 2)
-    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
-  else
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
+// Plain loads and non-volatile MMAs: the compiler may move them (never across the barriers, which clobber memory).
+template <int WORDS> __device__ __forceinline__ void lds_words(const uint8_t* at, uint32_t (&w)[WORDS]) {
+  if constexpr (WORDS == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(at);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (WORDS == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(at);
+  }
 }
-
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 // Four nibbles of each half of `r` as fp16 pairs: c, 16 c, c, 16 c, each times 2^-24 (subnormal, exact).
@@ -403,10 +406,11 @@ attn_int4_kernel(const AttnInt4Params p) {
       if (++next_stage == ST) { next_stage = 0; next_phase ^= 1; }
       ok = mbar_wait(bar_full + 8 * stage, phase, abort_flag);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
-      const uint32_t at = ring + stage * Cfg::kStage + warp * 16 * (DIM / 2), at_scale = ring + stage * Cfg::kStage + 2 * Cfg::kCodes + warp * 16 * (4 * NG);
+      const uint8_t* at = smem + stage * Cfg::kStage + warp * 16 * (DIM / 2);
+      const uint8_t* at_scale = smem + stage * Cfg::kStage + 2 * Cfg::kCodes + warp * 16 * (4 * NG);
       const int t0 = it.u * kUnit + warp * 16;
       uint32_t mask[1];
-      lds_words(ring + stage * Cfg::kStage + Cfg::kMask + 4 * warp, mask);
+      lds_words(smem + stage * Cfg::kStage + Cfg::kMask + 4 * warp, mask);
       if (mask[0]) {                                  // uniform in the warp, like `full`
         const bool full = mask[0] == 0xffffu && t0 + 16 <= all_see;       // every query sees every token
         // ---- S^T = K Q^T, log2 domain -------------------------------------------------------------------------------------
@@ -488,11 +492,14 @@ attn_int4_kernel(const AttnInt4Params p) {
         }
         // ---- whether the running maximum or the factor f has to move -----------------------------------------------------
         // the maximum may lag by 2^8: p stays below 256, and sums are exact whatever the reference is
-        float over = 0.f;
+        float over = 0.f, rel[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) over = fmaxf(over, sc[nt][e] - m[nt][e & 1]);
+          for (int e = 0; e < 4; ++e) {
+            rel[nt][e] = sc[nt][e] - m[nt][e & 1];
+            over = fmaxf(over, rel[nt][e]);
+          }
         if (__any_sync(0xffffffffu, over > 8.f || big > most)) {
           float top[NT][2];
 #pragma unroll
@@ -535,13 +542,15 @@ attn_int4_kernel(const AttnInt4Params p) {
                 acc[t][nt][e] *= both;
                 acc[t][nt][2 + e] *= both;
               }
+              rel[nt][e] = sc[nt][e] - m_new;
+              rel[nt][2 + e] = sc[nt][2 + e] - m_new;
             }
         }
         // ---- p and its sum ---------------------------------------------------------------------------------------------------
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[nt][e] = ex2_approx(sc[nt][e] - m[nt][e & 1]);
+          for (int e = 0; e < 4; ++e) sc[nt][e] = ex2_approx(rel[nt][e]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -554,17 +563,17 @@ attn_int4_kernel(const AttnInt4Params p) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float w[4] = {sc[nt][0] * f0, sc[nt][1] * f0, sc[nt][2] * f1, sc[nt][3] * f1};
-            float lo[4] = {sc[nt][0] * v0[gg].y, sc[nt][1] * v0[gg].y, sc[nt][2] * v1[gg].y, sc[nt][3] * v1[gg].y};
-            if (!full) {                              // a value that a query does not see may be NaN, which 0 does not cancel
+            if (full) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) low[gg][nt][e] = fmaf(sc[nt][e], v0[gg].y, fmaf(sc[nt][2 + e], v1[gg].y, low[gg][nt][e]));
+            } else {                                  // a value that a query does not see may be NaN, which 0 does not cancel
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const bool ok = see >> (4 * nt + e) & 1;
                 w[e] = ok ? w[e] : 0.f;
-                lo[e] = ok ? lo[e] : 0.f;
+                low[gg][nt][e & 1] += ok ? sc[nt][e] * (e < 2 ? v0[gg].y : v1[gg].y) : 0.f;
               }
             }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) low[gg][nt][e] += lo[e] + lo[2 + e];
             pb[nt][0] = movmatrix_trans(pack_f16(w[0], w[1]));
             pb[nt][1] = movmatrix_trans(pack_f16(w[2], w[3]));
             const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
