@@ -19,14 +19,17 @@
 //   * V: a register of the A operand is one column of two neighbouring tokens: one byte permute joins half words of the two.
 //   * Steps and minima never touch the codes:  q . k = s (q . c) + lo sum(q) per group, and the value's step multiplies p
 //     (rounded to fp16 with a power-of-two factor per warp that keeps p s in range: 2^-12 of each weight), its minimum
-//     adds p lo in fp32.  The weights' rounding should meet c - 8, not c, so 8 times the sum of the ROUNDED weights, from an
-//     MMA with ones, is taken off, and 8 s goes to the minimum.
+//     adds p lo in fp32.  For fp16 outputs the weights' rounding should meet c - 8, not c: 8 times the sum of the ROUNDED
+//     weights, from an MMA with ones, is taken off, and 8 s goes to the minimum (error against 64 bits 2.5e-4 of the
+//     output, 3.4e-4 without; of a bf16 output it is a fiftieth of the rounding either way, so there it is left out).
 // Every group of columns has its own MMAs, so a group's step can multiply the score or the weight.
 //
-// Work.  Sequences are cut into units of 128 tokens; the list of all (sequence, kv head, query tile, unit) is dealt out in
-// equal contiguous ranges to the CTAs, whatever the lengths.  A unit is a stage of a ring that bulk copies fill, page by
-// page, across the ends of sequences; the warps take turns to issue them, so that no warp falls behind and none is idle.
-// Each of the eight warps takes 16 tokens of a unit.  Their results are joined in shared memory,
+// Work.  Sequences are cut into units of 64 tokens; the list of all (sequence, kv head, query tile, unit) is dealt out in
+// equal contiguous ranges to the CTAs, whatever the lengths.  Each of the four warps takes 16 tokens of a unit, through a
+// ring of cp.async stages of its own that runs ahead across the ends of sequences: no warp waits for another inside a
+// segment (a ring of bulk copies shared by the warps was 40% slower: whoever refills a stage waits for the slowest).  Two
+// units at a time halve what control costs a token and give a warp two chains of MMAs to interleave; four such small CTAs
+// per SM cover each other's ends.  The warps' results are joined in shared memory,
 // a few rows at a time, at the end of a segment; a segment that CTAs share leaves fp32 partial sums, and the CTA that arrives last adds them up in
 // their fixed order, so the result does not depend on who that is.
 #include "sm100.cuh"
@@ -51,30 +54,35 @@ struct AttnInt4Params {
   float scale_log2;
   int* counters;                       // one per CTA, zero between calls
   float* partial;                      // [2 * gridDim.x][kRows * (dim + 2)]
-  int* status;
 };
 
-constexpr int kWarps = 8, kUnit = 16 * kWarps;
+constexpr int kWarps = 4, kUnit = 16 * kWarps;
 
 template <int DIM, int GROUP, int NT> struct I4Cfg {
   static constexpr int kGroups = DIM / GROUP;
-  static constexpr int kCodes = kUnit * DIM / 2;                        // a stage: codes of K and of V, their scales,
-  static constexpr int kScales = kUnit * 4 * kGroups;                   // a word of 16 live bits per warp
+  static constexpr int kCodes = 16 * DIM / 2;                           // a stage, 16 tokens: codes of K and of V, their scales,
+  static constexpr int kScales = 16 * 4 * kGroups;                      // a word of 16 live bits
   static constexpr int kMask = 2 * kCodes + 2 * kScales;
-  static constexpr int kStage = kMask + 4 * kWarps;
+  static constexpr int kStage = kMask + 16;
   static constexpr int kRows = 8 * NT;
-  static constexpr int kJoinRows = 4 * NT;                              // rows joined at a time
-  static constexpr int kPitch = DIM + 4;                                // floats of a row of the join buffer
-  static constexpr int kJoin = kWarps * (kJoinRows * kPitch + 2 * kRows) * 4;   // partial rows, maxima and sums of the eight warps
-  static constexpr int kCtas = DIM * NT <= 128 ? 2 : 1;                 // resident per SM: registers and shared memory
-  static constexpr int kFit = ((227 * 1024 / kCtas) - 1024 - kJoin - 384) / kStage;
-  static constexpr int kStages = kFit > 6 ? 6 : kFit;
-  static constexpr int kAhead = kStages - 2;                            // units in flight while one is worked on
-  static constexpr int kSmem = kStages * kStage + kJoin + 384;
-  static_assert(kStages >= 3 && kAhead <= kWarps, "ring");
-  static_assert(kStage % 16 == 0, "bulk copies are 16-byte aligned");
-  static_assert(kWarps * kJoinRows * kPitch >= 5 * 32 * kWarps, "the join buffer serves the merge of partial sums too");
+  static constexpr int kJoinRows = (DIM == 64 ? 4 : 2) * NT;            // rows joined at a time
+  static constexpr int kJoin = kWarps * (kJoinRows * DIM + 2 * kRows) * 4;      // partial rows, maxima and sums of the warps
+  static constexpr int kCtas = DIM * NT <= 128 ? 4 : 2;                 // resident per SM: registers and shared memory
+  static constexpr int kFit = (228 * 1024 / kCtas - 1024 - kJoin - 128) / (kWarps * kStage);
+  static constexpr int kStages = kFit > 8 ? 8 : kFit;
+  static constexpr int kSmem = kWarps * kStages * kStage + kJoin + 128;
+  static_assert(kStages >= 4, "two stages are worked on while two are on their way");
+  static_assert(kWarps * kJoinRows * DIM >= 5 * 32 * kWarps, "the join buffer serves the merge of partial sums too");
 };
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+template <int N> __device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Plain loads and non-volatile MMAs: the compiler may move them (never across the barriers, which clobber memory).
 template <int WORDS> __device__ __forceinline__ void lds_words(const uint8_t* at, uint32_t (&w)[WORDS]) {
@@ -92,6 +100,11 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {   // onto zeros
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
   uint32_t r;
@@ -142,32 +155,21 @@ __global__ void __launch_bounds__(32 * kWarps, I4Cfg<DIM, GROUP, NT>::kCtas)
 attn_int4_kernel(const AttnInt4Params p) {
   using Cfg = I4Cfg<DIM, GROUP, NT>;
   constexpr int NG = Cfg::kGroups, ST = Cfg::kStages, MT = DIM / 16, MG = GROUP / 16;
+  constexpr bool kCentre = std::is_same<T, __half>::value;       // the weights' rounding meets c - 8 (see above); bf16 outputs do not show it
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
-  uint8_t* tail = smem + ST * Cfg::kStage;
+  uint8_t* tail = smem + kWarps * ST * Cfg::kStage;
   float* join = reinterpret_cast<float*>(tail);                  // [warps][join rows][pitch]
-  float* join_m = join + kWarps * Cfg::kJoinRows * Cfg::kPitch;  // [warps][rows]
+  float* join_m = join + kWarps * Cfg::kJoinRows * DIM;  // [warps][rows]
   float* join_l = join_m + kWarps * Cfg::kRows;
   // what only the ends of segments need stays in shared memory
   struct Shared {
     int64_t sums[kWarps];
     int64_t total, ctas, start, end, seq_base;         // seq_base: first unit of sequence it.b
-    uint64_t full[ST], empty[ST];                      // a unit has landed; all warps have left it
-    int first_b, last, abort;
+    int first_b, last;
   };
   Shared& sh = *reinterpret_cast<Shared*>(join_l + kWarps * Cfg::kRows);
-  const uint32_t ring = smem_u32(smem), bar_full = smem_u32(sh.full), bar_empty = smem_u32(sh.empty);
-  // Row r of the 16-row operands is token r ^ (r >> 1 & 1) of the tile: with unswizzled rows of 64 bytes K is then read
-  // without bank conflicts and V with two-way ones.
-  const int tok = g ^ (g >> 1 & 1);
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < ST; ++i) {
-      mbar_init(bar_full + 8 * i, 1);
-      mbar_init(bar_empty + 8 * i, kWarps);
-    }
-    sh.abort = 0;
-    mbar_fence_init();
-  }
+  uint8_t* const ring = smem + warp * ST * Cfg::kStage;                    // this warp's stages
 
   // ---- this CTA's range of the list --------------------------------------------------------------------------------
   UnitIter it;
@@ -222,77 +224,93 @@ attn_int4_kernel(const AttnInt4Params p) {
     it.qt = seg - it.h * p.q_tiles;
   }
 
-  // ---- loads: one warp fills a stage with a unit, a lane per page ------------------------------------------------------
-  const bool whole_rows = p.page_size % 4 == 0;         // pieces of pages are multiples of four rows: of 16 bytes of scales
-  auto issue = [&](const UnitIter& w, int stage) {
-    const uint32_t at = ring + stage * Cfg::kStage, full = bar_full + 8 * stage;
-    const int t0 = w.u * kUnit, t1 = min(t0 + kUnit, w.len);
+  // ---- loads: the 16 tokens of a warp in a unit go into a stage; one commit group each, empty ones included -------------
+  constexpr int kLines = 256 / DIM, kChunks = DIM / 32;                     // rows per 128 bytes of shared memory, 16-byte chunks per row
+  const bool tile_in_page = p.page_size % 16 == 0;
+  const uint8_t* k_lane = p.k_codes + lane * 16;                            // the codes of 16 tokens of a page are contiguous
+  const uint8_t* v_lane = p.v_codes + lane * 16;
+  const uint8_t* s_lane = (lane < 16 ? p.k_scale : p.v_scale) + lane % 16 * (4 * NG);
+  // Rows of a stage are swizzled by 16-byte chunks, K in the tokens' order and V with tokens 2j, 2j + 1, 2j + 8, 2j + 9 in
+  // rows j, j + 4, j + 8, j + 12, so that neither operand's reads conflict.
+  auto k_place = [&](int row, int c) { return row * (DIM / 2) + (c ^ (row / kLines * (GROUP / 32)) % kChunks) * 16; };
+  auto v_place = [&](int rho, int c) { return Cfg::kCodes + rho * (DIM / 2) + (c ^ (rho / kLines * 2) % kChunks) * 16; };
+  uint32_t k_dst[DIM / 64], v_dst[DIM / 64];          // where chunk lane + 32 i of a tile goes
+#pragma unroll
+  for (int i = 0; i < DIM / 64; ++i) {
+    const int row = (lane + 32 * i) / kChunks, c = lane % kChunks;
+    k_dst[i] = k_place(row, c);
+    v_dst[i] = v_place((row >> 1 & 3) | (row & 1) << 2 | (row & 8), c);
+    asm("" : "+r"(k_dst[i]), "+r"(v_dst[i]));         // kept, not computed again for every tile
+  }
+  auto copy_scales = [&](uint32_t at, const uint8_t* from) {
+    const uint32_t to = at + 2 * Cfg::kCodes + lane * (4 * NG);
+    if constexpr (NG <= 2) cp_async_small<4 * NG>(to, from);
+    else
+#pragma unroll
+      for (int i = 0; i < NG / 4; ++i) cp_async16(to + 16 * i, from + 16 * i);
+  };
+  // a tile that lies in one page and is all there: `row0` is its first row of the cache
+  auto load_whole = [&](int stage, uint32_t row0) {
+    uint8_t* const stage_ptr = ring + stage * Cfg::kStage;
+    const uint32_t at = smem_u32(stage_ptr);
+    const uint8_t *k = k_lane + (uint64_t)row0 * (DIM / 2), *v = v_lane + (uint64_t)row0 * (DIM / 2);
+#pragma unroll
+    for (int i = 0; i < DIM / 64; ++i) cp_async16(at + k_dst[i], k + 512 * i);
+    copy_scales(at, s_lane + (uint64_t)row0 * (4 * NG));
+#pragma unroll
+    for (int i = 0; i < DIM / 64; ++i) cp_async16(at + v_dst[i], v + 512 * i);
+    *reinterpret_cast<uint32_t*>(stage_ptr + Cfg::kMask) = 0xffffu;          // every lane, the same word
+  };
+  auto row_of = [&](int page, int h, int t0) {        // rows of the cache are fewer than 2^32
+    const uint32_t off = (uint32_t)t0 - p.page_div((uint32_t)t0) * (uint32_t)p.page_size;
+    return ((uint32_t)page * p.h_kv + h) * (uint32_t)p.page_size + off;
+  };
+  auto load = [&](const UnitIter& w, int stage) {
+    uint8_t* const stage_ptr = ring + stage * Cfg::kStage;
+    const uint32_t at = smem_u32(stage_ptr);
+    const int t0 = w.u * kUnit + warp * 16;
     const int* table = p.table + (int64_t)w.b * p.max_pages;
-    uint32_t* masks = reinterpret_cast<uint32_t*>(smem + stage * Cfg::kStage + Cfg::kMask);
-    if (whole_rows) {
-      const int first = (int)p.page_div((uint32_t)t0);                    // at most 32 pages: they hold four tokens or more
-      const int64_t edge = (int64_t)(first + lane) * p.page_size;         // first token of this lane's page
-      const int begin = (int)max((int64_t)t0, min(edge, (int64_t)t1)), end = (int)min((int64_t)t1, edge + p.page_size);
-      int page = -1;
-      if (begin < end) page = __ldg(table + first + lane);
-      const bool have = begin < end && mla_page_ok(page, p.num_pages);
-      const int rows = have ? (end - begin + 3) / 4 * 4 : 0;              // up to three rows behind the last token, of the same page
-      if (__all_sync(0xffffffffu, have || begin >= end) && t1 == t0 + kUnit) {
-        if (lane < kWarps) masks[lane] = 0xffffu;
-      } else {
-        if (lane < kWarps) masks[lane] = 0;
-        __syncwarp();
-        if (have)
-          for (int i = (begin - t0) / 16; i * 16 < end - t0; ++i) {
-            const int lo = max(begin - t0 - i * 16, 0), hi = min(end - t0 - i * 16, 16);
-            atomicOr(masks + i, (1u << hi) - (1u << lo));
-          }
+    uint32_t mask = 0;
+    if (tile_in_page) {
+      const int page = t0 < w.len ? __ldg(table + p.page_div((uint32_t)t0)) : -1;
+      const int live = mla_page_ok(page, p.num_pages) ? min(w.len - t0, 16) : 0;
+      const uint32_t row0 = row_of(page, w.h, t0);
+      if (live == 16) {
+        load_whole(stage, row0);
+        return;
       }
-      const uint32_t all = __reduce_add_sync(0xffffffffu, (uint32_t)rows);
-      __syncwarp();
-      if (lane == 0) mbar_expect_tx(full, all * (DIM + 8 * NG));
-      __syncwarp();
-      if (have) {
-        // rows of the cache are fewer than 2^32
-        const uint32_t row = ((uint32_t)page * p.h_kv + w.h) * (uint32_t)p.page_size + (uint32_t)(begin - (int)edge);
-        const uint32_t n = (uint32_t)rows, to = (uint32_t)(begin - t0);
-        bulk_load(at + to * (DIM / 2), p.k_codes + (uint64_t)row * (DIM / 2), n * (DIM / 2), full);
-        bulk_load(at + 2 * Cfg::kCodes + to * (4 * NG), p.k_scale + (uint64_t)row * (4 * NG), n * (4 * NG), full);
-        bulk_load(at + Cfg::kCodes + to * (DIM / 2), p.v_codes + (uint64_t)row * (DIM / 2), n * (DIM / 2), full);
-        bulk_load(at + 2 * Cfg::kCodes + Cfg::kScales + to * (4 * NG), p.v_scale + (uint64_t)row * (4 * NG), n * (4 * NG), full);
-      }
-    } else {                                              // any page size: a lane per token, by plain loads and stores
-      uint8_t* stage_ptr = smem + stage * Cfg::kStage;
-#pragma unroll 1
-      for (int i = 0; i < kUnit / 32; ++i) {
-        const int to = i * 32 + lane, t = t0 + to;
-        bool have = t < t1;
-        uint32_t row = 0;
-        if (have) {
-          const uint32_t pg = p.page_div((uint32_t)t);
-          const int page = __ldg(table + pg);
-          have = mla_page_ok(page, p.num_pages);
-          row = ((uint32_t)page * p.h_kv + w.h) * (uint32_t)p.page_size + ((uint32_t)t - pg * (uint32_t)p.page_size);
+      mask = (1u << live) - 1u;
+      const uint8_t *k = k_lane + (uint64_t)row0 * (DIM / 2), *v = v_lane + (uint64_t)row0 * (DIM / 2);
+#pragma unroll
+      for (int i = 0; i < DIM / 64; ++i)
+        if ((lane + 32 * i) / kChunks < live) {
+          cp_async16(at + k_dst[i], k + 512 * i);
+          cp_async16(at + v_dst[i], v + 512 * i);
         }
-        const uint32_t mask = __ballot_sync(0xffffffffu, have);
-        if (lane < 2) masks[2 * i + lane] = mask >> (16 * lane) & 0xffffu;
-        if (have) {
-          const uint4 *k = reinterpret_cast<const uint4*>(p.k_codes + (uint64_t)row * (DIM / 2)),
-                      *v = reinterpret_cast<const uint4*>(p.v_codes + (uint64_t)row * (DIM / 2));
-          for (int c = 0; c < DIM / 32; ++c) {
-            reinterpret_cast<uint4*>(stage_ptr + to * (DIM / 2))[c] = __ldg(k + c);
-            reinterpret_cast<uint4*>(stage_ptr + Cfg::kCodes + to * (DIM / 2))[c] = __ldg(v + c);
-          }
-          for (int c = 0; c < NG; ++c) {
-            reinterpret_cast<uint32_t*>(stage_ptr + 2 * Cfg::kCodes)[to * NG + c] = __ldg(reinterpret_cast<const uint32_t*>(p.k_scale) + (uint64_t)row * NG + c);
-            reinterpret_cast<uint32_t*>(stage_ptr + 2 * Cfg::kCodes + Cfg::kScales)[to * NG + c] =
-                __ldg(reinterpret_cast<const uint32_t*>(p.v_scale) + (uint64_t)row * NG + c);
-          }
+      if (lane % 16 < live) copy_scales(at, s_lane + (uint64_t)row0 * (4 * NG));
+    } else {                                          // pages end inside the tile: a table entry per token
+      const int my = t0 + lane % 16;
+      bool live = my < w.len;
+      uint32_t row = 0;
+      if (live) {
+        const int id = __ldg(table + p.page_div((uint32_t)my));
+        live = mla_page_ok(id, p.num_pages);
+        row = row_of(id, w.h, my);
+      }
+      mask = __ballot_sync(0xffffffffu, live) & 0xffffu;
+#pragma unroll
+      for (int i = 0; i < DIM / 64; ++i) {
+        const int r = (lane + 32 * i) / kChunks;      // k_lane points at this lane's chunk of row lane / kChunks
+        const uint32_t from = __shfl_sync(0xffffffffu, row, r);
+        const int64_t o = (int64_t)from * (DIM / 2) - (lane / kChunks) * (DIM / 2);
+        if (mask >> r & 1) {
+          cp_async16(at + k_dst[i], k_lane + o);
+          cp_async16(at + v_dst[i], v_lane + o);
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(full);
+      if (live) copy_scales(at, s_lane + (int64_t)row * (4 * NG) - lane % 16 * (4 * NG));
     }
+    *reinterpret_cast<uint32_t*>(stage_ptr + Cfg::kMask) = mask;             // every lane, the same word
   };
   // the unit `by` behind `it`
   auto ahead_of = [&](UnitIter w, int by) {
@@ -305,15 +323,14 @@ attn_int4_kernel(const AttnInt4Params p) {
     }
     return w;
   };
-  volatile int* abort_flag = &sh.abort;
-  const int count = left;
-  if (warp < Cfg::kAhead && warp < count) issue(ahead_of(it, warp), warp);       // the ring is fresh: no wait
+#pragma unroll 1
+  for (int k = 0; k < ST; ++k) {
+    if (k < left) load(ahead_of(it, k), k);
+    cp_async_commit();
+  }
 
   // ---- segments -------------------------------------------------------------------------------------------------------
   int stage = 0;
-  uint32_t phase = 0;                                  // of the full barriers
-  int next_stage = Cfg::kAhead, next_phase = 1;        // where the unit kAhead further on goes, and the parity its empty barrier has by then
-  bool ok = true;
   while (left > 0) {
     const int rows = min(Cfg::kRows, p.rows - it.qt * Cfg::kRows);
     // the columns of Q as the B operand: permuted like the columns of the widened keys, times a power of two that brings the
@@ -388,7 +405,7 @@ attn_int4_kernel(const AttnInt4Params p) {
         m[nt][e] = -FLT_MAX;                          // finite, so that a score of -inf weighs 0 and not NaN
         l[nt][e] = 0.f;
 #pragma unroll
-        for (int gg = 0; gg < NG; ++gg) low[gg][nt][e] = wsum[gg][nt][e] = wsum[gg][nt][2 + e] = 0.f;
+        for (int gg = 0; gg < NG; ++gg) low[gg][nt][e] = wsum[gg][nt][e] = wsum[gg][nt][2 + e] = 0.f;     // wsum: fp16 only
       }
 #pragma unroll
       for (int t = 0; t < MT; ++t)
@@ -398,114 +415,131 @@ attn_int4_kernel(const AttnInt4Params p) {
 
     const int first_u = it.u;                         // the first unit of this CTA's share of the segment
     while (true) {
-      if (left > Cfg::kAhead && (count - left + Cfg::kAhead) % kWarps == warp) {          // this warp's turn
-        ok = mbar_wait(bar_empty + 8 * next_stage, next_phase, abort_flag);
-        if (!(ok = __all_sync(0xffffffffu, ok))) break;
-        issue(ahead_of(it, Cfg::kAhead), next_stage);
+      const bool two = left > 1 && it.u + 1 < it.units;       // two units of the segment, or its last one
+      const int stage1 = stage + 1 == ST ? 0 : stage + 1;
+      // Usually the two units ST further on belong to the segment, whole and in a page each: their pages are looked up here,
+      // for the loads at the end of this round.
+      const int next0 = (it.u + ST) * kUnit + warp * 16, next1 = next0 + kUnit;
+      const bool easy = two && left > ST + 1 && tile_in_page && next1 + 16 <= it.len;
+      int page0 = 0, page1 = 0;
+      if (easy) {
+        const int* table = p.table + (int64_t)it.b * p.max_pages;
+        page0 = __ldg(table + p.page_div((uint32_t)next0));
+        page1 = __ldg(table + p.page_div((uint32_t)next1));
       }
-      if (++next_stage == ST) { next_stage = 0; next_phase ^= 1; }
-      ok = mbar_wait(bar_full + 8 * stage, phase, abort_flag);
-      if (!(ok = __all_sync(0xffffffffu, ok))) break;
-      const uint8_t* at = smem + stage * Cfg::kStage + warp * 16 * (DIM / 2);
-      const uint8_t* at_scale = smem + stage * Cfg::kStage + 2 * Cfg::kCodes + warp * 16 * (4 * NG);
-      const int t0 = it.u * kUnit + warp * 16;
-      uint32_t mask[1];
-      lds_words(smem + stage * Cfg::kStage + Cfg::kMask + 4 * warp, mask);
-      if (mask[0]) {                                  // uniform in the warp, like `full`
-        const bool full = mask[0] == 0xffffu && t0 + 16 <= all_see;       // every query sees every token
+      cp_async_wait<ST - 2>();
+      __syncwarp();                                           // every lane's copies have landed
+      const uint8_t* base[2] = {ring + stage * Cfg::kStage, ring + stage1 * Cfg::kStage};
+      const int t0 = it.u * kUnit + warp * 16;                // tokens t0 .. t0 + 15 and t0 + kUnit ..
+      uint32_t mask[2];
+      mask[0] = *reinterpret_cast<const uint32_t*>(base[0] + Cfg::kMask);
+      mask[1] = two ? *reinterpret_cast<const uint32_t*>(base[1] + Cfg::kMask) : 0u;
+      if (!two) base[1] = base[0];
+      if (mask[0] | mask[1]) {                        // uniform in the warp, like `full`
+        const bool full = (mask[0] & mask[1]) == 0xffffu && t0 + kUnit + 16 <= all_see;       // every query sees every token
         // ---- S^T = K Q^T, log2 domain -------------------------------------------------------------------------------------
-        float sc[NT][4];
+        float sc[2][NT][4];
 #pragma unroll
         for (int gg = 0; gg < NG; ++gg) {
           constexpr int W = GROUP / 32;
-          uint32_t w0[W], w1[W];
-          {
-            const int b = gg * (GROUP / 2) + j * (GROUP / 8);
-            lds_words(at + tok * (DIM / 2) + b, w0);
-            lds_words(at + (tok + 8) * (DIM / 2) + b, w1);
+          uint32_t w0[2][W], w1[2][W];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int in_row = gg * (GROUP / 2) + j * (GROUP / 8);
+            lds_words(base[t] + k_place(g, in_row / 16) + in_row % 16, w0[t]);
+            lds_words(base[t] + k_place(g + 8, in_row / 16) + in_row % 16, w1[t]);
           }
-          float d[NT][4];
+          float d[2][NT][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int x = 0; x < W; ++x)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) d[nt][e] = 0.f;
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int x = 0; x < W; ++x) {
-            uint32_t u0[4], u1[4];
-            widen4(w0[x], u0);
-            widen4(w1[x], u1);
-            const uint32_t a0[4] = {u0[0], u1[0], u0[1], u1[1]}, a1[4] = {u0[2], u1[2], u0[3], u1[3]};
+              for (int t = 0; t < 2; ++t) {
+                const uint32_t r0 = half ? w0[t][x] >> 8 : w0[t][x], r1 = half ? w1[t][x] >> 8 : w1[t][x];
+                const uint32_t a[4] = {r0 & 0x000f000fu, r1 & 0x000f000fu, r0 & 0x00f000f0u, r1 & 0x00f000f0u};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816(d[nt], a0, qf[nt][gg * MG + 2 * x][0], qf[nt][gg * MG + 2 * x][1]);
-              mma16816(d[nt], a1, qf[nt][gg * MG + 2 * x + 1][0], qf[nt][gg * MG + 2 * x + 1][1]);
-            }
+                for (int nt = 0; nt < NT; ++nt) {
+                  const uint32_t(&q)[2] = qf[nt][gg * MG + 2 * x + half];
+                  if (x == 0 && half == 0) mma16816_zero(d[t][nt], a, q[0], q[1]);
+                  else mma16816(d[t][nt], a, q[0], q[1]);
+                }
+              }
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const uint8_t* at = base[t] + 2 * Cfg::kCodes + (g * NG + gg) * 4;
+            const float2 k0 = widen_scale<T>(*reinterpret_cast<const uint32_t*>(at)), k1 = widen_scale<T>(*reinterpret_cast<const uint32_t*>(at + 32 * NG));
+            const float a0 = k0.x * to_score, a1 = k1.x * to_score;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float lo0 = k0.y * qsum[gg][nt][e], lo1 = k1.y * qsum[gg][nt][e];
+                sc[t][nt][e] = fmaf(a0, d[t][nt][e], gg ? sc[t][nt][e] + lo0 : lo0);
+                sc[t][nt][2 + e] = fmaf(a1, d[t][nt][2 + e], gg ? sc[t][nt][2 + e] + lo1 : lo1);
+              }
           }
-          uint32_t s0[1], s1[1];
-          lds_words(at_scale + (tok * NG + gg) * 4, s0);
-          lds_words(at_scale + ((tok + 8) * NG + gg) * 4, s1);
-          const float2 k0 = widen_scale<T>(s0[0]), k1 = widen_scale<T>(s1[0]);
-          const float a0 = k0.x * to_score, a1 = k1.x * to_score;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float lo0 = k0.y * qsum[gg][nt][e], lo1 = k1.y * qsum[gg][nt][e];
-              sc[nt][e] = fmaf(a0, d[nt][e], gg ? sc[nt][e] + lo0 : lo0);
-              sc[nt][2 + e] = fmaf(a1, d[nt][2 + e], gg ? sc[nt][2 + e] + lo1 : lo1);
-            }
         }
         // ---- the values' steps and minima; what is not seen --------------------------------------------------------------
-        float2 v0[NG], v1[NG];
+        float2 v0[2][NG], v1[2][NG];
         float big = 0.f;
 #pragma unroll
-        for (int gg = 0; gg < NG; ++gg) {
-          uint32_t s0[1], s1[1];
-          lds_words(at_scale + Cfg::kScales + (tok * NG + gg) * 4, s0);
-          lds_words(at_scale + Cfg::kScales + ((tok + 8) * NG + gg) * 4, s1);
-          v0[gg] = widen_scale<T>(s0[0]);
-          v1[gg] = widen_scale<T>(s1[0]);
-        }
-        uint32_t see = 0xffffffffu;                   // bit 4 nt + e: query 2j + (e & 1) sees token tok + 8 (e >> 1)
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int gg = 0; gg < NG; ++gg) {
+            const uint8_t* at = base[t] + 2 * Cfg::kCodes + Cfg::kScales + (g * NG + gg) * 4;
+            v0[t][gg] = widen_scale<T>(*reinterpret_cast<const uint32_t*>(at));
+            v1[t][gg] = widen_scale<T>(*reinterpret_cast<const uint32_t*>(at + 32 * NG));
+          }
+        uint32_t see = 0xffffffffu;                   // bit 8 t + 4 nt + e: query 2j + (e & 1) sees token g + 8 (e >> 1) of unit t
         if (!full) {
-          const bool live0 = mask[0] >> tok & 1, live1 = mask[0] >> (tok + 8) & 1;
           see = 0;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const bool live0 = mask[t] >> g & 1, live1 = mask[t] >> (g + 8) & 1;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const bool ok2 = (e < 2 ? live0 : live1) && t0 + t * kUnit + g + (e < 2 ? 0 : 8) < limit[nt][e & 1];
+                sc[t][nt][e] = ok2 ? sc[t][nt][e] : -INFINITY;
+                see |= (ok2 ? 1u : 0u) << (4 * NT * t + 4 * nt + e);
+              }
+#pragma unroll
+            for (int gg = 0; gg < NG; ++gg) {         // rows behind the last token hold anything
+              v0[t][gg] = live0 ? v0[t][gg] : make_float2(0.f, 0.f);
+              v1[t][gg] = live1 ? v1[t][gg] : make_float2(0.f, 0.f);
+            }
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int gg = 0; gg < NG; ++gg) {
+            big = fmaxf(big, fmaxf(fabsf(v0[t][gg].x), fabsf(v1[t][gg].x)));
+            if constexpr (kCentre) {                  // the middle of the range
+              v0[t][gg].y = fmaf(8.f, v0[t][gg].x, v0[t][gg].y);
+              v1[t][gg].y = fmaf(8.f, v1[t][gg].x, v1[t][gg].y);
+            }
+          }
+        // ---- whether the running maximum or the factor f has to move -----------------------------------------------------
+        // the maximum may lag by 2^8: p stays below 256, and sums are exact whatever the reference is
+        float over = 0.f, rel[2][NT][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const bool ok = (e < 2 ? live0 : live1) && t0 + tok + (e < 2 ? 0 : 8) < limit[nt][e & 1];
-              sc[nt][e] = ok ? sc[nt][e] : -INFINITY;
-              see |= (ok ? 1u : 0u) << (4 * nt + e);
+              rel[t][nt][e] = sc[t][nt][e] - m[nt][e & 1];
+              over = fmaxf(over, rel[t][nt][e]);
             }
-#pragma unroll
-          for (int gg = 0; gg < NG; ++gg) {           // rows behind the last token hold anything
-            v0[gg] = live0 ? v0[gg] : make_float2(0.f, 0.f);
-            v1[gg] = live1 ? v1[gg] : make_float2(0.f, 0.f);
-          }
-        }
-#pragma unroll
-        for (int gg = 0; gg < NG; ++gg) {
-          big = fmaxf(big, fmaxf(fabsf(v0[gg].x), fabsf(v1[gg].x)));
-          v0[gg].y = fmaf(8.f, v0[gg].x, v0[gg].y);   // the middle of the range: the weights' rounding meets c - 8
-          v1[gg].y = fmaf(8.f, v1[gg].x, v1[gg].y);
-        }
-        // ---- whether the running maximum or the factor f has to move -----------------------------------------------------
-        // the maximum may lag by 2^8: p stays below 256, and sums are exact whatever the reference is
-        float over = 0.f, rel[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            rel[nt][e] = sc[nt][e] - m[nt][e & 1];
-            over = fmaxf(over, rel[nt][e]);
-          }
         if (__any_sync(0xffffffffu, over > 8.f || big > most)) {
           float top[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) top[nt][e] = fmaxf(sc[nt][e], sc[nt][2 + e]);
+            for (int e = 0; e < 2; ++e) top[nt][e] = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][2 + e]), fmaxf(sc[1][nt][e], sc[1][nt][2 + e]));
 #pragma unroll
           for (int o = 4; o < 32; o *= 2) {
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
@@ -534,90 +568,112 @@ attn_int4_kernel(const AttnInt4Params p) {
 #pragma unroll
               for (int gg = 0; gg < NG; ++gg) {
                 low[gg][nt][e] *= alpha;
-                wsum[gg][nt][e] *= both;
-                wsum[gg][nt][2 + e] *= both;
+                if constexpr (kCentre) {
+                  wsum[gg][nt][e] *= both;
+                  wsum[gg][nt][2 + e] *= both;
+                }
               }
 #pragma unroll
               for (int t = 0; t < MT; ++t) {
                 acc[t][nt][e] *= both;
                 acc[t][nt][2 + e] *= both;
               }
-              rel[nt][e] = sc[nt][e] - m_new;
-              rel[nt][2 + e] = sc[nt][2 + e] - m_new;
+#pragma unroll
+              for (int t = 0; t < 2; ++t) {
+                rel[t][nt][e] = sc[t][nt][e] - m_new;
+                rel[t][nt][2 + e] = sc[t][nt][2 + e] - m_new;
+              }
             }
         }
         // ---- p and its sum ---------------------------------------------------------------------------------------------------
 #pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[t][nt][e] = ex2_approx(rel[t][nt][e]);
+#pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[nt][e] = ex2_approx(rel[nt][e]);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) l[nt][e] += sc[nt][e] + sc[nt][2 + e];
+          for (int e = 0; e < 2; ++e) l[nt][e] += (sc[0][nt][e] + sc[0][nt][2 + e]) + (sc[1][nt][e] + sc[1][nt][2 + e]);
         // ---- O^T += V^T P^T, group by group ----------------------------------------------------------------------------------
 #pragma unroll
         for (int gg = 0; gg < NG; ++gg) {
-          uint32_t pb[NT][2];
-          const float f0 = v0[gg].x * f, f1 = v1[gg].x * f;
+          uint32_t pb[2][NT][2];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float w[4] = {sc[nt][0] * f0, sc[nt][1] * f0, sc[nt][2] * f1, sc[nt][3] * f1};
-            if (full) {
+          for (int t = 0; t < 2; ++t) {
+            const float f0 = v0[t][gg].x * f, f1 = v1[t][gg].x * f;
 #pragma unroll
-              for (int e = 0; e < 2; ++e) low[gg][nt][e] = fmaf(sc[nt][e], v0[gg].y, fmaf(sc[nt][2 + e], v1[gg].y, low[gg][nt][e]));
-            } else {                                  // a value that a query does not see may be NaN, which 0 does not cancel
+            for (int nt = 0; nt < NT; ++nt) {
+              const float(&pr)[4] = sc[t][nt];
+              float w[4] = {pr[0] * f0, pr[1] * f0, pr[2] * f1, pr[3] * f1};
+              if (full) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const bool ok = see >> (4 * nt + e) & 1;
-                w[e] = ok ? w[e] : 0.f;
-                low[gg][nt][e & 1] += ok ? sc[nt][e] * (e < 2 ? v0[gg].y : v1[gg].y) : 0.f;
+                for (int e = 0; e < 2; ++e) low[gg][nt][e] = fmaf(pr[e], v0[t][gg].y, fmaf(pr[2 + e], v1[t][gg].y, low[gg][nt][e]));
+              } else {                                // a value that a query does not see may be NaN, which 0 does not cancel
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const bool ok2 = see >> (4 * NT * t + 4 * nt + e) & 1;
+                  w[e] = ok2 ? w[e] : 0.f;
+                  low[gg][nt][e & 1] += ok2 ? pr[e] * (e < 2 ? v0[t][gg].y : v1[t][gg].y) : 0.f;
+                }
+              }
+              pb[t][nt][0] = movmatrix_trans(pack_f16(w[0], w[1]));
+              pb[t][nt][1] = movmatrix_trans(pack_f16(w[2], w[3]));
+              if constexpr (kCentre) {
+                const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+                mma16816(wsum[gg][nt], ones, pb[t][nt][0], pb[t][nt][1]);
               }
             }
-            pb[nt][0] = movmatrix_trans(pack_f16(w[0], w[1]));
-            pb[nt][1] = movmatrix_trans(pack_f16(w[2], w[3]));
-            const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-            mma16816(wsum[gg][nt], ones, pb[nt][0], pb[nt][1]);
           }
           // words of the tokens of operand rows 2j, 2j + 1, 2j + 8, 2j + 9
           constexpr int W = GROUP >= 64 ? GROUP / 64 : 1;
-          uint32_t w[4][W];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = ((2 * j + (i & 1)) ^ (j & 1)) + 8 * (i >> 1);
-            lds_words(at + Cfg::kCodes + row * (DIM / 2) + gg * (GROUP / 2) + (GROUP >= 64 ? g * (GROUP / 16) : (g >> 1) * 4), w[i]);
-          }
+          for (int t = 0; t < 2; ++t) {
+            uint32_t w[4][W];
 #pragma unroll
-          for (int x = 0; x < W; ++x)
-#pragma unroll
-            for (int half = 0; half < (GROUP >= 64 ? 2 : 1); ++half) {
-              const uint32_t sel = GROUP >= 64 ? (half ? 0x7632u : 0x5410u) : ((g & 1) ? 0x7632u : 0x5410u);
-              uint32_t ua[4], ub[4];
-              widen4(__byte_perm(w[0][x], w[1][x], sel), ua);
-              widen4(__byte_perm(w[2][x], w[3][x], sel), ub);
-              const int t = gg * MG + (GROUP >= 64 ? 4 * x + 2 * half : 0);
-              const uint32_t a0[4] = {ua[0], ua[1], ub[0], ub[1]}, a1[4] = {ua[2], ua[3], ub[2], ub[3]};
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma16816(acc[t][nt], a0, pb[nt][0], pb[nt][1]);
-                mma16816(acc[t + 1][nt], a1, pb[nt][0], pb[nt][1]);
-              }
+            for (int i = 0; i < 4; ++i) {
+              const int in_row = gg * (GROUP / 2) + (GROUP >= 64 ? g * (GROUP / 16) : (g >> 1) * 4);
+              lds_words(base[t] + v_place(j + 4 * i, in_row / 16) + in_row % 16, w[i]);
             }
+#pragma unroll
+            for (int x = 0; x < W; ++x)
+#pragma unroll
+              for (int half = 0; half < (GROUP >= 64 ? 2 : 1); ++half) {
+                const uint32_t sel = GROUP >= 64 ? (half ? 0x7632u : 0x5410u) : ((g & 1) ? 0x7632u : 0x5410u);
+                uint32_t ua[4], ub[4];
+                widen4(__byte_perm(w[0][x], w[1][x], sel), ua);
+                widen4(__byte_perm(w[2][x], w[3][x], sel), ub);
+                const int mt = gg * MG + (GROUP >= 64 ? 4 * x + 2 * half : 0);
+                const uint32_t a0[4] = {ua[0], ua[1], ub[0], ub[1]}, a1[4] = {ua[2], ua[3], ub[2], ub[3]};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  mma16816(acc[mt][nt], a0, pb[t][nt][0], pb[t][nt][1]);
+                  mma16816(acc[mt + 1][nt], a1, pb[t][nt][0], pb[t][nt][1]);
+                }
+              }
+          }
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_empty + 8 * stage);
-      if (++stage == ST) { stage = 0; phase ^= 1; }
-      --left;
-      if (left == 0 || it.u + 1 == it.units) break;
-      ++it.u;
+      __syncwarp();                                   // every lane has left the stages: the units ST further on go there
+      if (easy && mla_page_ok(page0, p.num_pages) && mla_page_ok(page1, p.num_pages)) {
+        load_whole(stage, row_of(page0, it.h, next0));
+        cp_async_commit();
+        load_whole(stage1, row_of(page1, it.h, next1));
+        cp_async_commit();
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < (two ? 2 : 1); ++k) {
+          if (left > ST + k) load(ahead_of(it, ST + k), k ? stage1 : stage);
+          cp_async_commit();
+        }
+      }
+      stage = two ? (stage1 + 1 == ST ? 0 : stage1 + 1) : stage1;
+      left -= two ? 2 : 1;
+      it.u += two ? 2 : 1;
+      if (left == 0 || it.u == it.units) break;
     }
-    if (!ok) {
-      // a wait gave up: let the copies in flight land before the shared memory is released, report, leave
-      for (int i = 0; i < 64; ++i) __nanosleep(20000);
-      if (lane == 0 && p.status) *p.status = *abort_flag;
-      return;
-    }
+    --it.u;                                           // the segment's last unit here
 
     // ---- join the warps ---------------------------------------------------------------------------------------------------
 #pragma unroll
@@ -668,14 +724,14 @@ attn_int4_kernel(const AttnInt4Params p) {
         for (int e = 0; e < 2; ++e) {
           const int r = nt * 8 + 2 * j + e - r0;
           if (r >= 0 && r < Cfg::kJoinRows) {
-            float* dst = join + (warp * Cfg::kJoinRows + r) * Cfg::kPitch;
+            float* dst = join + (warp * Cfg::kJoinRows + r) * DIM;
 #pragma unroll
             for (int gg = 0; gg < NG; ++gg)
 #pragma unroll
               for (int t = 0; t < MG; ++t) {
                 const int d = gg * GROUP + g * (GROUP / 8) + 2 * t;
-                const float a0 = fmaf(acc[gg * MG + t][nt][e], 0x1p24f, -8.f * wsum[gg][nt][e]);
-                const float a1 = fmaf(acc[gg * MG + t][nt][2 + e], 0x1p20f, -8.f * wsum[gg][nt][e]);
+                const float off = kCentre ? -8.f * wsum[gg][nt][e] : 0.f;
+                const float a0 = fmaf(acc[gg * MG + t][nt][e], 0x1p24f, off), a1 = fmaf(acc[gg * MG + t][nt][2 + e], 0x1p20f, off);
                 *reinterpret_cast<float2*>(dst + d) =
                     make_float2(fmaf(a0, inv_f, low[gg][nt][e]) * part[nt][e], fmaf(a1, inv_f, low[gg][nt][e]) * part[nt][e]);
               }
@@ -689,7 +745,7 @@ attn_int4_kernel(const AttnInt4Params p) {
         float sum = 0.f, top = join_m[r];
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float4 a = *reinterpret_cast<const float4*>(join + (w * Cfg::kJoinRows + rj) * Cfg::kPitch + d);
+          const float4 a = *reinterpret_cast<const float4*>(join + (w * Cfg::kJoinRows + rj) * DIM + d);
           v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
           sum += join_l[w * Cfg::kRows + r];
           top = fmaxf(top, join_m[w * Cfg::kRows + r]);
@@ -738,7 +794,7 @@ attn_int4_kernel(const AttnInt4Params p) {
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
           float sum = 0.f;
           if (on) {
-#pragma unroll 8
+#pragma unroll 16
             for (int c = team; c < count; c += teams) {
               const float* s = slot_of(c);
               const float mc = __ldcg(s + Cfg::kRows * DIM + r), lc = __ldcg(s + Cfg::kRows * (DIM + 1) + r);
@@ -783,7 +839,7 @@ attn_int4_kernel(const AttnInt4Params p) {
 // ---- host --------------------------------------------------------------------------------------------------------------
 // Query rows of a kv head go in tiles of 8; from 9 rows on of 16 (dim 64, 128), where a widened key serves twice as many.
 static int q_tile_rows(int64_t rows, int64_t dim) { return rows > 8 && dim <= 128 ? 16 : 8; }
-static int ctas_per_sm(int64_t dim, int tile_rows) { return dim * (tile_rows / 8) <= 128 ? 2 : 1; }
+static int ctas_per_sm(int64_t dim, int tile_rows) { return dim * (tile_rows / 8) <= 128 ? 4 : 2; }
 
 struct I4Plan {
   int tile_rows, q_tiles, grid;
@@ -878,7 +934,6 @@ extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache
   p.rows = (int)(s_q * (h_q / h_kv)); p.q_tiles = plan.q_tiles;
   p.page_div = FastDiv((uint32_t)page_size);
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  p.status = device_status_word();
   TL_REQUIRE((batch * h_kv * plan.q_tiles) / plan.grid + 1 < (1ll << 31) / (p.len_cap / kUnit + 1),
              "attn_decode_paged_int4: more units of work than a CTA counts");
   TL_REQUIRE(plan.grid * 4 <= TL_B200_ATTN_INT4_ZERO_BYTES, "attn_decode_paged_int4: more SMs than counters");

@@ -68,17 +68,25 @@ inline cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, dim3 b
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// t / divisor for 0 <= t < 2^31 as a multiplication: a shift for powers of two, else floor(t m / 2^(32 + k)) with
-// k = floor(log2 divisor) and m = ceil(2^(32 + k) / divisor) < 2^32.  m * divisor exceeds 2^(32 + k) by less than
-// divisor < 2^(k + 1), so the quotient is exact for t < 2^31.
+// t / divisor for 0 <= t < 2^31 as a multiplication: floor(t m / 2^(32 + k)) with k = floor(log2 divisor) and
+// m = ceil(2^(32 + k) / divisor) < 2^32, or k one less and m = 2^31 for powers of two.  m * divisor exceeds 2^(32 + k) by
+// less than divisor < 2^(k + 1), so the quotient is exact for t < 2^31.
 struct FastDiv {
-  uint32_t mul = 0, shift = 0;
+  uint32_t mul = 0, shift = 0;            // mul 0: divisor 1
   FastDiv() = default;
   explicit FastDiv(uint32_t divisor) {
     while ((divisor >> (shift + 1)) != 0) ++shift;
-    if ((divisor & (divisor - 1)) != 0) mul = (uint32_t)(((1ull << (32 + shift)) + divisor - 1) / divisor);
+    if ((divisor & (divisor - 1)) != 0) {
+      mul = (uint32_t)(((1ull << (32 + shift)) + divisor - 1) / divisor);
+    } else if (shift > 0) {
+      mul = 1u << 31;
+      --shift;
+    }
   }
-  __device__ __forceinline__ uint32_t operator()(uint32_t t) const { return mul ? __umulhi(t, mul) >> shift : t >> shift; }
+  __device__ __forceinline__ uint32_t operator()(uint32_t t) const {
+    const uint32_t q = __umulhi(t, mul) >> shift;
+    return mul ? q : t;
+  }
 };
 
 inline int dtype_bytes(int dtype) {
