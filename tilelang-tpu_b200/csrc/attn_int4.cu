@@ -158,6 +158,8 @@ attn_int4_kernel(const AttnInt4Params p) {
   constexpr bool kCentre = std::is_same<T, __half>::value;       // the weights' rounding meets c - 8 (see above); bf16 outputs do not show it
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
+  dependency_wait();
+  dependency_release();
   uint8_t* tail = smem + kWarps * ST * Cfg::kStage;
   float* join = reinterpret_cast<float*>(tail);                  // [warps][join rows][pitch]
   float* join_m = join + kWarps * Cfg::kJoinRows * DIM;  // [warps][rows]
@@ -196,7 +198,11 @@ attn_int4_kernel(const AttnInt4Params p) {
     total *= per_unit;
     const int64_t ctas = total < gridDim.x ? total : gridDim.x;          // every one of them has a unit
     if (blockIdx.x >= ctas) return;                                      // the whole CTA
-    const int64_t start = (int64_t)blockIdx.x * total / ctas, end = ((int64_t)blockIdx.x + 1) * total / ctas;
+    // CTA i begins at floor(i * total / ctas)
+    const int64_t quot = total >> 32 ? total / ctas : (int64_t)((uint32_t)total / (uint32_t)ctas);
+    const uint32_t rest = (uint32_t)(total - quot * ctas);               // times a CTA number: below 2^32
+    const int64_t start = blockIdx.x * quot + blockIdx.x * rest / (uint32_t)ctas;
+    const int64_t end = (blockIdx.x + 1) * quot + (blockIdx.x + 1) * rest / (uint32_t)ctas;
     int64_t base = before + incl - mine;
     if (base * per_unit <= start && start < (base + mine) * per_unit) {  // exactly one thread
       int b = b0, units = 0;
@@ -218,7 +224,7 @@ attn_int4_kernel(const AttnInt4Params p) {
     it.len = mla_len(p.lens, it.b, p.len_cap);
     it.units = units_of(it.len);
     const int64_t off = start - sh.seq_base;
-    const int seg = (int)(off / it.units);
+    const int seg = off >> 32 ? (int)(off / it.units) : (int)((uint32_t)off / (uint32_t)it.units);
     it.u = (int)(off - (int64_t)seg * it.units);
     it.h = seg / p.q_tiles;
     it.qt = seg - it.h * p.q_tiles;
@@ -265,14 +271,12 @@ attn_int4_kernel(const AttnInt4Params p) {
     const uint32_t off = (uint32_t)t0 - p.page_div((uint32_t)t0) * (uint32_t)p.page_size;
     return ((uint32_t)page * p.h_kv + h) * (uint32_t)p.page_size + off;
   };
-  auto load = [&](const UnitIter& w, int stage) {
+  auto load = [&](const UnitIter& w, int stage, int page) {               // page: of the tile's first token, where tiles lie in one
     uint8_t* const stage_ptr = ring + stage * Cfg::kStage;
     const uint32_t at = smem_u32(stage_ptr);
     const int t0 = w.u * kUnit + warp * 16;
-    const int* table = p.table + (int64_t)w.b * p.max_pages;
     uint32_t mask = 0;
     if (tile_in_page) {
-      const int page = t0 < w.len ? __ldg(table + p.page_div((uint32_t)t0)) : -1;
       const int live = mla_page_ok(page, p.num_pages) ? min(w.len - t0, 16) : 0;
       const uint32_t row0 = row_of(page, w.h, t0);
       if (live == 16) {
@@ -293,7 +297,7 @@ attn_int4_kernel(const AttnInt4Params p) {
       bool live = my < w.len;
       uint32_t row = 0;
       if (live) {
-        const int id = __ldg(table + p.page_div((uint32_t)my));
+        const int id = __ldg(p.table + (int64_t)w.b * p.max_pages + p.page_div((uint32_t)my));
         live = mla_page_ok(id, p.num_pages);
         row = row_of(id, w.h, my);
       }
@@ -312,6 +316,10 @@ attn_int4_kernel(const AttnInt4Params p) {
     }
     *reinterpret_cast<uint32_t*>(stage_ptr + Cfg::kMask) = mask;             // every lane, the same word
   };
+  auto page_at = [&](const UnitIter& w) {
+    const int t0 = w.u * kUnit + warp * 16;
+    return tile_in_page && t0 < w.len ? __ldg(p.table + (int64_t)w.b * p.max_pages + p.page_div((uint32_t)t0)) : -1;
+  };
   // the unit `by` behind `it`
   auto ahead_of = [&](UnitIter w, int by) {
     w.u += by;
@@ -323,14 +331,9 @@ attn_int4_kernel(const AttnInt4Params p) {
     }
     return w;
   };
-#pragma unroll 1
-  for (int k = 0; k < ST; ++k) {
-    if (k < left) load(ahead_of(it, k), k);
-    cp_async_commit();
-  }
-
   // ---- segments -------------------------------------------------------------------------------------------------------
   int stage = 0;
+  bool first = true;
   while (left > 0) {
     const int rows = min(Cfg::kRows, p.rows - it.qt * Cfg::kRows);
     // the columns of Q as the B operand: permuted like the columns of the widened keys, times a power of two that brings the
@@ -354,6 +357,25 @@ attn_int4_kernel(const AttnInt4Params p) {
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) limit[nt][e] = it.len - p.s_q + (it.qt * Cfg::kRows + nt * 8 + 2 * j + e) / p.per + 1;
+      }
+      if (first) {                                    // fill the ring: lane k looks up the page of unit k, all at once
+        first = false;
+        const int page = lane < min(ST, left) ? page_at(ahead_of(it, lane)) : -1;
+#pragma unroll 1
+        for (int k = 0; k < ST; ++k) {
+          const int pg = __shfl_sync(0xffffffffu, page, k);
+          if (k < left) load(ahead_of(it, k), k, pg);
+          cp_async_commit();
+        }
+      }
+      if (lane < 2 * NT && it.units - it.u < left) {  // the queries of the next segment here: on their way to L2 by then
+        const UnitIter n = ahead_of(it, it.units - it.u);
+        const int row = n.qt * Cfg::kRows + (warp * 2 * NT + lane), qi = row / p.per;
+        if (row < p.rows) {
+          const T* at = reinterpret_cast<const T*>(p.q) + n.b * p.q_sb + qi * p.q_ss + ((int64_t)n.h * p.per + (row - qi * p.per)) * DIM;
+#pragma unroll
+          for (int i = 0; i < DIM; i += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + i));
+        }
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -664,7 +686,10 @@ attn_int4_kernel(const AttnInt4Params p) {
       } else {
 #pragma unroll 1
         for (int k = 0; k < (two ? 2 : 1); ++k) {
-          if (left > ST + k) load(ahead_of(it, ST + k), k ? stage1 : stage);
+          if (left > ST + k) {
+            const UnitIter w = ahead_of(it, ST + k);
+            load(w, k ? stage1 : stage, page_at(w));
+          }
           cp_async_commit();
         }
       }
@@ -766,14 +791,16 @@ attn_int4_kernel(const AttnInt4Params p) {
     if (!whole) {
       // CTAs c0 .. c1 share the segment; the last to arrive adds up their partial sums
       const int64_t total = sh.total, ctas = sh.ctas;
-      const int c0 = (int)(((seg_first + 1) * ctas - 1) / total), c1 = (int)((seg_end * ctas - 1) / total);
+      const int c0 = seg_first >= sh.start ? (int)blockIdx.x : (int)(((seg_first + 1) * ctas - 1) / total);
+      const int c1 = seg_end <= sh.end ? (int)blockIdx.x : (int)((seg_end * ctas - 1) / total);
       int* counter = p.counters + c0;                // only one shared segment begins in a CTA's range: its last
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) sh.last = atomicAdd(counter, 1) == c1 - c0;
+      if (threadIdx.x == 0) {                        // behind the barrier above: the fence covers every thread's partial sums
+        __threadfence();
+        sh.last = atomicAdd(counter, 1) == c1 - c0;
+        __threadfence();
+      }
       __syncthreads();
       if (sh.last) {
-        __threadfence();
         if (threadIdx.x == 0) *counter = 0;            // ready for the next call
         // the segment is the last of CTA c0 (slot 1 unless it is its first as well) and the first of all others (slot 0)
         const float* slots = p.partial + (int64_t)c0 * 2 * kSlot;
@@ -860,7 +887,7 @@ static int launch_i4(const AttnInt4Params& p, int grid, cudaStream_t s) {
   auto kernel = attn_int4_kernel<T, DIM, GROUP, NT>;
   constexpr int smem = I4Cfg<DIM, GROUP, NT>::kSmem;
   TL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kernel<<<grid, 32 * kWarps, smem, s>>>(p);
+  TL_CUDA(launch_overlapped(kernel, dim3(grid), dim3(32 * kWarps), smem, s, p));
   TL_LAUNCH_CHECK("attn_int4_kernel");
   return TL_B200_OK;
 }
