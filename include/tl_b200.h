@@ -308,7 +308,7 @@ int tl_b200_kv_cache_read(const int64_t* slots, const void* k_cache, const void*
  * `workspace`: tl_b200_attn_decode_paged_int4_workspace_bytes(...) bytes (0 for sizes the call refuses), 16-byte aligned.
  * Its first TL_B200_ATTN_INT4_ZERO_BYTES bytes must be zero before the first call and are zero again after each call,
  * whatever the sizes of the calls; calls that may overlap on the GPU need workspaces of their own.                 */
-#define TL_B200_ATTN_INT4_ZERO_BYTES 4096
+#define TL_B200_ATTN_INT4_ZERO_BYTES 8192
 int64_t tl_b200_attn_decode_paged_int4_workspace_bytes(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim);
 int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache, const void* k_scale, const void* v_cache,
                                    const void* v_scale, const int32_t* block_table, const int32_t* cache_seqlens, void* out,

@@ -52,11 +52,17 @@ struct AttnInt4Params {
   int rows, q_tiles;                   // query rows of a kv head (s_q * per), tiles of them
   FastDiv page_div;                    // t / page_size
   float scale_log2;
-  int* counters;                       // one per CTA, zero between calls
+  int* counters;                       // three per CTA, zero between calls
   float* partial;                      // [2 * gridDim.x][kRows * (dim + 2)]
 };
 
 constexpr int kWarps = 4, kUnit = 16 * kWarps;
+
+// CTAs per SM, by the registers a thread needs: 128 (four CTAs), 168 with four groups' steps and sums (32 x 4096 tokens:
+// 63 us, 73 us with four CTAs that spill), 255 with twice the accumulators (24 sequences of 4 tokens, dim 64: 39 us, 42 us).
+__host__ __device__ constexpr int i4_ctas(int dim, int groups, int nt) {
+  return nt == 2 || dim == 256 ? 2 : dim == 128 && groups == 4 ? 3 : 4;
+}
 
 template <int DIM, int GROUP, int NT> struct I4Cfg {
   static constexpr int kGroups = DIM / GROUP;
@@ -67,12 +73,11 @@ template <int DIM, int GROUP, int NT> struct I4Cfg {
   static constexpr int kRows = 8 * NT;
   static constexpr int kJoinRows = (DIM == 64 ? 4 : 2) * NT;            // rows joined at a time
   static constexpr int kJoin = kWarps * (kJoinRows * DIM + 2 * kRows) * 4;      // partial rows, maxima and sums of the warps
-  static constexpr int kCtas = DIM * NT <= 128 ? 4 : 2;                 // resident per SM: registers and shared memory
+  static constexpr int kCtas = i4_ctas(DIM, kGroups, NT);               // resident per SM
   static constexpr int kFit = (228 * 1024 / kCtas - 1024 - kJoin - 128) / (kWarps * kStage);
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static constexpr int kSmem = kWarps * kStages * kStage + kJoin + 128;
   static_assert(kStages >= 4, "two stages are worked on while two are on their way");
-  static_assert(kWarps * kJoinRows * DIM >= 5 * 32 * kWarps, "the join buffer serves the merge of partial sums too");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -789,65 +794,96 @@ attn_int4_kernel(const AttnInt4Params p) {
       __syncthreads();                                 // the join buffer is free again
     }
     if (!whole) {
-      // CTAs c0 .. c1 share the segment; the last to arrive adds up their partial sums
+      // CTAs c0 .. c1 share the segment.  They are taken in groups of sixteen neighbours: the last of a group to arrive adds
+      // its partial results up into the slot of the group's first CTA, the last group to be done adds up the groups'.  (One
+      // CTA adding up 74 takes 12 us.)
       const int64_t total = sh.total, ctas = sh.ctas;
       const int c0 = seg_first >= sh.start ? (int)blockIdx.x : (int)(((seg_first + 1) * ctas - 1) / total);
       const int c1 = seg_end <= sh.end ? (int)blockIdx.x : (int)((seg_end * ctas - 1) / total);
-      int* counter = p.counters + c0;                // only one shared segment begins in a CTA's range: its last
-      if (threadIdx.x == 0) {                        // behind the barrier above: the fence covers every thread's partial sums
-        __threadfence();
-        sh.last = atomicAdd(counter, 1) == c1 - c0;
-        __threadfence();
-      }
-      __syncthreads();
-      if (sh.last) {
-        if (threadIdx.x == 0) *counter = 0;            // ready for the next call
-        // the segment is the last of CTA c0 (slot 1 unless it is its first as well) and the first of all others (slot 0)
-        const float* slots = p.partial + (int64_t)c0 * 2 * kSlot;
-        const int in_c0 = seg_first > (int64_t)c0 * total / ctas ? kSlot : 0, count = c1 - c0 + 1;
-        auto slot_of = [&](int c) { return slots + (c == 0 ? in_c0 : (int64_t)c * 2 * kSlot); };
+      // the segment is the last of CTA c0 (slot 1 unless it is its first as well) and the first of all others (slot 0)
+      const int in_c0 = seg_first > (int64_t)c0 * total / ctas ? 1 : 0;
+      auto slot_of = [&](int c) { return p.partial + ((int64_t)c * 2 + (c == c0 ? in_c0 : 0)) * kSlot; };
+      constexpr int kGroup = 16;
+      const int lead = max(c0, (int)blockIdx.x / kGroup * kGroup), tail = min(c1, (int)blockIdx.x / kGroup * kGroup + kGroup - 1);
+      const int groups = c1 / kGroup - c0 / kGroup + 1;
+      // Three counters a CTA.  Only one shared segment begins in a CTA's range (its last), and a group of another segment
+      // that begins with this CTA goes by the counter of those that only pass through.
+      int* const group_counter = p.counters + 3 * lead + (lead == c0 ? 1 : 0);
+      int* const seg_counter = p.counters + 3 * c0 + 2;
+      auto arrive = [&](int* counter, int others) {    // behind a barrier: the fence covers every thread's stores
+        if (threadIdx.x == 0) {
+          __threadfence();
+          sh.last = atomicAdd(counter, 1) == others;
+          if (sh.last) *counter = 0;                   // ready for the next call
+          __threadfence();
+        }
+        __syncthreads();
+        return sh.last;
+      };
+      // Adds up `many` partial results in their order; `emit(r, d, sums, sum, top)` takes four columns of a row.
+      auto add_up = [&](int many, auto slot_at, auto emit) {
         constexpr int kRowThreads = DIM / 4 < 32 ? DIM / 4 : 32;         // neighbouring lanes with one row
-        const int items = rows * (DIM / 4), teams = 32 * kWarps > items ? 32 * kWarps / items : 1;
-        float4* team_v = reinterpret_cast<float4*>(join);               // [teams][items], at most 256
-        float* team_l = join + 4 * 32 * kWarps;
-        for (int i0 = 0; i0 < items; i0 += 32 * kWarps) {                // one round, unless a tile has more than 256 items
-          const int team = items < 32 * kWarps ? threadIdx.x / items : 0, i = items < 32 * kWarps ? threadIdx.x % items : i0 + threadIdx.x;
-          const bool on = team < teams && i < items;
+        constexpr int kBatch = 8;                      // loads on their way at once, in the last batch too
+        const int items = rows * (DIM / 4), rounds = (items + 32 * kWarps - 1) / (32 * kWarps);
+        for (int k = 0; k < rounds; ++k) {
+          const int i = k * 32 * kWarps + threadIdx.x;
+          const bool on = i < items;
           const int r = on ? i / (DIM / 4) : 0, d = i % (DIM / 4) * 4;
           float top = -FLT_MAX;
-          for (int c = lane % kRowThreads; c < count; c += kRowThreads) top = fmaxf(top, __ldcg(slot_of(c) + Cfg::kRows * DIM + r));
+#pragma unroll 2
+          for (int c = lane % kRowThreads; c < many; c += kRowThreads) top = fmaxf(top, __ldcg(slot_at(c) + Cfg::kRows * DIM + r));
 #pragma unroll
           for (int o = 1; o < kRowThreads; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
           float sum = 0.f;
-          if (on) {
-#pragma unroll 16
-            for (int c = team; c < count; c += teams) {
-              const float* s = slot_of(c);
-              const float mc = __ldcg(s + Cfg::kRows * DIM + r), lc = __ldcg(s + Cfg::kRows * (DIM + 1) + r);
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(s + r * DIM + d));
-              const float a = ex2_approx(mc - top);
-              v.x = fmaf(x.x, a, v.x); v.y = fmaf(x.y, a, v.y); v.z = fmaf(x.z, a, v.z); v.w = fmaf(x.w, a, v.w);
-              sum = fmaf(lc, a, sum);
+          for (int c = 0; c < many; c += kBatch) {
+            float4 x[kBatch];
+            float mc[kBatch], lc[kBatch];
+#pragma unroll
+            for (int q = 0; q < kBatch; ++q) {
+              const float* s = slot_at(min(c + q, many - 1));
+              mc[q] = __ldcg(s + Cfg::kRows * DIM + r);
+              lc[q] = __ldcg(s + Cfg::kRows * (DIM + 1) + r);
+              x[q] = __ldcg(reinterpret_cast<const float4*>(s + r * DIM + d));
             }
-          }
-          if (teams > 1) {                             // in a fixed order
-            if (on) {
-              team_v[team * items + i] = v;
-              team_l[team * items + i] = sum;
-            }
-            __syncthreads();
-            if (on && team == 0)
-              for (int t = 1; t < teams; ++t) {
-                const float4 x = team_v[t * items + i];
-                v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-                sum += team_l[t * items + i];
+#pragma unroll
+            for (int q = 0; q < kBatch; ++q)
+              if (c + q < many) {
+                const float w = ex2_approx(mc[q] - top);
+                v.x = fmaf(x[q].x, w, v.x); v.y = fmaf(x[q].y, w, v.y); v.z = fmaf(x[q].z, w, v.z); v.w = fmaf(x[q].w, w, v.w);
+                sum = fmaf(lc[q], w, sum);
               }
           }
-          if (on && team == 0) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            store_out(r, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+          if (on) emit(r, d, v, sum, top);
+        }
+      };
+      auto to_out = [&](int r, int d, float4 v, float sum, float) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        store_out(r, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+      };
+      if (arrive(group_counter, tail - lead)) {
+        auto member = [&](int i) { return slot_of(lead + i); };
+        if (groups == 1) {
+          add_up(tail - lead + 1, member, to_out);
+        } else {
+          float* const into = slot_of(lead);
+          // a thread reads all it needs of a row's columns before it writes them; the maxima and sums, which the threads of a
+          // row share, are written behind a barrier
+          add_up(tail - lead + 1, member, [&](int r, int d, float4 v, float sum, float top) {
+            __stcg(reinterpret_cast<float4*>(into + r * DIM + d), v);
+            if (d == 0) {
+              join_l[r] = sum;                         // free since the rows were joined
+              join_m[r] = top;
+            }
+          });
+          __syncthreads();
+          if (threadIdx.x < rows) {
+            __stcg(into + Cfg::kRows * DIM + threadIdx.x, join_m[threadIdx.x]);
+            __stcg(into + Cfg::kRows * (DIM + 1) + threadIdx.x, join_l[threadIdx.x]);
           }
+          __syncthreads();
+          if (arrive(seg_counter, groups - 1))
+            add_up(groups, [&](int i) { return slot_of(max(c0, (c0 / kGroup + i) * kGroup)); }, to_out);
         }
       }
     }
@@ -866,18 +902,17 @@ attn_int4_kernel(const AttnInt4Params p) {
 // ---- host --------------------------------------------------------------------------------------------------------------
 // Query rows of a kv head go in tiles of 8; from 9 rows on of 16 (dim 64, 128), where a widened key serves twice as many.
 static int q_tile_rows(int64_t rows, int64_t dim) { return rows > 8 && dim <= 128 ? 16 : 8; }
-static int ctas_per_sm(int64_t dim, int tile_rows) { return dim * (tile_rows / 8) <= 128 ? 4 : 2; }
 
 struct I4Plan {
   int tile_rows, q_tiles, grid;
   int64_t bytes;
 };
-static I4Plan i4_plan(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim) {
+static I4Plan i4_plan(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim, int64_t group) {
   I4Plan r;
   const int64_t rows = s_q * (h_q / h_kv);
   r.tile_rows = q_tile_rows(rows, dim);
   r.q_tiles = (int)((rows + r.tile_rows - 1) / r.tile_rows);
-  r.grid = sm_count() * ctas_per_sm(dim, r.tile_rows);
+  r.grid = sm_count() * i4_ctas((int)dim, (int)(dim / group), r.tile_rows / 8);
   r.bytes = TL_B200_ATTN_INT4_ZERO_BYTES + (int64_t)r.grid * 2 * r.tile_rows * (dim + 2) * 4;
   return r;
 }
@@ -918,7 +953,7 @@ static bool i4_sizes_ok(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, i
 using namespace tl;
 
 extern "C" int64_t tl_b200_attn_decode_paged_int4_workspace_bytes(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim) {
-  return i4_sizes_ok(batch, s_q, h_q, h_kv, dim) ? i4_plan(batch, s_q, h_q, h_kv, dim).bytes : 0;
+  return i4_sizes_ok(batch, s_q, h_q, h_kv, dim) ? i4_plan(batch, s_q, h_q, h_kv, dim, dim).bytes : 0;
 }
 
 extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache, const void* k_scale, const void* v_cache,
@@ -945,7 +980,7 @@ extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache
              "attn_decode_paged_int4: null tensor pointer");
   TL_REQUIRE(aligned16(q) && aligned16(out) && aligned16(k_cache) && aligned16(v_cache) && aligned16(k_scale) && aligned16(v_scale) &&
                  q_stride_batch % 8 == 0 && q_stride_token % 8 == 0, "attn_decode_paged_int4: tensors and rows of q must be 16-byte aligned");
-  const I4Plan plan = i4_plan(batch, s_q, h_q, h_kv, dim);
+  const I4Plan plan = i4_plan(batch, s_q, h_q, h_kv, dim, group);
   TL_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= plan.bytes,
              "attn_decode_paged_int4: needs a 16-byte aligned workspace of %lld bytes, got %lld", (long long)plan.bytes,
              (long long)workspace_bytes);
@@ -963,7 +998,7 @@ extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   TL_REQUIRE((batch * h_kv * plan.q_tiles) / plan.grid + 1 < (1ll << 31) / (p.len_cap / kUnit + 1),
              "attn_decode_paged_int4: more units of work than a CTA counts");
-  TL_REQUIRE(plan.grid * 4 <= TL_B200_ATTN_INT4_ZERO_BYTES, "attn_decode_paged_int4: more SMs than counters");
+  TL_REQUIRE(plan.grid * 12 <= TL_B200_ATTN_INT4_ZERO_BYTES, "attn_decode_paged_int4: more SMs than counters");
   p.counters = (int*)workspace;
   p.partial = (float*)((uint8_t*)workspace + TL_B200_ATTN_INT4_ZERO_BYTES);
   cudaStream_t s = (cudaStream_t)stream;

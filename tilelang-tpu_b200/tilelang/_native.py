@@ -17,7 +17,7 @@ DEFAULT_LIB = _PKG_ROOT / "lib" / "libtl_b200.so"
 
 TL_F32, TL_F16, TL_BF16, TL_E4M3, TL_I32, TL_U32, TL_I16, TL_U4G = range(8)
 ABI_VERSION = 100          # TL_B200_VERSION of include/tl_b200.h
-ATTN_INT4_ZERO_BYTES = 4096   # TL_B200_ATTN_INT4_ZERO_BYTES
+ATTN_INT4_ZERO_BYTES = 8192   # TL_B200_ATTN_INT4_ZERO_BYTES
 
 # name -> (restype, argtypes).  Kept in declaration order of include/tl_b200.h.
 PROTOTYPES = {
