@@ -24,7 +24,7 @@ __device__ __forceinline__ float activate(float x, int act) {
     case TL_B200_ACT_RELU: return x < 0.f ? 0.f : x;                                            // NaN stays NaN
     case TL_B200_ACT_GELU: return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
     case TL_B200_ACT_GELU_TANH: return 0.5f * x * (1.f + tanhf(0.79788456080286536f * fmaf(0.044715f * x * x, x, x)));
-    case TL_B200_ACT_SILU: return x / (1.f + expf(-x));
+    case TL_B200_ACT_SILU: return __fdividef(x, 1.f + expf(-x));                                // a quotient below 2^-120 may be zero
     default: return x;
   }
 }
@@ -93,6 +93,7 @@ template <int MT> struct SkinnyCfg {
 struct SkinnyParams {
   void* c;
   int m, n, k, splits, in_fmt;
+  int vec;                 // rows of C, the residual and the bias allow vectors of four
   int* status;
 };
 
@@ -113,7 +114,8 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int tile = blockIdx.x / p.splits, split = blockIdx.x % p.splits;         // the splits of a tile are one cluster
   const int num_kb = (p.k + kBK - 1) / kBK;
-  const int kb0 = (int)((int64_t)split * num_kb / p.splits), kb1 = (int)((int64_t)(split + 1) * num_kb / p.splits);
+  // K blocks split, split + splits, ...: together the cluster reads a contiguous piece of every weight row
+  const int mine = (num_kb - split + p.splits - 1) / p.splits;
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -134,12 +136,14 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
+  dependency_wait();            // what came before runs under the set-up above
+  dependency_release();
 
   if (warp == 0) {
     if (elect_one()) {
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int stage = (kb - kb0) % STAGES;
-        if (!mbar_wait(bar_empty + 8 * stage, (((kb - kb0) / STAGES) & 1) ^ 1, abort_flag)) break;
+      for (int i = 0; i < mine; ++i) {
+        const int stage = i % STAGES, kb = split + i * p.splits;
+        if (!mbar_wait(bar_empty + 8 * stage, ((i / STAGES) & 1) ^ 1, abort_flag)) break;
         const uint32_t full = bar_full + 8 * stage, dst = base + stage * Cfg::kStage;
         mbar_expect_tx(full, Cfg::kStage);
         if constexpr (W_MN_MAJOR) {          // weights [k, n]: two slabs of 64 columns x 64 k rows
@@ -155,16 +159,16 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
     if (elect_one()) {
       const uint32_t idesc = make_idesc(p.in_fmt, p.in_fmt, W_MN_MAJOR, false, kBM, MT);
       bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int stage = (kb - kb0) % STAGES;
-        if (!(ok = mbar_wait(bar_full + 8 * stage, ((kb - kb0) / STAGES) & 1, abort_flag))) break;
+      for (int i = 0; i < mine; ++i) {
+        const int stage = i % STAGES;
+        if (!(ok = mbar_wait(bar_full + 8 * stage, (i / STAGES) & 1, abort_flag))) break;
         tc_fence_after_sync();
         const uint32_t w = base + stage * Cfg::kStage, x = w + Cfg::kStageW;
 #pragma unroll
         for (int kk = 0; kk < kRowBytes / kUmmaBytes; ++kk) {
           const uint64_t a = W_MN_MAJOR ? smem_desc_sw128(w + kk * 16 * kRowBytes, kBK * kRowBytes, 1024)
                                         : smem_desc_sw128(w + kk * kUmmaBytes, 16, 1024);
-          mma_f16_ss(tmem_base, a, smem_desc_sw128(x + kk * kUmmaBytes, 16, 1024), idesc, (kb > kb0 || kk) ? 1u : 0u);
+          mma_f16_ss(tmem_base, a, smem_desc_sw128(x + kk * kUmmaBytes, 16, 1024), idesc, (i | kk) ? 1u : 0u);
         }
         mma_commit(bar_empty + 8 * stage);
       }
@@ -172,65 +176,94 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
     }
   }
   __syncwarp();
-  // ---- the tile: thread = weight row (column of C), registers = rows of A --------------------------------------------
+  // ---- the tile: each warp's 32 weight rows (columns of C) to shared memory, row by row of A ----------------------------
   bool ok = mbar_wait(bar_done, 0, abort_flag);
   ok = __all_sync(0xffffffffu, ok);
   tc_fence_after_sync();
-  const int col = tile * kBM + warp * 32 + lane;
-  const T* residual = reinterpret_cast<const T*>(ep.residual);
-  TOut* c = reinterpret_cast<TOut*>(p.c);
-  auto finish = [&](float x, int row) {
-    if (ep.bias) x += to_f32(reinterpret_cast<const T*>(ep.bias)[col]);
-    x = activate(x, ep.act);
-    const int64_t at = (int64_t)row * p.n + col;
-    if (residual) x += to_f32(residual[at]);
-    c[at] = from_f32<TOut>(x);
-  };
   const uint32_t t_addr = tmem_base + ((uint32_t)(warp * 32) << 16);
   float* part = reinterpret_cast<float*>(base_ptr);               // [MT][kPitch]: every MMA that read the ring has retired
   if (ok) {
 #pragma unroll 1
-    for (int c0 = 0; c0 < MT; c0 += 16) {
-      if (c0 >= p.m) break;
+    for (int c0 = 0; c0 < p.m; c0 += 16) {
       uint32_t v[16];
       tmem_ld_32x16(t_addr + c0, v);
       tmem_ld_wait();
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if (p.splits == 1) {
-          if (c0 + e < p.m && col < p.n) finish(__uint_as_float(v[e]), c0 + e);
-        } else {
-          part[(c0 + e) * Cfg::kPitch + warp * 32 + lane] = __uint_as_float(v[e]);
-        }
-      }
+      for (int e = 0; e < 16; ++e) part[(c0 + e) * Cfg::kPitch + warp * 32 + lane] = __uint_as_float(v[e]);
     }
   }
-  if (p.splits > 1) {
-    cluster_sync_all();                                           // also publishes the partial tiles
-    if (ok) {
-      // this CTA's share of the tile's elements, four neighbouring columns a thread
-      const int r0 = (int)((int64_t)split * p.m / p.splits), r1 = (int)((int64_t)(split + 1) * p.m / p.splits);
-      for (int r = r0 + warp; r < r1; r += 4) {
-        const uint32_t at = smem_u32(part + r * Cfg::kPitch + lane * 4);
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < p.splits; ++s) {
-          float y[4];
-          asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3])
-                       : "r"(map_to_cta(at, s)) : "memory");
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] += y[e];
-        }
-        const int n0 = tile * kBM + lane * 4;
+  if (p.splits > 1) cluster_sync_all();                           // the cluster's partial tiles are there
+  else __syncthreads();
+  if (ok) {
+    // this CTA's share of the tile, four neighbouring columns a thread; all the partial sums of an element at once
+    const int items = p.m * (kBM / 4);
+    const int i0 = (int)((int64_t)split * items / p.splits), i1 = (int)((int64_t)(split + 1) * items / p.splits);
+    const T *bias = reinterpret_cast<const T*>(ep.bias), *residual = reinterpret_cast<const T*>(ep.residual);
+    TOut* c = reinterpret_cast<TOut*>(p.c);
+    for (int i = i0 + threadIdx.x; i < i1; i += 128) {
+      const int r = i / (kBM / 4), in_tile = i % (kBM / 4) * 4, n0 = tile * kBM + in_tile;
+      const int valid = min(4, p.n - n0);
+      if (valid <= 0) continue;
+      const int64_t at = (int64_t)r * p.n + n0;
+      union { uint2 raw; T e[4]; } b, res;
+      b.raw = res.raw = make_uint2(0, 0);
+      if (p.vec && valid == 4) {
+        if (bias) b.raw = *reinterpret_cast<const uint2*>(bias + n0);
+        if (residual) res.raw = *reinterpret_cast<const uint2*>(residual + at);
+      } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (n0 + e < p.n) {
-            float z = x[e];
-            if (ep.bias) z += to_f32(reinterpret_cast<const T*>(ep.bias)[n0 + e]);
-            z = activate(z, ep.act);
-            const int64_t o = (int64_t)r * p.n + n0 + e;
-            if (residual) z += to_f32(residual[o]);
-            c[o] = from_f32<TOut>(z);
+          if (e < valid) {
+            if (bias) b.e[e] = bias[n0 + e];
+            if (residual) res.e[e] = residual[at + e];
           }
+      }
+      const uint32_t mine_at = smem_u32(part + r * Cfg::kPitch + in_tile);
+      float y[8][4];
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s < p.splits)
+          asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(y[s][0]), "=f"(y[s][1]), "=f"(y[s][2]), "=f"(y[s][3])
+                       : "r"(map_to_cta(mine_at, s)) : "memory");
+        else
+          y[s][0] = y[s][1] = y[s][2] = y[s][3] = 0.f;
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = y[0][e];
+#pragma unroll
+        for (int s = 1; s < 8; ++s) x[e] += y[s][e];
+        if (bias) x[e] += to_f32(b.e[e]);
+      }
+      if (ep.act != TL_B200_ACT_NONE) {
+        switch (ep.act) {      // outside the loop: one copy of each function
+          case TL_B200_ACT_RELU:
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = activate(x[e], TL_B200_ACT_RELU);
+            break;
+          case TL_B200_ACT_GELU:
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = activate(x[e], TL_B200_ACT_GELU);
+            break;
+          case TL_B200_ACT_GELU_TANH:
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = activate(x[e], TL_B200_ACT_GELU_TANH);
+            break;
+          default:
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = activate(x[e], TL_B200_ACT_SILU);
+        }
+      }
+      union { uint4 raw16; uint2 raw8; TOut e[4]; } o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o.e[e] = from_f32<TOut>(residual ? x[e] + to_f32(res.e[e]) : x[e]);
+      if (p.vec && valid == 4) {
+        if constexpr (sizeof(TOut) == 4) *reinterpret_cast<uint4*>(c + at) = o.raw16;
+        else *reinterpret_cast<uint2*>(c + at) = o.raw8;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < valid) c[at + e] = o.e[e];
       }
     }
   }
@@ -254,17 +287,19 @@ template <int MT, bool W_MN_MAJOR, typename T, typename TOut>
 static int launch_skinny(const CUtensorMap& tw, const CUtensorMap& tx, const SkinnyParams& p, const EpilogueArgs& ep, cudaStream_t s) {
   auto kernel = gemm_skinny_kernel<MT, W_MN_MAJOR, T, TOut>;
   TL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SkinnyCfg<MT>::kSmemBytes));
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)p.splits;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.splits;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((p.n + kBM - 1) / kBM * p.splits));
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = SkinnyCfg<MT>::kSmemBytes;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = p.splits > 1 ? 2 : 1;
   TL_CUDA(cudaLaunchKernelEx(&cfg, kernel, tw, tx, p, ep));
   TL_LAUNCH_CHECK("gemm_skinny_kernel");
   return TL_B200_OK;
@@ -301,6 +336,7 @@ static int gemm_skinny(const void* a, const void* b, void* c, int m, int n, int 
   SkinnyParams p;
   p.c = c; p.m = m; p.n = n; p.k = k;
   p.in_fmt = bf ? kFmtBF16 : kFmtF16;
+  p.vec = n % 4 == 0 && aligned16(c) && aligned16(ep.bias) && aligned16(ep.residual);
   p.status = device_status_word();
   // as many splits of K (1, 2, 4, 8: a portable cluster) as two CTAs per SM have room for, with at least four K blocks each
   const int tiles = (n + kBM - 1) / kBM, num_kb = (k + 63) / 64;
