@@ -31,6 +31,7 @@ struct CacheArgs {
   int heads, page_size;
   FastDiv head_div, page_div, vec_div;
   int64_t total_slots;
+  int wide;                   // rows are 32-byte aligned: one 256-bit access for 16 columns
 };
 
 // NaN-propagating minimum and maximum of two packed 16-bit values.
@@ -81,6 +82,8 @@ __global__ void __launch_bounds__(256)
 kv_write_u4g_kernel(const CacheArgs p) {
   using P = typename Pair<T>::type;
   constexpr int kLanes = DIM / 16, kGroupLanes = GROUP / 16;
+  dependency_wait();
+  dependency_release();
   const Side side = blockIdx.y ? p.v : p.k;
   const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   const int part = threadIdx.x % kLanes;
@@ -92,8 +95,14 @@ kv_write_u4g_kernel(const CacheArgs p) {
   in.raw[0] = in.raw[1] = make_uint4(0, 0, 0, 0);
   if (row < p.rows) {                 // whatever the slot: the two loads need not wait for each other
     const T* src = reinterpret_cast<const T*>(side.x) + t * side.stride + h * DIM + part * 16;
-    in.raw[0] = ld_stream16(src);
-    in.raw[1] = ld_stream16(src + 8);
+    if (p.wide) {                     // two 16-byte loads would each fetch every sector
+      const Vec32<T> v = ld_stream32<T>(src);
+      in.raw[0] = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+      in.raw[1] = make_uint4(v.w[4], v.w[5], v.w[6], v.w[7]);
+    } else {
+      in.raw[0] = ld_stream16(src);
+      in.raw[1] = ld_stream16(src + 8);
+    }
   }
   P lo2 = in.v[0], hi2 = in.v[0];
 #pragma unroll
@@ -146,43 +155,65 @@ kv_write_u4g_kernel(const CacheArgs p) {
   }
 }
 
+// A thread widens 16 columns of two rows; both rows' slots, then both rows' codes are on their way at once.
 template <typename T, int DIM, int GROUP>
 __global__ void __launch_bounds__(256)
 kv_read_u4g_kernel(const CacheArgs p) {
   using P = typename Pair<T>::type;
-  constexpr int kLanes = DIM / 16, kGroupLanes = GROUP / 16;
+  constexpr int kLanes = DIM / 16, kGroupLanes = GROUP / 16, kRows = 256 / kLanes;
+  dependency_wait();
+  dependency_release();
   const Side side = blockIdx.y ? p.v : p.k;
-  const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   const int part = threadIdx.x % kLanes;
-  if (row >= p.rows) return;
-  const uint32_t t = p.head_div(row);
-  const int h = (int)(row - t * p.heads);
-  const int64_t slot = __ldg(p.slots + t);
-  if (slot < 0 || slot >= p.total_slots) return;
-  const uint32_t s32 = (uint32_t)slot, page = p.page_div(s32), off = s32 - page * (uint32_t)p.page_size;
-  const int64_t src = ((int64_t)page * p.heads + h) * p.page_size + off;
-  const uint2 codes = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(side.cache) + src * (DIM / 2) + part * 8);
-  const float2 sc = widen2(reinterpret_cast<const P*>(side.scale)[src * (DIM / GROUP) + part / kGroupLanes]);
-  const float2 s2 = make_float2(sc.x, sc.x), l2 = make_float2(sc.y, sc.y), m128 = make_float2(-128.f, -128.f);
-  uint32_t out[8];
+  uint32_t t[2];
+  int h[2];
+  int64_t slot[2];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const uint32_t w = half ? codes.y : codes.x;
-    float2 f[4];                      // columns i and i + 4 of the word
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;          // bf16 pair of 128 + code
-      const float2 c = sm100::add2(make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)), m128);
-      f[i] = sm100::fma2(s2, c, l2);  // s * code is exact in fp32, so this is one rounding; then the output's
-    }
-    out[half * 4 + 0] = narrow2<T>(make_float2(f[0].x, f[1].x));
-    out[half * 4 + 1] = narrow2<T>(make_float2(f[2].x, f[3].x));
-    out[half * 4 + 2] = narrow2<T>(make_float2(f[0].y, f[1].y));
-    out[half * 4 + 3] = narrow2<T>(make_float2(f[2].y, f[3].y));
+  for (int k = 0; k < 2; ++k) {
+    const uint32_t row = (blockIdx.x * 2 + k) * kRows + threadIdx.x / kLanes;
+    t[k] = p.head_div(row);
+    h[k] = (int)(row - t[k] * p.heads);
+    slot[k] = row < p.rows ? __ldg(p.slots + t[k]) : -1;
   }
-  uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(side.x) + t * side.stride + h * DIM + part * 16);
-  dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
-  dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+  uint2 codes[2];
+  P scale[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (slot[k] >= 0 && slot[k] < p.total_slots) {
+      const uint32_t s32 = (uint32_t)slot[k], page = p.page_div(s32), off = s32 - page * (uint32_t)p.page_size;
+      const int64_t src = ((int64_t)page * p.heads + h[k]) * p.page_size + off;
+      codes[k] = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(side.cache) + src * (DIM / 2) + part * 8);
+      scale[k] = reinterpret_cast<const P*>(side.scale)[src * (DIM / GROUP) + part / kGroupLanes];
+    }
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (slot[k] >= 0 && slot[k] < p.total_slots) {
+      const float2 sc = widen2(scale[k]);
+      const float2 s2 = make_float2(sc.x, sc.x), l2 = make_float2(sc.y, sc.y), m128 = make_float2(-128.f, -128.f);
+      Vec32<T> out;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t w = half ? codes[k].y : codes[k].x;
+        float2 f[4];                  // columns i and i + 4 of the word
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;        // bf16 pair of 128 + code
+          const float2 c = sm100::add2(make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)), m128);
+          f[i] = sm100::fma2(s2, c, l2);      // s * code is exact in fp32, so this is one rounding; then the output's
+        }
+        out.w[half * 4 + 0] = narrow2<T>(make_float2(f[0].x, f[1].x));
+        out.w[half * 4 + 1] = narrow2<T>(make_float2(f[2].x, f[3].x));
+        out.w[half * 4 + 2] = narrow2<T>(make_float2(f[0].y, f[1].y));
+        out.w[half * 4 + 3] = narrow2<T>(make_float2(f[2].y, f[3].y));
+      }
+      T* dst = reinterpret_cast<T*>(side.x) + t[k] * side.stride + h[k] * DIM + part * 16;
+      if (p.wide) {
+        st_stream32(dst, out);
+      } else {
+        reinterpret_cast<uint4*>(dst)[0] = make_uint4(out.w[0], out.w[1], out.w[2], out.w[3]);
+        reinterpret_cast<uint4*>(dst)[1] = make_uint4(out.w[4], out.w[5], out.w[6], out.w[7]);
+      }
+    }
 }
 
 // ---- e4m3: a warp owns a row and keeps it in registers, 8 columns (16 bytes) a lane and pass ----------------------------
@@ -190,6 +221,8 @@ template <typename T, int PASSES>
 __global__ void __launch_bounds__(256)
 kv_write_e4m3_kernel(const CacheArgs p, const int dim) {
   using P = typename Pair<T>::type;
+  dependency_wait();
+  dependency_release();
   const Side side = blockIdx.y ? p.v : p.k;
   const int lane = threadIdx.x % 32;
   const uint32_t t = blockIdx.x * 8 + threadIdx.x / 32;
@@ -234,48 +267,80 @@ kv_write_e4m3_kernel(const CacheArgs p, const int dim) {
   if (lane == 0) reinterpret_cast<float*>(side.scale)[slot] = s;
 }
 
-// 8 columns a thread; a block takes kReadTokens tokens, their columns dealt out over its threads.
-constexpr int kReadTokens = 8;
-template <typename T>
+// COLS columns a thread and item; a block takes `per_block` tokens, at most two items a thread, both on their way at once.
+template <typename T, int COLS>
 __global__ void __launch_bounds__(256)
-kv_read_e4m3_kernel(const CacheArgs p, const int dim) {
+kv_read_e4m3_kernel(const CacheArgs p, const int dim, const int per_block) {
+  dependency_wait();
+  dependency_release();
   const Side side = blockIdx.y ? p.v : p.k;
-  const int vecs = dim / 8;
-  const uint32_t t0 = blockIdx.x * kReadTokens;
-  const int items = (int)min((uint32_t)kReadTokens, p.tokens - t0) * vecs;
-  for (int i = threadIdx.x; i < items; i += 256) {
-    const uint32_t k = p.vec_div((uint32_t)i), t = t0 + k;
-    const int c = (i - (int)k * vecs) * 8;
-    const int64_t slot = __ldg(p.slots + t);
-    if (slot < 0 || slot >= p.total_slots) continue;
-    const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(side.cache) + slot * dim + c);
-    const float s = reinterpret_cast<const float*>(side.scale)[slot];
-    uint32_t out[4];
+  const int vecs = dim / COLS;
+  const uint32_t t0 = blockIdx.x * (uint32_t)per_block;
+  const int items = (int)min((uint32_t)per_block, p.tokens - t0) * vecs;
+  uint32_t t[2];
+  int col[2];
+  int64_t slot[2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((e < 2 ? w.x : w.y) >> (16 * (e & 1))), __NV_E4M3);
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));      // e4m3 -> fp16 is exact
-      out[e] = narrow2<T>(make_float2(f.x * s, f.y * s));
-    }
-    *reinterpret_cast<uint4*>(reinterpret_cast<T*>(side.x) + t * side.stride + c) = make_uint4(out[0], out[1], out[2], out[3]);
+  for (int k = 0; k < 2; ++k) {
+    const int i = threadIdx.x + 256 * k;
+    const uint32_t in_block = p.vec_div((uint32_t)i);
+    t[k] = t0 + in_block;
+    col[k] = (i - (int)in_block * vecs) * COLS;
+    slot[k] = i < items ? __ldg(p.slots + t[k]) : -1;
   }
+  uint32_t codes[2][COLS / 4];
+  float s[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (slot[k] >= 0 && slot[k] < p.total_slots) {
+      const uint8_t* src = reinterpret_cast<const uint8_t*>(side.cache) + slot[k] * dim + col[k];
+      if constexpr (COLS == 16) {
+        const uint4 w = *reinterpret_cast<const uint4*>(src);
+        codes[k][0] = w.x; codes[k][1] = w.y; codes[k][2] = w.z; codes[k][3] = w.w;
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(src);
+        codes[k][0] = w.x; codes[k][1] = w.y;
+      }
+      s[k] = reinterpret_cast<const float*>(side.scale)[slot[k]];
+    }
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (slot[k] >= 0 && slot[k] < p.total_slots) {
+      uint32_t out[COLS / 2];
+#pragma unroll
+      for (int e = 0; e < COLS / 2; ++e) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes[k][e / 2] >> (16 * (e & 1))), __NV_E4M3);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));    // e4m3 -> fp16 is exact
+        out[e] = narrow2<T>(make_float2(f.x * s[k], f.y * s[k]));
+      }
+      T* dst = reinterpret_cast<T*>(side.x) + t[k] * side.stride + col[k];
+      if constexpr (COLS == 16) {
+        Vec32<T> v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.w[e] = out[e];
+        st_stream32(dst, v);
+      } else {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
+      }
+    }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
 template <typename T, int DIM>
 static int launch_u4g(const CacheArgs& a, int group, int sides, bool write, cudaStream_t s) {
-  constexpr unsigned kRowsPerBlock = 256 / (DIM / 16);
-  const dim3 grid((a.rows + kRowsPerBlock - 1) / kRowsPerBlock, (unsigned)sides);
+  const unsigned rows_per_block = 256 / (DIM / 16) * (write ? 1 : 2);
+  const dim3 grid((a.rows + rows_per_block - 1) / rows_per_block, (unsigned)sides);
+  cudaError_t rc = cudaSuccess;
   auto go = [&](auto g) {
     constexpr int G = decltype(g)::value;
     if constexpr (G <= DIM) {
-      if (write) kv_write_u4g_kernel<T, DIM, G><<<grid, 256, 0, s>>>(a);
-      else kv_read_u4g_kernel<T, DIM, G><<<grid, 256, 0, s>>>(a);
+      rc = launch_overlapped(write ? kv_write_u4g_kernel<T, DIM, G> : kv_read_u4g_kernel<T, DIM, G>, grid, dim3(256), 0, s, a);
     }
   };
   if (group == 32) go(std::integral_constant<int, 32>());
   else if (group == 64) go(std::integral_constant<int, 64>());
   else go(std::integral_constant<int, 128>());
+  TL_CUDA(rc);
   TL_LAUNCH_CHECK(write ? "kv_write_u4g_kernel" : "kv_read_u4g_kernel");
   return TL_B200_OK;
 }
@@ -289,15 +354,17 @@ static int launch_cache(const CacheArgs& a, int64_t dim, int64_t group, int form
   }
   if (write) {
     const dim3 grid((unsigned)((a.tokens + 7) / 8), (unsigned)sides);
-    const int d = (int)dim;
-    if (dim <= 256) kv_write_e4m3_kernel<T, 1><<<grid, 256, 0, s>>>(a, d);
-    else if (dim <= 512) kv_write_e4m3_kernel<T, 2><<<grid, 256, 0, s>>>(a, d);
-    else if (dim <= 768) kv_write_e4m3_kernel<T, 3><<<grid, 256, 0, s>>>(a, d);
-    else kv_write_e4m3_kernel<T, 4><<<grid, 256, 0, s>>>(a, d);
+    auto kernel = dim <= 256 ? kv_write_e4m3_kernel<T, 1> : dim <= 512 ? kv_write_e4m3_kernel<T, 2>
+                : dim <= 768 ? kv_write_e4m3_kernel<T, 3> : kv_write_e4m3_kernel<T, 4>;
+    TL_CUDA(launch_overlapped(kernel, grid, dim3(256), 0, s, a, (int)dim));
     TL_LAUNCH_CHECK("kv_write_e4m3_kernel");
   } else {
-    const dim3 grid((a.tokens + kReadTokens - 1) / kReadTokens, (unsigned)sides);
-    kv_read_e4m3_kernel<T><<<grid, 256, 0, s>>>(a, (int)dim);
+    const bool sixteen = dim % 16 == 0 && a.wide;
+    const int vecs = (int)dim / (sixteen ? 16 : 8), per_block = vecs > 512 ? 1 : 512 / vecs;
+    CacheArgs b = a;
+    b.vec_div = FastDiv((uint32_t)vecs);
+    const dim3 grid((a.tokens + per_block - 1) / per_block, (unsigned)sides);
+    TL_CUDA(launch_overlapped(sixteen ? kv_read_e4m3_kernel<T, 16> : kv_read_e4m3_kernel<T, 8>, grid, dim3(256), 0, s, b, (int)dim, per_block));
     TL_LAUNCH_CHECK("kv_read_e4m3_kernel");
   }
   return TL_B200_OK;
@@ -338,7 +405,7 @@ static int cache_call(const char* who, const int64_t* slots, int64_t tokens, con
   a.total_slots = num_pages * page_size;
   a.head_div = FastDiv((uint32_t)heads);
   a.page_div = FastDiv((uint32_t)page_size);
-  a.vec_div = FastDiv((uint32_t)(dim / 8));
+  a.wide = aligned32(k) && k_stride % 16 == 0 && (!both || (aligned32(v) && v_stride % 16 == 0));
   cudaStream_t s = (cudaStream_t)stream;
   const int sides = both ? 2 : 1;
   return dtype == TL_BF16 ? launch_cache<__nv_bfloat16>(a, dim, group, format, sides, write, s)
