@@ -398,6 +398,10 @@ int tl_b200_tile_program(const tl_b200_vm_instr* instrs, int n_instr, const void
 #define TL_B200_K_FLASH_ATTN_FWD 15
 #define TL_B200_K_MLA_DECODE_DENSE 16
 #define TL_B200_K_MLA_DECODE_PAGED 17
+#define TL_B200_K_KV_CACHE_WRITE 18
+#define TL_B200_K_KV_CACHE_READ 19
+#define TL_B200_K_ATTN_DECODE_PAGED_INT4 20
+#define TL_B200_K_GEMM_EPILOGUE 21
 int tl_b200_run(int kernel_id, void** args, const int64_t* meta, void* stream);
 
 #ifdef __cplusplus

@@ -277,3 +277,37 @@ def test_a_decode_step_with_all_of_them(cuda_device):
         assert ((att.cpu().double() - ref).abs() <= tolerance(host, ref)).all()
         ref_x = O.gemm_epilogue(att.cpu().view(b, -1), wo.cpu(), residual=before, transpose_b=True)
         assert torch.allclose(x.cpu().double(), ref_x, rtol=2.0 ** -8, atol=1e-4)
+
+
+def test_the_same_through_compiled_programs(cuda_device):
+    """Write, attention and projection as library programs with host tensors: the same bits as the operators."""
+    import tilelang
+    from tilelang import programs as P
+    dev, h_q, h_kv, dim, page = cuda_device, 8, 2, 64, 16
+    w = problem([40, 7], 1, h_q, h_kv, dim, 32, page, BF, 61)
+    pages, tokens = w["k_cache"].shape[0], 2
+    g = torch.Generator().manual_seed(62)
+    k, v = (torch.randn(tokens, h_kv, dim, generator=g).to(BF) for _ in range(2))
+    last = (w["cache_seqlens"] - 1).long()
+    slots = w["block_table"].gather(1, (last // page)[:, None])[:, 0].long() * page + last % page
+    t = {n: x.to(dev) for n, x in w.items()}
+    ops.kv_cache_write(slots.to(dev), k.to(dev), t["k_cache"], t["k_scale"], v.to(dev), t["v_cache"], t["v_scale"])
+    ref = run(t, dev)
+    write = tilelang.compile(P.kv_cache_write(tokens, h_kv, dim, pages, page, 32), out_idx=[2, 3, 5, 6], target="b200")
+    assert write(slots, k, w["k_cache"], w["k_scale"], v, w["v_cache"], w["v_scale"]) == 0
+    for n in ("k_cache", "v_cache"):
+        assert torch.equal(w[n], t[n].cpu())
+    attn = tilelang.compile(P.attn_decode_paged_int4(2, 1, h_q, h_kv, dim, pages, page, w["block_table"].shape[1], 32), out_idx=-1, target="b200")
+    out = torch.zeros_like(w["q"])
+    assert attn(w["q"], w["k_cache"], w["k_scale"], w["v_cache"], w["v_scale"], w["block_table"], w["cache_seqlens"], out) == 0
+    assert torch.equal(out.view(torch.int16), ref.view(torch.int16))
+    read = tilelang.compile(P.kv_cache_read(tokens, h_kv, dim, pages, page, 32), out_idx=[3, 6], target="b200")
+    ko, vo = torch.zeros_like(k), torch.zeros_like(v)
+    assert read(slots, w["k_cache"], w["k_scale"], ko, w["v_cache"], w["v_scale"], vo) == 0
+    codes, sc = O.quantise_u4g(k, 32)
+    assert torch.equal(ko.view(torch.int16), O.values_u4g(codes, sc).float().to(BF).view(torch.int16))
+    wo = (torch.randn(96, h_q * dim, generator=g) * 0.05).to(BF)
+    res, bias, c = torch.randn(2, 96, generator=g).to(BF), torch.randn(96, generator=g).to(BF), torch.zeros(2, 96, dtype=BF)
+    proj = tilelang.compile(P.gemm_epilogue(2, 96, h_q * dim, bias=True, activation="silu", residual=True, transpose_b=True), out_idx=-1, target="b200")
+    assert proj(out.view(2, -1), wo, bias, res, c) == 0
+    assert torch.allclose(c.double(), O.gemm_epilogue(out.view(2, -1), wo, bias, "silu", res, True), rtol=2.0 ** -8, atol=1e-4)

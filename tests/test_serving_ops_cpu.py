@@ -117,3 +117,28 @@ def test_the_oracle_quantiser_keeps_half_a_step():
     codes, sc = O.quantise_u4g(x, 32)
     step = sc[..., 0].double().repeat_interleave(32, -1)
     assert ((O.values_u4g(codes, sc) - x.double()).abs() <= step * (0.5 + 15 * 2.0 ** -10)).all()
+
+
+def test_generic_entry_point_reaches_them():
+    f = N.float_bits
+    assert N.run("kv_cache_write", [A, 0, A, A, 0, 0, 0], [4, 128, 0, 2, 64, 32, 4, 16, N.TL_U4G, N.TL_BF16], None) == -1 and "null" in N.last_error()
+    assert N.run("kv_cache_read", [A, A, A, A, 0, 0, 0], [4, 64, 0, 2, 64, 32, 4, 16, N.TL_U4G, N.TL_BF16], None) == -1
+    assert "overlap" in N.last_error()
+    meta = [2, 1, 4, 2, 80, 16, 320, 320, 16, 4, 8, f(0.1), N.TL_BF16, 1 << 30]
+    assert N.run("attn_decode_paged_int4", [A] * 9, meta, None) == -1 and "64, 128 or 256" in N.last_error()
+    assert N.run("gemm_epilogue", [A] * 5, [4, 8, 8, 1, 9, N.TL_BF16, N.TL_BF16], None) == -1 and "activation" in N.last_error()
+
+
+def test_library_programs_bind():
+    from tilelang import programs as P
+    from tilelang.engine.matcher import bind
+    for prog, entry, names in [
+            (P.kv_cache_write(3, 2, 64, 4, 16, 32), "tl_b200_kv_cache_write", "Slots K KCache KScale V VCache VScale"),
+            (P.kv_cache_write(3, 1, 576, 4, 64, cache_dtype="float8_e4m3"), "tl_b200_kv_cache_write", "Slots K KCache KScale"),
+            (P.kv_cache_read(3, 2, 64, 4, 16, 32), "tl_b200_kv_cache_read", "Slots KCache KScale K VCache VScale V"),
+            (P.attn_decode_paged_int4(2, 1, 8, 2, 128, 9, 16, 4), "tl_b200_attn_decode_paged_int4",
+             "Q KCache KScale VCache VScale BlockTable CacheSeqlens Out"),
+            (P.gemm_epilogue(4, 8, 16, bias=True, activation="gelu", residual=True), "tl_b200_gemm_epilogue", "A B Bias Residual C")]:
+        bound = bind(prog)
+        assert bound.entry_point == entry and [b.name for b in prog.params] == names.split()
+        assert bound.full_outputs == (not entry.startswith("tl_b200_kv"))

@@ -57,6 +57,18 @@ extern "C" int tl_b200_run(int kernel_id, void** a, const int64_t* m, void* stre
       return tl_b200_mla_decode_paged(a[0], a[1], (const float*)a[2], (const int32_t*)a[3], (const int32_t*)a[4], a[5],
                                       m[0], m[1], m[2], m[3], m[4], m[5], m[6], meta_f32(m[7]), (int)m[8], (int)m[9],
                                       a[6], m[10], stream);
+    case TL_B200_K_KV_CACHE_WRITE:
+      return tl_b200_kv_cache_write((const int64_t*)a[0], a[1], a[2], a[3], a[4], a[5], a[6], m[0], m[1], m[2], m[3], m[4], m[5], m[6],
+                                    m[7], (int)m[8], (int)m[9], stream);
+    case TL_B200_K_KV_CACHE_READ:
+      return tl_b200_kv_cache_read((const int64_t*)a[0], a[1], a[2], a[3], a[4], a[5], a[6], m[0], m[1], m[2], m[3], m[4], m[5], m[6],
+                                   m[7], (int)m[8], (int)m[9], stream);
+    case TL_B200_K_ATTN_DECODE_PAGED_INT4:
+      return tl_b200_attn_decode_paged_int4(a[0], a[1], a[2], a[3], a[4], (const int32_t*)a[5], (const int32_t*)a[6], a[7], m[0], m[1],
+                                            m[2], m[3], m[4], m[5], m[6], m[7], m[8], m[9], m[10], meta_f32(m[11]), (int)m[12], a[8],
+                                            m[13], stream);
+    case TL_B200_K_GEMM_EPILOGUE:
+      return tl_b200_gemm_epilogue(a[0], a[1], a[2], a[3], a[4], m[0], m[1], m[2], (int)m[3], (int)m[4], (int)m[5], (int)m[6], stream);
     default:
       return ::tl::fail(TL_B200_EINVAL, "tl_b200_run: unknown kernel id %d", kernel_id);
   }

@@ -69,7 +69,8 @@ PROTOTYPES = {
 # kernel ids of tl_b200_run (values of the TL_B200_K_* macros)
 KERNEL_IDS = {name: i + 1 for i, name in enumerate(
     ["rmsnorm", "rope", "swiglu", "reduce_rows", "unary", "binary", "rope_add", "copy2d", "fill", "gather_rows", "topk",
-     "gemm", "mlp_gate_up", "gemm_fp8_blockscale", "flash_attn_fwd", "mla_decode_dense", "mla_decode_paged"])}
+     "gemm", "mlp_gate_up", "gemm_fp8_blockscale", "flash_attn_fwd", "mla_decode_dense", "mla_decode_paged", "kv_cache_write",
+     "kv_cache_read", "attn_decode_paged_int4", "gemm_epilogue"])}
 
 
 def float_bits(v: float) -> int:

@@ -665,6 +665,21 @@ def _match_library_program(func: PrimFunc):
     if kernel == "mlp":
         return BoundKernel("mlp", "tl_b200_mlp_gate_up + tl_b200_gemm",
                            lambda out, x, wg, wu, wd: native.mlp(x, wg, wu, wd, out), facts)
+    if kernel == "kv_cache_write":         # padded tokens and all other rows of the caches stay as they are
+        return BoundKernel(kernel, "tl_b200_kv_cache_write", lambda *t: native.kv_cache_write(*t), facts, full_outputs=False)
+    if kernel == "kv_cache_read":
+        return BoundKernel(kernel, "tl_b200_kv_cache_read", lambda *t: native.kv_cache_read(*t), facts, full_outputs=False)
+    if kernel == "attn_decode_paged_int4":
+        return BoundKernel(kernel, "tl_b200_attn_decode_paged_int4",
+                           lambda *t: native.attn_decode_paged_int4(*t, softmax_scale=facts["softmax_scale"]), facts)
+    if kernel == "gemm_epilogue":
+        def run(a, b, *rest):
+            rest = list(rest)
+            bias = rest.pop(0) if facts["bias"] else None
+            residual = rest.pop(0) if facts["residual"] else None
+            return native.gemm_epilogue(a, b, rest[0], bias=bias, activation=facts["activation"], residual=residual,
+                                        transpose_b=facts["transpose_b"])
+        return BoundKernel(kernel, "tl_b200_gemm_epilogue", run, facts)
     raise UnsupportedProgram(f"unknown library kernel {kernel!r}")
 
 

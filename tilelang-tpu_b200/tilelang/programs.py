@@ -163,3 +163,59 @@ def mla_decode_paged(batch: int, heads: int, d: int, dv: int, num_pages: int, pa
     return _library_program("mla_decode_paged", params, "mla_decode_paged", batch=batch, heads=heads, d=d, dv=dv,
                             page_size=page_size, scaled=fp8,
                             softmax_scale=float(softmax_scale if softmax_scale is not None else d ** -0.5))
+
+
+def _cache_params(tokens: int, heads: int, dim: int, num_pages: int, page_size: int, group: int, dtype: str, cache_dtype: str):
+    """((rows, cache, scale) of keys, the same of values or nothing): a 4-bit cache holds both, an e4m3 cache latent rows."""
+    if cache_dtype == "uint8":
+        return [(f"{w}", (tokens, heads, dim), dtype, f"{w}Cache", (num_pages, heads, page_size, dim // 2), cache_dtype,
+                 f"{w}Scale", (num_pages, heads, page_size, dim // group, 2), dtype) for w in "KV"]
+    assert heads == 1, "an e4m3 cache has a single kv head"
+    return [("K", (tokens, dim), dtype, "KCache", (num_pages, page_size, dim), cache_dtype, "KScale", (num_pages, page_size), "float32")]
+
+
+def kv_cache_write(tokens: int, heads: int, dim: int, num_pages: int, page_size: int, group: int = 128, dtype: str = "bfloat16",
+                   cache_dtype: str = "uint8") -> PrimFunc:
+    """Quantise `tokens` rows of keys and values into a paged 4-bit cache (cache_dtype "uint8"), or of latent rows into the
+    e4m3 cache that mla_decode_paged reads ("float8_e4m3", heads 1); layouts as in tilelang.ops.kv_cache_write.  Parameters:
+    Slots, then K, KCache, KScale and for a 4-bit cache V, VCache, VScale."""
+    params = [("Slots", (tokens,), "int64")]
+    for side in _cache_params(tokens, heads, dim, num_pages, page_size, group, dtype, cache_dtype):
+        params += [side[0:3], side[3:6], side[6:9]]
+    return _library_program("kv_cache_write", params, "kv_cache_write", dim=dim, group=group, page_size=page_size, cache_dtype=cache_dtype)
+
+
+def kv_cache_read(tokens: int, heads: int, dim: int, num_pages: int, page_size: int, group: int = 128, dtype: str = "bfloat16",
+                  cache_dtype: str = "uint8") -> PrimFunc:
+    """The reverse of kv_cache_write.  Parameters: Slots, then KCache, KScale, K and for a 4-bit cache VCache, VScale, V."""
+    params = [("Slots", (tokens,), "int64")]
+    for side in _cache_params(tokens, heads, dim, num_pages, page_size, group, dtype, cache_dtype):
+        params += [side[3:6], side[6:9], side[0:3]]
+    return _library_program("kv_cache_read", params, "kv_cache_read", dim=dim, group=group, page_size=page_size, cache_dtype=cache_dtype)
+
+
+def attn_decode_paged_int4(batch: int, s_q: int, q_heads: int, kv_heads: int, dim: int, num_pages: int, page_size: int, max_pages: int,
+                           group: int = 128, dtype: str = "bfloat16", softmax_scale: float | None = None) -> PrimFunc:
+    """Attention of s_q new tokens per sequence over a paged 4-bit cache (tilelang.ops.attn_decode_paged_int4): Q
+    (batch, s_q, q_heads, dim), KCache, KScale, VCache, VScale, BlockTable (batch, max_pages), CacheSeqlens (batch,), Out."""
+    cache, scale = (num_pages, kv_heads, page_size, dim // 2), (num_pages, kv_heads, page_size, dim // group, 2)
+    rows = (batch, s_q, q_heads, dim)
+    return _library_program(
+        "attn_decode_paged_int4",
+        [("Q", rows, dtype), ("KCache", cache, "uint8"), ("KScale", scale, dtype), ("VCache", cache, "uint8"), ("VScale", scale, dtype),
+         ("BlockTable", (batch, max_pages), "int32"), ("CacheSeqlens", (batch,), "int32"), ("Out", rows, dtype)],
+        "attn_decode_paged_int4", softmax_scale=float(softmax_scale if softmax_scale is not None else dim ** -0.5))
+
+
+def gemm_epilogue(M: int, N: int, K: int, bias: bool = False, activation: str | None = None, residual: bool = False,
+                  transpose_b: bool = False, dtype: str = "bfloat16", out_dtype: str | None = None) -> PrimFunc:
+    """C = act(A B + Bias) + Residual (tilelang.ops.gemm_epilogue).  Parameters: A, B, then Bias (N,) and Residual (M, N)
+    where asked for, then C."""
+    params = [("A", (M, K), dtype), ("B", (N, K) if transpose_b else (K, N), dtype)]
+    if bias:
+        params.append(("Bias", (N,), dtype))
+    if residual:
+        params.append(("Residual", (M, N), dtype))
+    params.append(("C", (M, N), out_dtype or dtype))
+    return _library_program("gemm_epilogue", params, "gemm_epilogue", bias=bool(bias), activation=activation, residual=bool(residual),
+                            transpose_b=bool(transpose_b))
