@@ -145,6 +145,28 @@ def test_non_finite_values_that_are_seen(cuda_device):
     assert out[0, 0, 2:].isnan().all() and not out[0, 0, :2].isnan().any() and not out[1].isnan().any()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_queries_of_very_different_size(cuda_device, dtype):
+    """Heads of one kv head 2^10 (fp16) or 2^40 (bf16) apart: each against a tolerance of its own."""
+    w = problem([150], 1, 4, 1, 128, 64, 16, dtype, 26)
+    factor = torch.tensor([1.0, 2.0 ** -5, 2.0 ** -10, 2.0 ** 4] if dtype == HF else [1.0, 2.0 ** -20, 2.0 ** -40, 2.0 ** 4])
+    w["q"] = (w["q"].float() * factor[None, None, :, None]).to(dtype)
+    out, ref = run(w, cuda_device), reference(w)
+    for h in range(4):
+        one = {**w, "q": w["q"][:, :, h:h + 1]}
+        assert ((out[:, :, h].double() - ref[:, :, h]).abs() <= tolerance(one, ref[:, :, h])).all()
+
+
+def test_non_finite_queries(cuda_device):
+    w = problem([90], 1, 4, 1, 64, 32, 16, BF, 27)
+    ref = run(w, cuda_device)
+    w["q"][0, 0, 1, 3] = float("nan")
+    w["q"][0, 0, 2, 5] = float("inf")
+    out = run(w, cuda_device)
+    assert out[0, 0, 1].isnan().all() and out[0, 0, 2].isnan().all()             # infinity meets keys of both signs
+    assert torch.equal(out[0, 0, [0, 3]].view(torch.int16), ref[0, 0, [0, 3]].view(torch.int16))
+
+
 def test_bad_pages_and_lengths(cuda_device):
     """Ids outside the cache mask their tokens; a length beyond the table is cut to it, a negative one is empty."""
     w = problem([160, 160, 160, 64], 2, 8, 2, 64, 64, 16, BF, 23)

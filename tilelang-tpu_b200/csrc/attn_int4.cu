@@ -15,7 +15,7 @@
 // core multiplies exactly; the powers of two are taken back outside the loop.
 //   * K: a lane holds whole 32-bit words of a key; word & 0x000f000f are columns 0 and 4 of the word, one register of the A
 //     operand.  The columns of Q are permuted (and those of odd nibbles divided by 16) when they are loaded, once a
-//     sequence; a power of two per query tile brings Q into fp16's range, and what falls below it is 2^-35 of its largest.
+//     sequence; a power of two per query brings Q into fp16's range, and what falls below it is 2^-35 of its largest.
 //   * V: a register of the A operand is one column of two neighbouring tokens: one byte permute joins half words of the two.
 //   * Steps and minima never touch the codes:  q . k = s (q . c) + lo sum(q) per group, and the value's step multiplies p
 //     (rounded to fp16 with a power-of-two factor per warp that keeps p s in range: 2^-12 of each weight), its minimum
@@ -165,6 +165,7 @@ attn_int4_kernel(const AttnInt4Params p) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
   dependency_wait();
   dependency_release();
+  const int* lens = behind_wait(p.lens);
   uint8_t* tail = smem + kWarps * ST * Cfg::kStage;
   float* join = reinterpret_cast<float*>(tail);                  // [warps][join rows][pitch]
   float* join_m = join + kWarps * Cfg::kJoinRows * DIM;  // [warps][rows]
@@ -186,7 +187,7 @@ attn_int4_kernel(const AttnInt4Params p) {
     const int chunk = (p.batch + 32 * kWarps - 1) / (32 * kWarps);
     const int b0 = min((int)threadIdx.x * chunk, p.batch), b1 = min(b0 + chunk, p.batch);
     int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += units_of(mla_len(p.lens, b, p.len_cap));
+    for (int b = b0; b < b1; ++b) mine += units_of(mla_len(lens, b, p.len_cap));
     int64_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -342,13 +343,12 @@ attn_int4_kernel(const AttnInt4Params p) {
   while (left > 0) {
     const int rows = min(Cfg::kRows, p.rows - it.qt * Cfg::kRows);
     // the columns of Q as the B operand: permuted like the columns of the widened keys, times a power of two that brings the
-    // largest (finite) one to 2^14, odd nibbles' columns divided by 16
+    // query's largest (finite) one to 2^14, odd nibbles' columns divided by 16
     uint32_t qf[NT][DIM / 16][2];
-    float qsum[NG][NT][2], to_score;                  // scale * sum of q over the group for queries 2j, 2j + 1; scale of the dot products
+    float qsum[NG][NT][2], to_score[NT][2];           // for queries 2j, 2j + 1: scale * sum of q over the group; scale of the dot products
     int limit[NT][2];                                 // keys that queries 2j and 2j + 1 see
     {
       uint4 raw[NT][DIM / 32];
-      float big = 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int r = nt * 8 + g, row = it.qt * Cfg::kRows + r;
@@ -383,7 +383,8 @@ attn_int4_kernel(const AttnInt4Params p) {
         }
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float big = 0.f;
 #pragma unroll
         for (int x = 0; x < DIM / 32; ++x) {
           const uint32_t w[4] = {raw[nt][x].x, raw[nt][x].y, raw[nt][x].z, raw[nt][x].w};
@@ -394,12 +395,13 @@ attn_int4_kernel(const AttnInt4Params p) {
             big = fmaxf(big, fabsf(f.y) < INFINITY ? fabsf(f.y) : 0.f);
           }
         }
-      big = warp_max(big);
-      const int up = min(14 - ((int)(__float_as_uint(big) >> 23) - 127), 120);         // big < 2^128, so up >= -113
-      const float mul = __uint_as_float((uint32_t)(127 + up) << 23), mul16 = mul * 0.0625f;
-      to_score = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23) * 0x1p24f;
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        const int up = min(14 - ((int)(__float_as_uint(big) >> 23) - 127), 120);       // big < 2^128, so up >= -113
+        const float mul = __uint_as_float((uint32_t)(127 + up) << 23), mul16 = mul * 0.0625f;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int e = 0; e < 2; ++e)
+          to_score[nt][e] = p.scale_log2 * (__uint_as_float((uint32_t)(127 - __shfl_sync(0xffffffffu, up, (2 * j + e) * 4)) << 23) * 0x1p24f);
 #pragma unroll
         for (int x = 0; x < DIM / 32; ++x) {
           const float2 e01 = widen_scale<T>(raw[nt][x].x), e23 = widen_scale<T>(raw[nt][x].y), e45 = widen_scale<T>(raw[nt][x].z),
@@ -409,6 +411,7 @@ attn_int4_kernel(const AttnInt4Params p) {
           qf[nt][2 * x + 1][0] = pack_f16(e23.x * mul, e67.x * mul);
           qf[nt][2 * x + 1][1] = pack_f16(e23.y * mul16, e67.y * mul16);
         }
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -417,8 +420,8 @@ attn_int4_kernel(const AttnInt4Params p) {
           float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int ks = 0; ks < MG; ++ks) mma16816(d, ones, qf[nt][gg * MG + ks][0], qf[nt][gg * MG + ks][1]);
-          qsum[gg][nt][0] = d[0] * (to_score * 0x1p-24f);
-          qsum[gg][nt][1] = d[1] * (to_score * 0x1p-24f);
+          qsum[gg][nt][0] = d[0] * (to_score[nt][0] * 0x1p-24f);
+          qsum[gg][nt][1] = d[1] * (to_score[nt][1] * 0x1p-24f);
         }
     }
     const int all_see = it.len - p.s_q + 1;           // tokens before this one are seen by every query
@@ -496,14 +499,13 @@ attn_int4_kernel(const AttnInt4Params p) {
           for (int t = 0; t < 2; ++t) {
             const uint8_t* at = base[t] + 2 * Cfg::kCodes + (g * NG + gg) * 4;
             const float2 k0 = widen_scale<T>(*reinterpret_cast<const uint32_t*>(at)), k1 = widen_scale<T>(*reinterpret_cast<const uint32_t*>(at + 32 * NG));
-            const float a0 = k0.x * to_score, a1 = k1.x * to_score;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const float lo0 = k0.y * qsum[gg][nt][e], lo1 = k1.y * qsum[gg][nt][e];
-                sc[t][nt][e] = fmaf(a0, d[t][nt][e], gg ? sc[t][nt][e] + lo0 : lo0);
-                sc[t][nt][2 + e] = fmaf(a1, d[t][nt][2 + e], gg ? sc[t][nt][2 + e] + lo1 : lo1);
+                sc[t][nt][e] = fmaf(k0.x, d[t][nt][e] * to_score[nt][e], gg ? sc[t][nt][e] + lo0 : lo0);
+                sc[t][nt][2 + e] = fmaf(k1.x, d[t][nt][2 + e] * to_score[nt][e], gg ? sc[t][nt][2 + e] + lo1 : lo1);
               }
           }
         }
@@ -550,7 +552,7 @@ attn_int4_kernel(const AttnInt4Params p) {
             }
           }
         // ---- whether the running maximum or the factor f has to move -----------------------------------------------------
-        // the maximum may lag by 2^8: p stays below 256, and sums are exact whatever the reference is
+        // the maximum may lag by 2^4: p stays below 16, and sums are exact whatever the reference is
         float over = 0.f, rel[2][NT][4];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -561,7 +563,7 @@ attn_int4_kernel(const AttnInt4Params p) {
               rel[t][nt][e] = sc[t][nt][e] - m[nt][e & 1];
               over = fmaxf(over, rel[t][nt][e]);
             }
-        if (__any_sync(0xffffffffu, over > 8.f || big > most)) {
+        if (__any_sync(0xffffffffu, over > 4.f || big > most)) {
           float top[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -577,13 +579,13 @@ attn_int4_kernel(const AttnInt4Params p) {
           }
           float ratio = 1.f;                          // what the factor f changes by
           if (big > most) {
-            // f = 2^(4 - exponent): the largest step times f lies in [16, 32), and steps up to four times as large need no
-            // change; exponents of f stay normal
+            // f = 2^(8 - exponent): the largest step times f lies in [256, 512), and steps up to twice as large need no
+            // change, so a weight is below 2^14; one that is 2^-22 of the largest is still normal
             const int ex = max((int)(__float_as_uint(big) >> 23) - 127, -112);
-            const float f_new = __uint_as_float((uint32_t)(127 + 4 - min(ex, 127)) << 23);
+            const float f_new = __uint_as_float((uint32_t)(127 + 8 - min(ex, 127)) << 23);
             ratio = f == 0.f ? 0.f : f_new / f;
             f = f_new;
-            most = 64.f / f_new;                      // infinity at the upper end
+            most = 1024.f / f_new;                    // infinity at the upper end
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)

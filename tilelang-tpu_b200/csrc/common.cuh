@@ -50,6 +50,13 @@ void count_launch(int n = 1);
 __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void dependency_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// A pointer whose loads cannot be moved in front of the dependency_wait() before this (loads through the read-only path
+// are not held back by a memory clobber).
+template <typename T> __device__ __forceinline__ const T* behind_wait(const T* p) {
+  asm volatile("" : "+l"(p)::"memory");
+  return p;
+}
+
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
                                      Args... args) {

@@ -84,12 +84,13 @@ kv_write_u4g_kernel(const CacheArgs p) {
   constexpr int kLanes = DIM / 16, kGroupLanes = GROUP / 16;
   dependency_wait();
   dependency_release();
+  const int64_t* slots = behind_wait(p.slots);
   const Side side = blockIdx.y ? p.v : p.k;
   const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   const int part = threadIdx.x % kLanes;
   const uint32_t t = p.head_div(row);
   const int h = (int)(row - t * p.heads);
-  const int64_t slot = row < p.rows ? __ldg(p.slots + t) : -1;
+  const int64_t slot = row < p.rows ? __ldg(slots + t) : -1;
   const bool live = slot >= 0 && slot < p.total_slots;
   union { uint4 raw[2]; P v[8]; } in;
   in.raw[0] = in.raw[1] = make_uint4(0, 0, 0, 0);
@@ -163,6 +164,7 @@ kv_read_u4g_kernel(const CacheArgs p) {
   constexpr int kLanes = DIM / 16, kGroupLanes = GROUP / 16, kRows = 256 / kLanes;
   dependency_wait();
   dependency_release();
+  const int64_t* slots = behind_wait(p.slots);
   const Side side = blockIdx.y ? p.v : p.k;
   const int part = threadIdx.x % kLanes;
   uint32_t t[2];
@@ -173,7 +175,7 @@ kv_read_u4g_kernel(const CacheArgs p) {
     const uint32_t row = (blockIdx.x * 2 + k) * kRows + threadIdx.x / kLanes;
     t[k] = p.head_div(row);
     h[k] = (int)(row - t[k] * p.heads);
-    slot[k] = row < p.rows ? __ldg(p.slots + t[k]) : -1;
+    slot[k] = row < p.rows ? __ldg(slots + t[k]) : -1;
   }
   uint2 codes[2];
   P scale[2];
@@ -223,11 +225,12 @@ kv_write_e4m3_kernel(const CacheArgs p, const int dim) {
   using P = typename Pair<T>::type;
   dependency_wait();
   dependency_release();
+  const int64_t* slots = behind_wait(p.slots);
   const Side side = blockIdx.y ? p.v : p.k;
   const int lane = threadIdx.x % 32;
   const uint32_t t = blockIdx.x * 8 + threadIdx.x / 32;
   if (t >= p.tokens) return;                                   // the whole warp
-  const int64_t slot = __ldg(p.slots + t);
+  const int64_t slot = __ldg(slots + t);
   const T* src = reinterpret_cast<const T*>(side.x) + t * side.stride;
   union { uint4 raw; P v[4]; } in[PASSES];
 #pragma unroll
@@ -273,6 +276,7 @@ __global__ void __launch_bounds__(256)
 kv_read_e4m3_kernel(const CacheArgs p, const int dim, const int per_block) {
   dependency_wait();
   dependency_release();
+  const int64_t* slots = behind_wait(p.slots);
   const Side side = blockIdx.y ? p.v : p.k;
   const int vecs = dim / COLS;
   const uint32_t t0 = blockIdx.x * (uint32_t)per_block;
@@ -286,7 +290,7 @@ kv_read_e4m3_kernel(const CacheArgs p, const int dim, const int per_block) {
     const uint32_t in_block = p.vec_div((uint32_t)i);
     t[k] = t0 + in_block;
     col[k] = (i - (int)in_block * vecs) * COLS;
-    slot[k] = i < items ? __ldg(p.slots + t[k]) : -1;
+    slot[k] = i < items ? __ldg(slots + t[k]) : -1;
   }
   uint32_t codes[2][COLS / 4];
   float s[2];
