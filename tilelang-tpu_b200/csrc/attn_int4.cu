@@ -24,11 +24,11 @@
 //     output, 3.4e-4 without; of a bf16 output it is a fiftieth of the rounding either way, so there it is left out).
 // Every group of columns has its own MMAs, so a group's step can multiply the score or the weight.
 //
-// Work.  Sequences are cut into units of 64 tokens; the list of all (sequence, kv head, query tile, unit) is dealt out in
-// equal contiguous ranges to the CTAs, whatever the lengths.  Each of the four warps takes 16 tokens of a unit, through a
+// Work.  Sequences are cut into units of 128 tokens; the list of all (sequence, kv head, query tile, unit) is dealt out in
+// equal contiguous ranges to the CTAs, whatever the lengths.  Each of the four warps takes two tiles of 16 tokens of a unit, through a
 // ring of cp.async stages of its own that runs ahead across the ends of sequences: no warp waits for another inside a
 // segment (a ring of bulk copies shared by the warps was 40% slower: whoever refills a stage waits for the slowest).  Two
-// units at a time halve what control costs a token and give a warp two chains of MMAs to interleave; four such small CTAs
+// tiles at a time halve what control costs a token and give a warp two chains of MMAs to interleave; four such small CTAs
 // per SM cover each other's ends.  The warps' results are joined in shared memory,
 // a few rows at a time, at the end of a segment; a segment that CTAs share leaves fp32 partial sums, and the CTA that arrives last adds them up in
 // their fixed order, so the result does not depend on who that is.
@@ -56,7 +56,7 @@ struct AttnInt4Params {
   float* partial;                      // [2 * gridDim.x][kRows * (dim + 2)]
 };
 
-constexpr int kWarps = 4, kUnit = 16 * kWarps;
+constexpr int kWarps = 4, kHalf = 16 * kWarps, kUnit = 2 * kHalf;      // a warp's two tiles of a unit lie kHalf tokens apart
 
 // CTAs per SM, by the registers a thread needs: 128 (four CTAs), 168 with four groups' steps and sums (32 x 4096 tokens:
 // 63 us, 73 us with four CTAs that spill), 255 with twice the accumulators (24 sequences of 4 tokens, dim 64: 39 us, 42 us).
@@ -277,10 +277,11 @@ attn_int4_kernel(const AttnInt4Params p) {
     const uint32_t off = (uint32_t)t0 - p.page_div((uint32_t)t0) * (uint32_t)p.page_size;
     return ((uint32_t)page * p.h_kv + h) * (uint32_t)p.page_size + off;
   };
-  auto load = [&](const UnitIter& w, int stage, int page) {               // page: of the tile's first token, where tiles lie in one
+  // tile `half` of the unit; page: of its first token, where tiles lie in one
+  auto load = [&](const UnitIter& w, int half, int stage, int page) {
     uint8_t* const stage_ptr = ring + stage * Cfg::kStage;
     const uint32_t at = smem_u32(stage_ptr);
-    const int t0 = w.u * kUnit + warp * 16;
+    const int t0 = w.u * kUnit + half * kHalf + warp * 16;
     uint32_t mask = 0;
     if (tile_in_page) {
       const int live = mla_page_ok(page, p.num_pages) ? min(w.len - t0, 16) : 0;
@@ -322,8 +323,8 @@ attn_int4_kernel(const AttnInt4Params p) {
     }
     *reinterpret_cast<uint32_t*>(stage_ptr + Cfg::kMask) = mask;             // every lane, the same word
   };
-  auto page_at = [&](const UnitIter& w) {
-    const int t0 = w.u * kUnit + warp * 16;
+  auto page_at = [&](const UnitIter& w, int half) {
+    const int t0 = w.u * kUnit + half * kHalf + warp * 16;
     return tile_in_page && t0 < w.len ? __ldg(p.table + (int64_t)w.b * p.max_pages + p.page_div((uint32_t)t0)) : -1;
   };
   // the unit `by` behind `it`
@@ -363,13 +364,13 @@ attn_int4_kernel(const AttnInt4Params p) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) limit[nt][e] = it.len - p.s_q + (it.qt * Cfg::kRows + nt * 8 + 2 * j + e) / p.per + 1;
       }
-      if (first) {                                    // fill the ring: lane k looks up the page of unit k, all at once
+      if (first) {                                    // fill the ring: lane k looks up the page of tile k, all at once
         first = false;
-        const int page = lane < min(ST, left) ? page_at(ahead_of(it, lane)) : -1;
+        const int page = lane < min(ST, 2 * left) ? page_at(ahead_of(it, lane / 2), lane % 2) : -1;
 #pragma unroll 1
         for (int k = 0; k < ST; ++k) {
           const int pg = __shfl_sync(0xffffffffu, page, k);
-          if (k < left) load(ahead_of(it, k), k, pg);
+          if (k < 2 * left) load(ahead_of(it, k / 2), k % 2, k, pg);
           cp_async_commit();
         }
       }
@@ -445,12 +446,11 @@ attn_int4_kernel(const AttnInt4Params p) {
 
     const int first_u = it.u;                         // the first unit of this CTA's share of the segment
     while (true) {
-      const bool two = left > 1 && it.u + 1 < it.units;       // two units of the segment, or its last one
       const int stage1 = stage + 1 == ST ? 0 : stage + 1;
-      // Usually the two units ST further on belong to the segment, whole and in a page each: their pages are looked up here,
+      // Usually the two tiles ST further on belong to the segment, whole and in a page each: their pages are looked up here,
       // for the loads at the end of this round.
-      const int next0 = (it.u + ST) * kUnit + warp * 16, next1 = next0 + kUnit;
-      const bool easy = two && left > ST + 1 && tile_in_page && next1 + 16 <= it.len;
+      const int next0 = it.u * kUnit + ST * kHalf + warp * 16, next1 = next0 + kHalf;
+      const bool easy = 2 * left > ST + 1 && tile_in_page && next1 + 16 <= it.len;
       int page0 = 0, page1 = 0;
       if (easy) {
         const int* table = p.table + (int64_t)it.b * p.max_pages;
@@ -460,13 +460,12 @@ attn_int4_kernel(const AttnInt4Params p) {
       cp_async_wait<ST - 2>();
       __syncwarp();                                           // every lane's copies have landed
       const uint8_t* base[2] = {ring + stage * Cfg::kStage, ring + stage1 * Cfg::kStage};
-      const int t0 = it.u * kUnit + warp * 16;                // tokens t0 .. t0 + 15 and t0 + kUnit ..
+      const int t0 = it.u * kUnit + warp * 16;                // tokens t0 .. t0 + 15 and t0 + kHalf ..
       uint32_t mask[2];
       mask[0] = *reinterpret_cast<const uint32_t*>(base[0] + Cfg::kMask);
-      mask[1] = two ? *reinterpret_cast<const uint32_t*>(base[1] + Cfg::kMask) : 0u;
-      if (!two) base[1] = base[0];
+      mask[1] = *reinterpret_cast<const uint32_t*>(base[1] + Cfg::kMask);
       if (mask[0] | mask[1]) {                        // uniform in the warp, like `full`
-        const bool full = (mask[0] & mask[1]) == 0xffffu && t0 + kUnit + 16 <= all_see;       // every query sees every token
+        const bool full = (mask[0] & mask[1]) == 0xffffu && t0 + kHalf + 16 <= all_see;       // every query sees every token
         // ---- S^T = K Q^T, log2 domain -------------------------------------------------------------------------------------
         float sc[2][NT][4];
 #pragma unroll
@@ -520,7 +519,7 @@ attn_int4_kernel(const AttnInt4Params p) {
             v0[t][gg] = widen_scale<T>(*reinterpret_cast<const uint32_t*>(at));
             v1[t][gg] = widen_scale<T>(*reinterpret_cast<const uint32_t*>(at + 32 * NG));
           }
-        uint32_t see = 0xffffffffu;                   // bit 8 t + 4 nt + e: query 2j + (e & 1) sees token g + 8 (e >> 1) of unit t
+        uint32_t see = 0xffffffffu;                   // bit 8 t + 4 nt + e: query 2j + (e & 1) sees token g + 8 (e >> 1) of tile t
         if (!full) {
           see = 0;
 #pragma unroll
@@ -530,7 +529,7 @@ attn_int4_kernel(const AttnInt4Params p) {
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const bool ok2 = (e < 2 ? live0 : live1) && t0 + t * kUnit + g + (e < 2 ? 0 : 8) < limit[nt][e & 1];
+                const bool ok2 = (e < 2 ? live0 : live1) && t0 + t * kHalf + g + (e < 2 ? 0 : 8) < limit[nt][e & 1];
                 sc[t][nt][e] = ok2 ? sc[t][nt][e] : -INFINITY;
                 see |= (ok2 ? 1u : 0u) << (4 * NT * t + 4 * nt + e);
               }
@@ -684,7 +683,7 @@ attn_int4_kernel(const AttnInt4Params p) {
           }
         }
       }
-      __syncwarp();                                   // every lane has left the stages: the units ST further on go there
+      __syncwarp();                                   // every lane has left the stages: the tiles ST further on go there
       if (easy && mla_page_ok(page0, p.num_pages) && mla_page_ok(page1, p.num_pages)) {
         load_whole(stage, row_of(page0, it.h, next0));
         cp_async_commit();
@@ -692,17 +691,17 @@ attn_int4_kernel(const AttnInt4Params p) {
         cp_async_commit();
       } else {
 #pragma unroll 1
-        for (int k = 0; k < (two ? 2 : 1); ++k) {
-          if (left > ST + k) {
-            const UnitIter w = ahead_of(it, ST + k);
-            load(w, k ? stage1 : stage, page_at(w));
+        for (int k = 0; k < 2; ++k) {
+          if (ST + k < 2 * left) {
+            const UnitIter w = ahead_of(it, (ST + k) / 2);
+            load(w, (ST + k) % 2, k ? stage1 : stage, page_at(w, (ST + k) % 2));
           }
           cp_async_commit();
         }
       }
-      stage = two ? (stage1 + 1 == ST ? 0 : stage1 + 1) : stage1;
-      left -= two ? 2 : 1;
-      it.u += two ? 2 : 1;
+      stage = stage1 + 1 == ST ? 0 : stage1 + 1;
+      --left;
+      ++it.u;
       if (left == 0 || it.u == it.units) break;
     }
     --it.u;                                           // the segment's last unit here
