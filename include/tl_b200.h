@@ -304,7 +304,8 @@ int tl_b200_kv_cache_read(const int64_t* slots, const void* k_cache, const void*
  * tl_b200_mla_decode_paged_gqa); head h reads kv head h / (h_q / h_kv).  K and V are caches of format TL_U4G (above).
  * q [batch, s_q, h_q, dim] with q_stride_batch / q_stride_token elements between sequences / tokens (heads of a token
  * contiguous), out dense.  A row that sees no key is zero; lengths are clamped to the table's width, tokens of a page id
- * outside the cache are masked, and cache rows behind a sequence's last token may hold anything.
+ * outside the cache are masked, and cache rows behind a sequence's last token may hold anything.  Queries up to 2^117 in
+ * size (a larger finite one may give NaN).
  * `workspace`: tl_b200_attn_decode_paged_int4_workspace_bytes(...) bytes (0 for sizes the call refuses), 16-byte aligned.
  * Its first TL_B200_ATTN_INT4_ZERO_BYTES bytes must be zero before the first call and are zero again after each call,
  * whatever the sizes of the calls; calls that may overlap on the GPU need workspaces of their own.                 */
@@ -320,7 +321,7 @@ int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache, const voi
 /* ---- dense GEMM with epilogue -------------------------------------------------------
  * c = act(a b + bias) + residual, products accumulated and the epilogue evaluated in fp32, one rounding to out_dtype.
  * a, b, trans_b, in_dtype and out_dtype as in tl_b200_gemm (TL_F32, TL_F16, TL_BF16); bias [n] and residual [m, n] of
- * in_dtype, either may be NULL; residual may be c itself where out_dtype is in_dtype.                              */
+ * in_dtype, either may be NULL; residual may be c itself where out_dtype is in_dtype, but not overlap it otherwise. */
 #define TL_B200_ACT_NONE 0
 #define TL_B200_ACT_RELU 1
 #define TL_B200_ACT_GELU 2        /* x/2 (1 + erf(x / sqrt 2)) */

@@ -142,3 +142,12 @@ def test_library_programs_bind():
         bound = bind(prog)
         assert bound.entry_point == entry and [b.name for b in prog.params] == names.split()
         assert bound.full_outputs == (not entry.startswith("tl_b200_kv"))
+
+
+def test_sizes_at_the_ends_of_the_ranges():
+    assert write(page=2 ** 31, pages=0) == -1 and "too large" in N.last_error()
+    assert write(pages=0, kc=None, ks=None) == 0                 # no slot lies in a cache without pages
+    big = 2 ** 24 - 1                                            # the product of all three wraps 64 bits
+    assert attn(batch=big, s_q=big, h_q=65536) == -1 and "too large" in N.last_error()
+    assert N.load().tl_b200_attn_decode_paged_int4_workspace_bytes(big, big, 65536, 2, 64) == 0
+    assert gemm(n=2 ** 31 - 8) == -1 and "2^31" in N.last_error()

@@ -213,7 +213,7 @@ attn_int4_kernel(const AttnInt4Params p) {
     if (base * per_unit <= start && start < (base + mine) * per_unit) {  // exactly one thread
       int b = b0, units = 0;
       for (; b < b1; ++b) {
-        units = units_of(mla_len(p.lens, b, p.len_cap));
+        units = units_of(mla_len(lens, b, p.len_cap));
         if (start < (base + units) * per_unit) break;
         base += units;
       }
@@ -227,7 +227,7 @@ attn_int4_kernel(const AttnInt4Params p) {
     __syncthreads();
     left = (int)(end - start);                                           // the host checks that it fits
     it.b = sh.first_b;
-    it.len = mla_len(p.lens, it.b, p.len_cap);
+    it.len = mla_len(lens, it.b, p.len_cap);
     it.units = units_of(it.len);
     const int64_t off = start - sh.seq_base;
     const int seg = off >> 32 ? (int)(off / it.units) : (int)((uint32_t)off / (uint32_t)it.units);
@@ -946,7 +946,7 @@ static int launch_i4_dim(const AttnInt4Params& p, const I4Plan& plan, int64_t di
 
 static bool i4_sizes_ok(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int64_t dim) {
   return batch >= 0 && s_q >= 0 && h_q >= 1 && h_kv >= 1 && h_q % h_kv == 0 && batch < (1 << 24) && s_q < (1 << 24) && h_q <= 65536 &&
-         batch * s_q * h_q < (1ll << 31) && (dim == 64 || dim == 128 || dim == 256);
+         batch * s_q < (1ll << 31) && batch * s_q * h_q < (1ll << 31) && (dim == 64 || dim == 128 || dim == 256);
 }
 
 }  // namespace tl
@@ -970,7 +970,7 @@ extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache
   TL_REQUIRE((group == 32 || group == 64 || group == 128) && group <= dim,
              "attn_decode_paged_int4: groups of 32, 64 or 128 columns, at most the row");
   TL_REQUIRE(h_q % h_kv == 0, "attn_decode_paged_int4: h_q must be a multiple of h_kv");
-  TL_REQUIRE(batch < (1 << 24) && s_q < (1 << 24) && h_q <= 65536 && batch * s_q * h_q < (1ll << 31),
+  TL_REQUIRE(batch < (1 << 24) && s_q < (1 << 24) && h_q <= 65536 && batch * s_q < (1ll << 31) && batch * s_q * h_q < (1ll << 31),
              "attn_decode_paged_int4: size too large");
   TL_REQUIRE(num_pages < (1ll << 31) && page_size < (1ll << 31) && num_pages * page_size < (1ll << 31) && max_pages_per_seq < (1ll << 31) &&
                  num_pages * page_size * h_kv < (1ll << 32),            // 2^32 rows of 32 bytes and their values are over 256 GB

@@ -438,7 +438,8 @@ using namespace tl;
 extern "C" int tl_b200_gemm_epilogue(const void* a, const void* b, const void* bias, const void* residual, void* c, int64_t m, int64_t n,
                                      int64_t k, int trans_b, int act, int in_dtype, int out_dtype, void* stream) {
   TL_REQUIRE(m >= 0 && n >= 0 && k >= 0, "gemm_epilogue: negative size");
-  TL_REQUIRE(m < (1ll << 31) && n < (1ll << 31) && k < (1ll << 31), "gemm_epilogue: dimension exceeds 2^31");
+  constexpr int64_t kMost = (1ll << 31) - (1 << 23);              // sizes rounded up to tiles and grid strides stay below 2^31
+  TL_REQUIRE(m <= kMost && n <= kMost && k <= kMost, "gemm_epilogue: dimension exceeds 2^31 - 2^23");
   TL_REQUIRE(act >= TL_B200_ACT_NONE && act <= TL_B200_ACT_SILU, "gemm_epilogue: unknown activation %d", act);
   TL_REQUIRE(in_dtype == TL_F32 || in_dtype == TL_F16 || in_dtype == TL_BF16, "gemm_epilogue: unsupported input dtype %d", in_dtype);
   TL_REQUIRE(out_dtype == in_dtype || out_dtype == TL_F32, "gemm_epilogue: output must be the input type or float32");

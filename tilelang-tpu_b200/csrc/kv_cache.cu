@@ -387,9 +387,9 @@ static int cache_call(const char* who, const int64_t* slots, int64_t tokens, con
     TL_REQUIRE(heads == 1, "%s: an e4m3 cache has a single kv head", who);
     TL_REQUIRE(dim % 8 == 0 && dim <= 1024, "%s: e4m3 rows have a multiple of 8 columns, at most 1024", who);
   }
-  TL_REQUIRE(num_pages <= (1ll << 31) && page_size <= (1ll << 31) && num_pages * page_size < (1ll << 31), "%s: cache too large", who);
+  TL_REQUIRE(num_pages < (1ll << 31) && page_size < (1ll << 31) && num_pages * page_size < (1ll << 31), "%s: cache too large", who);
   TL_REQUIRE(heads <= 65536 && tokens < (1ll << 31) && tokens * heads < (1ll << 31) - 256, "%s: size too large", who);
-  if (tokens == 0) return TL_B200_OK;
+  if (tokens == 0 || num_pages == 0) return TL_B200_OK;        // no slot is inside a cache without pages
   const bool both = v != nullptr || v_cache != nullptr || v_scale != nullptr;
   TL_REQUIRE(slots && k && k_cache && k_scale, "%s: null tensor pointer", who);
   TL_REQUIRE(!both || (v && v_cache && v_scale), "%s: null tensor pointer", who);
