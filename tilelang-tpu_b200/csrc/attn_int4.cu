@@ -25,13 +25,18 @@
 // Every group of columns has its own MMAs, so a group's step can multiply the score or the weight.
 //
 // Work.  Sequences are cut into units of 128 tokens; the list of all (sequence, kv head, query tile, unit) is dealt out in
-// equal contiguous ranges to the CTAs, whatever the lengths.  Each of the four warps takes two tiles of 16 tokens of a unit, through a
+// equal contiguous ranges to teams of four warps, whatever the lengths.  Each warp takes two tiles of 16 tokens of a unit, through a
 // ring of cp.async stages of its own that runs ahead across the ends of sequences: no warp waits for another inside a
 // segment (a ring of bulk copies shared by the warps was 40% slower: whoever refills a stage waits for the slowest).  Two
-// tiles at a time halve what control costs a token and give a warp two chains of MMAs to interleave; four such small CTAs
-// per SM cover each other's ends.  The warps' results are joined in shared memory,
-// a few rows at a time, at the end of a segment; a segment that CTAs share leaves fp32 partial sums, and the CTA that arrives last adds them up in
-// their fixed order, so the result does not depend on who that is.
+// tiles at a time halve what control costs a token and give a warp two chains of MMAs to interleave; the teams of an SM
+// cover each other's ends.  The warps' results are joined in shared memory,
+// a few rows at a time, at the end of a segment; a segment that teams share leaves fp32 partial sums, and the team that arrives
+// last adds them up in their fixed order, so the result does not depend on who that is.
+//
+// Measured (bf16, dim 128, one group, 32 query and 8 kv heads, at a copy rate of 6.55 TB/s): 64 sequences of 2048 to 12288
+// tokens 114 us, 4.4 TB/s of cache; one of 131077 tokens 49 us, 3.1 TB/s; one of 777 tokens 10.9 us.  A round of 32 tokens
+// issues some 300 instructions a warp, and issue slots are what the long loop is bound by; about 18 us of a call are the
+// first loads, the joins and the launch.
 #include "sm100.cuh"
 #include "mla_common.cuh"
 
@@ -52,15 +57,15 @@ struct AttnInt4Params {
   int rows, q_tiles;                   // query rows of a kv head (s_q * per), tiles of them
   FastDiv page_div;                    // t / page_size
   float scale_log2;
-  int* counters;                       // three per CTA, zero between calls
-  float* partial;                      // [2 * gridDim.x][kRows * (dim + 2)]
+  int* counters;                       // three per team, zero between calls
+  float* partial;                      // [2 * teams][kRows * (dim + 2)]
 };
 
 constexpr int kWarps = 4, kHalf = 16 * kWarps, kUnit = 2 * kHalf;      // a warp's two tiles of a unit lie kHalf tokens apart
 
-// CTAs per SM, by the registers a thread needs: 128 (four CTAs), 168 with four groups' steps and sums (32 x 4096 tokens:
-// 63 us, 73 us with four CTAs that spill), 255 with twice the accumulators (24 sequences of 4 tokens, dim 64: 39 us, 42 us).
-__host__ __device__ constexpr int i4_ctas(int dim, int groups, int nt) {
+// Teams per SM, by the registers a thread needs: 128 (four teams), 168 with four groups' steps and sums (32 x 4096 tokens:
+// 62 us, 73 us with four teams that spill), 255 with twice the accumulators (24 sequences of 4 tokens, dim 64: 39 us, 42 us).
+__host__ __device__ constexpr int i4_teams(int dim, int groups, int nt) {
   return nt == 2 || dim == 256 ? 2 : dim == 128 && groups == 4 ? 3 : 4;
 }
 
@@ -73,10 +78,10 @@ template <int DIM, int GROUP, int NT> struct I4Cfg {
   static constexpr int kRows = 8 * NT;
   static constexpr int kJoinRows = (DIM == 64 ? 4 : 2) * NT;            // rows joined at a time
   static constexpr int kJoin = kWarps * (kJoinRows * DIM + 2 * kRows) * 4;      // partial rows, maxima and sums of the warps
-  static constexpr int kCtas = i4_ctas(DIM, kGroups, NT);               // resident per SM
-  static constexpr int kFit = (228 * 1024 / kCtas - 1024 - kJoin - 128) / (kWarps * kStage);
+  static constexpr int kTeams = i4_teams(DIM, kGroups, NT);             // of four warps, on an SM
+  static constexpr int kFit = (228 * 1024 / kTeams - 1024 - kJoin - 256) / (kWarps * kStage);
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
-  static constexpr int kSmem = kWarps * kStages * kStage + kJoin + 128;
+  static constexpr int kSmem = (kWarps * kStages * kStage + kJoin + 128 + 127) / 128 * 128;             // of a team
   static_assert(kStages >= 4, "two stages are worked on while two are on their way");
 };
 
@@ -155,14 +160,23 @@ __device__ __forceinline__ bool advance(UnitIter& it, const AttnInt4Params& p) {
   return true;
 }
 
-template <typename T, int DIM, int GROUP, int NT>
-__global__ void __launch_bounds__(32 * kWarps, I4Cfg<DIM, GROUP, NT>::kCtas)
+template <typename T, int DIM, int GROUP, int NT, int TEAMS>
+__global__ void __launch_bounds__(32 * kWarps * TEAMS, I4Cfg<DIM, GROUP, NT>::kTeams / TEAMS)
 attn_int4_kernel(const AttnInt4Params p) {
   using Cfg = I4Cfg<DIM, GROUP, NT>;
   constexpr int NG = Cfg::kGroups, ST = Cfg::kStages, MT = DIM / 16, MG = GROUP / 16;
   constexpr bool kCentre = std::is_same<T, __half>::value;       // the weights' rounding meets c - 8 (see above); bf16 outputs do not show it
-  extern __shared__ __align__(128) uint8_t smem[];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4;
+  extern __shared__ __align__(128) uint8_t all_smem[];
+  // With TEAMS > 1, warp w of the block runs on scheduler w % 4 and is the (w / 4)-th oldest there; a team has one warp on each scheduler,
+  // each of another age.
+  const int scheduler = threadIdx.x / 32 % 4, team = TEAMS == 1 ? 0 : (threadIdx.x / 128 + scheduler) % TEAMS;
+  const int warp = scheduler, lane = threadIdx.x % 32, g = lane / 4, j = lane % 4, tid = warp * 32 + lane;
+  const int me = team * gridDim.x + blockIdx.x, all_teams = gridDim.x * TEAMS;      // few of them go to SMs of their own
+  uint8_t* const smem = all_smem + team * Cfg::kSmem;
+  auto team_sync = [&]() {
+    if constexpr (TEAMS == 1) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(32 * kWarps) : "memory");
+  };
   dependency_wait();
   dependency_release();
   const int* lens = behind_wait(p.lens);
@@ -179,13 +193,13 @@ attn_int4_kernel(const AttnInt4Params p) {
   Shared& sh = *reinterpret_cast<Shared*>(join_l + kWarps * Cfg::kRows);
   uint8_t* const ring = smem + warp * ST * Cfg::kStage;                    // this warp's stages
 
-  // ---- this CTA's range of the list --------------------------------------------------------------------------------
+  // ---- this team's range of the list --------------------------------------------------------------------------------
   UnitIter it;
-  int left;                                            // units of this CTA still to do
+  int left;                                            // units of this team still to do
   {
     const int64_t per_unit = (int64_t)p.h_kv * p.q_tiles;
     const int chunk = (p.batch + 32 * kWarps - 1) / (32 * kWarps);
-    const int b0 = min((int)threadIdx.x * chunk, p.batch), b1 = min(b0 + chunk, p.batch);
+    const int b0 = min((int)tid * chunk, p.batch), b1 = min(b0 + chunk, p.batch);
     int64_t mine = 0;
     for (int b = b0; b < b1; ++b) mine += units_of(mla_len(lens, b, p.len_cap));
     int64_t incl = mine;
@@ -195,20 +209,20 @@ attn_int4_kernel(const AttnInt4Params p) {
       if (lane >= o) incl += v;
     }
     if (lane == 31) sh.sums[warp] = incl;
-    __syncthreads();
+    team_sync();
     int64_t before = 0, total = 0;
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) before += sh.sums[w];
       total += sh.sums[w];
     }
     total *= per_unit;
-    const int64_t ctas = total < gridDim.x ? total : gridDim.x;          // every one of them has a unit
-    if (blockIdx.x >= ctas) return;                                      // the whole CTA
-    // CTA i begins at floor(i * total / ctas)
+    const int64_t ctas = total < all_teams ? total : all_teams;          // every one of them has a unit
+    if (me >= ctas) return;                                              // the whole team
+    // team i begins at floor(i * total / ctas)
     const int64_t quot = total >> 32 ? total / ctas : (int64_t)((uint32_t)total / (uint32_t)ctas);
-    const uint32_t rest = (uint32_t)(total - quot * ctas);               // times a CTA number: below 2^32
-    const int64_t start = blockIdx.x * quot + blockIdx.x * rest / (uint32_t)ctas;
-    const int64_t end = (blockIdx.x + 1) * quot + (blockIdx.x + 1) * rest / (uint32_t)ctas;
+    const uint32_t rest = (uint32_t)(total - quot * ctas);               // times a team's number: below 2^32
+    const int64_t start = me * quot + me * rest / (uint32_t)ctas;
+    const int64_t end = (me + 1) * quot + (me + 1) * rest / (uint32_t)ctas;
     int64_t base = before + incl - mine;
     if (base * per_unit <= start && start < (base + mine) * per_unit) {  // exactly one thread
       int b = b0, units = 0;
@@ -224,7 +238,7 @@ attn_int4_kernel(const AttnInt4Params p) {
       sh.start = start;
       sh.end = end;
     }
-    __syncthreads();
+    team_sync();
     left = (int)(end - start);                                           // the host checks that it fits
     it.b = sh.first_b;
     it.len = mla_len(lens, it.b, p.len_cap);
@@ -444,7 +458,7 @@ attn_int4_kernel(const AttnInt4Params p) {
         for (int e = 0; e < 4; ++e) acc[t][nt][e] = 0.f;
     }
 
-    const int first_u = it.u;                         // the first unit of this CTA's share of the segment
+    const int first_u = it.u;                         // the first unit of this team's share of the segment
     while (true) {
       const int stage1 = stage + 1 == ST ? 0 : stage + 1;
       // Usually the two tiles ST further on belong to the segment, whole and in a page each: their pages are looked up here,
@@ -722,7 +736,7 @@ attn_int4_kernel(const AttnInt4Params p) {
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) join_m[warp * Cfg::kRows + nt * 8 + 2 * j + e] = m[nt][e];
-    __syncthreads();
+    team_sync();
     const float inv_f = f == 0.f ? 0.f : 1.f / f;
     float part[NT][2];                                // this warp's weight in the joint result
 #pragma unroll
@@ -746,7 +760,7 @@ attn_int4_kernel(const AttnInt4Params p) {
       *reinterpret_cast<uint2*>(dst) = o.raw;
     };
     constexpr int kSlot = Cfg::kRows * (DIM + 2);      // floats of one partial result: rows, maxima, sums
-    float* slot = p.partial + ((int64_t)blockIdx.x * 2 + (seg_first + first_u > sh.start ? 1 : 0)) * kSlot;
+    float* slot = p.partial + ((int64_t)me * 2 + (seg_first + first_u > sh.start ? 1 : 0)) * kSlot;
 #pragma unroll 1
     for (int r0 = 0; r0 < rows; r0 += Cfg::kJoinRows) {
 #pragma unroll
@@ -768,9 +782,9 @@ attn_int4_kernel(const AttnInt4Params p) {
               }
           }
         }
-      __syncthreads();
+      team_sync();
       // the segment's rows: to the output, or to the partial sums
-      for (int i = threadIdx.x; i < min(rows - r0, Cfg::kJoinRows) * (DIM / 4); i += 32 * kWarps) {
+      for (int i = tid; i < min(rows - r0, Cfg::kJoinRows) * (DIM / 4); i += 32 * kWarps) {
         const int rj = i / (DIM / 4), r = r0 + rj, d = i % (DIM / 4) * 4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         float sum = 0.f, top = join_m[r];
@@ -792,51 +806,47 @@ attn_int4_kernel(const AttnInt4Params p) {
           }
         }
       }
-      __syncthreads();                                 // the join buffer is free again
+      team_sync();                                 // the join buffer is free again
     }
     if (!whole) {
-      // CTAs c0 .. c1 share the segment.  They are taken in groups of sixteen neighbours: the last of a group to arrive adds
-      // its partial results up into the slot of the group's first CTA, the last group to be done adds up the groups'.  (One
-      // CTA adding up 74 takes 12 us.)
+      // Teams c0 .. c1 share the segment.  They are taken in groups of sixteen neighbours: the last of a group to arrive adds
+      // its partial results up into the slot of the group's first team, the last group to be done adds up the groups'.  (One
+      // team adding up 74 takes 12 us.)
       const int64_t total = sh.total, ctas = sh.ctas;
-      const int c0 = seg_first >= sh.start ? (int)blockIdx.x : (int)(((seg_first + 1) * ctas - 1) / total);
-      const int c1 = seg_end <= sh.end ? (int)blockIdx.x : (int)((seg_end * ctas - 1) / total);
-      // the segment is the last of CTA c0 (slot 1 unless it is its first as well) and the first of all others (slot 0)
+      const int c0 = seg_first >= sh.start ? me : (int)(((seg_first + 1) * ctas - 1) / total);
+      const int c1 = seg_end <= sh.end ? me : (int)((seg_end * ctas - 1) / total);
+      // the segment is the last of team c0 (slot 1 unless it is its first as well) and the first of all others (slot 0)
       const int in_c0 = seg_first > (int64_t)c0 * total / ctas ? 1 : 0;
       auto slot_of = [&](int c) { return p.partial + ((int64_t)c * 2 + (c == c0 ? in_c0 : 0)) * kSlot; };
       constexpr int kGroup = 16;
-      const int lead = max(c0, (int)blockIdx.x / kGroup * kGroup), tail = min(c1, (int)blockIdx.x / kGroup * kGroup + kGroup - 1);
+      const int lead = max(c0, me / kGroup * kGroup), tail = min(c1, me / kGroup * kGroup + kGroup - 1);
       const int groups = c1 / kGroup - c0 / kGroup + 1;
-      // Three counters a CTA.  Only one shared segment begins in a CTA's range (its last), and a group of another segment
-      // that begins with this CTA goes by the counter of those that only pass through.
+      // Three counters a team.  Only one shared segment begins in a team's range (its last), and a group of another segment
+      // that begins with this team goes by the counter of those that only pass through.
       int* const group_counter = p.counters + 3 * lead + (lead == c0 ? 1 : 0);
       int* const seg_counter = p.counters + 3 * c0 + 2;
-      auto arrive = [&](int* counter, int others) {    // behind a barrier: the fence covers every thread's stores
-        if (threadIdx.x == 0) {
-          __threadfence();
-          sh.last = atomicAdd(counter, 1) == others;
+      auto arrive = [&](int* counter, int others) {    // behind a barrier, so it speaks for every thread's stores
+        if (tid == 0) {
+          int seen;                                    // releases this team's stores, acquires those of the teams before
+          asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(counter) : "memory");
+          sh.last = seen == others;
           if (sh.last) *counter = 0;                   // ready for the next call
-          __threadfence();
         }
-        __syncthreads();
+        team_sync();
         return sh.last;
       };
       // Adds up `many` partial results in their order; `emit(r, d, sums, sum, top)` takes four columns of a row.
       auto add_up = [&](int many, auto slot_at, auto emit) {
-        constexpr int kRowThreads = DIM / 4 < 32 ? DIM / 4 : 32;         // neighbouring lanes with one row
-        constexpr int kBatch = 8;                      // loads on their way at once, in the last batch too
+        // Four at a time, all on their way at once, in the last batch too; most segments are shared by two or three (16 at a
+        // time: 1 x 777 tokens 12.3 us for 10.9, and the registers make the loop above spill)
+        constexpr int kBatch = 4;
         const int items = rows * (DIM / 4), rounds = (items + 32 * kWarps - 1) / (32 * kWarps);
         for (int k = 0; k < rounds; ++k) {
-          const int i = k * 32 * kWarps + threadIdx.x;
+          const int i = k * 32 * kWarps + tid;
           const bool on = i < items;
           const int r = on ? i / (DIM / 4) : 0, d = i % (DIM / 4) * 4;
-          float top = -FLT_MAX;
-#pragma unroll 2
-          for (int c = lane % kRowThreads; c < many; c += kRowThreads) top = fmaxf(top, __ldcg(slot_at(c) + Cfg::kRows * DIM + r));
-#pragma unroll
-          for (int o = 1; o < kRowThreads; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          float sum = 0.f;
+          float sum = 0.f, top = -FLT_MAX;
           for (int c = 0; c < many; c += kBatch) {
             float4 x[kBatch];
             float mc[kBatch], lc[kBatch];
@@ -847,6 +857,13 @@ attn_int4_kernel(const AttnInt4Params p) {
               lc[q] = __ldcg(s + Cfg::kRows * (DIM + 1) + r);
               x[q] = __ldcg(reinterpret_cast<const float4*>(s + r * DIM + d));
             }
+            float higher = top;
+#pragma unroll
+            for (int q = 0; q < kBatch; ++q) higher = fmaxf(higher, mc[q]);
+            const float keep = ex2_approx(top - higher);
+            top = higher;
+            v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
+            sum *= keep;
 #pragma unroll
             for (int q = 0; q < kBatch; ++q)
               if (c + q < many) {
@@ -877,24 +894,24 @@ attn_int4_kernel(const AttnInt4Params p) {
               join_m[r] = top;
             }
           });
-          __syncthreads();
-          if (threadIdx.x < rows) {
-            __stcg(into + Cfg::kRows * DIM + threadIdx.x, join_m[threadIdx.x]);
-            __stcg(into + Cfg::kRows * (DIM + 1) + threadIdx.x, join_l[threadIdx.x]);
+          team_sync();
+          if (tid < rows) {
+            __stcg(into + Cfg::kRows * DIM + tid, join_m[tid]);
+            __stcg(into + Cfg::kRows * (DIM + 1) + tid, join_l[tid]);
           }
-          __syncthreads();
+          team_sync();
           if (arrive(seg_counter, groups - 1))
             add_up(groups, [&](int i) { return slot_of(max(c0, (c0 / kGroup + i) * kGroup)); }, to_out);
         }
       }
     }
-    __syncthreads();                                   // sh, the maxima and the join buffer are free again
+    team_sync();                                   // sh, the maxima and the join buffer are free again
     if (left > 0) {
       const int b = it.b;
       const int64_t next = (int64_t)it.units * p.h_kv * p.q_tiles;
       advance(it, p);
       if (it.b != b) {                                 // read again only behind the barriers of the next segment's end
-        if (threadIdx.x == 0) sh.seq_base += next;
+        if (tid == 0) sh.seq_base += next;
       }
     }
   }
@@ -913,17 +930,32 @@ static I4Plan i4_plan(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int
   const int64_t rows = s_q * (h_q / h_kv);
   r.tile_rows = q_tile_rows(rows, dim);
   r.q_tiles = (int)((rows + r.tile_rows - 1) / r.tile_rows);
-  r.grid = sm_count() * i4_ctas((int)dim, (int)(dim / group), r.tile_rows / 8);
+  r.grid = sm_count() * i4_teams((int)dim, (int)(dim / group), r.tile_rows / 8);
   r.bytes = TL_B200_ATTN_INT4_ZERO_BYTES + (int64_t)r.grid * 2 * r.tile_rows * (dim + 2) * 4;
   return r;
 }
 
 template <typename T, int DIM, int GROUP, int NT>
 static int launch_i4(const AttnInt4Params& p, int grid, cudaStream_t s) {
-  auto kernel = attn_int4_kernel<T, DIM, GROUP, NT>;
-  constexpr int smem = I4Cfg<DIM, GROUP, NT>::kSmem;
-  TL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  TL_CUDA(launch_overlapped(kernel, dim3(grid), dim3(32 * kWarps), smem, s, p));
+  auto launch = [&](auto teams) {
+    constexpr int N = decltype(teams)::value, smem = N * I4Cfg<DIM, GROUP, NT>::kSmem;
+    auto kernel = attn_int4_kernel<T, DIM, GROUP, NT, N>;
+    if (const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return rc;
+    return launch_overlapped(kernel, dim3(grid / N), dim3(32 * kWarps * N), smem, s, p);
+  };
+  cudaError_t rc;
+  // Four small teams to an SM are one CTA where there are many segments: the schedulers favour the oldest warps, and as CTAs
+  // of their own the teams end at 80, 92, 105 and 118 us (64 sequences of 2048 to 12288 tokens: 120 us; 115 us as one CTA,
+  // whose teams have a warp of every age).  With few, long segments the early ends pay, since each sets off an addition of
+  // partial results: one sequence of 131077 tokens 49.4 and 52.1 us, 24 of 4096 44.5 and 44.8 us, 32 of 4096 50.8 and 50.0 us.
+  // Two and three teams an SM: 52.0 us as CTAs and 54.4 us as one (16 x 4096 tokens, dim 256).
+  if constexpr (I4Cfg<DIM, GROUP, NT>::kTeams == 4) {
+    if ((int64_t)p.batch * p.h_kv * p.q_tiles * 3 >= grid) rc = launch(std::integral_constant<int, 4>());
+    else rc = launch(std::integral_constant<int, 1>());
+  } else {
+    rc = launch(std::integral_constant<int, 1>());
+  }
+  TL_CUDA(rc);
   TL_LAUNCH_CHECK("attn_int4_kernel");
   return TL_B200_OK;
 }
