@@ -34,8 +34,8 @@
 // last adds them up in their fixed order, so the result does not depend on who that is.
 //
 // Measured (bf16, dim 128, one group, 32 query and 8 kv heads, at a copy rate of 6.55 TB/s): 64 sequences of 2048 to 12288
-// tokens 114 us, 4.4 TB/s of cache; one of 131077 tokens 49 us, 3.1 TB/s; one of 777 tokens 10.9 us.  A round of 32 tokens
-// issues some 300 instructions a warp, and issue slots are what the long loop is bound by; about 18 us of a call are the
+// tokens 114 us, 4.4 TB/s of cache; one of 131077 tokens 48 us, 3.1 TB/s; one of 777 tokens 9.7 us.  A round of 32 tokens
+// issues some 300 instructions a warp, and issue slots are what the long loop is bound by; about 17 us of a call are the
 // first loads, the joins and the launch.
 #include "sm100.cuh"
 #include "mla_common.cuh"
@@ -809,7 +809,7 @@ attn_int4_kernel(const AttnInt4Params p) {
       team_sync();                                 // the join buffer is free again
     }
     if (!whole) {
-      // Teams c0 .. c1 share the segment.  They are taken in groups of sixteen neighbours: the last of a group to arrive adds
+      // Teams c0 .. c1 share the segment.  They are taken in groups of twelve neighbours: the last of a group to arrive adds
       // its partial results up into the slot of the group's first team, the last group to be done adds up the groups'.  (One
       // team adding up 74 takes 12 us.)
       const int64_t total = sh.total, ctas = sh.ctas;
@@ -818,9 +818,9 @@ attn_int4_kernel(const AttnInt4Params p) {
       // the segment is the last of team c0 (slot 1 unless it is its first as well) and the first of all others (slot 0)
       const int in_c0 = seg_first > (int64_t)c0 * total / ctas ? 1 : 0;
       auto slot_of = [&](int c) { return p.partial + ((int64_t)c * 2 + (c == c0 ? in_c0 : 0)) * kSlot; };
-      constexpr int kGroup = 16;
-      const int lead = max(c0, me / kGroup * kGroup), tail = min(c1, me / kGroup * kGroup + kGroup - 1);
-      const int groups = c1 / kGroup - c0 / kGroup + 1;
+      constexpr int kGroup = 12;
+      const int lead = c0 + (me - c0) / kGroup * kGroup, tail = min(c1, lead + kGroup - 1);
+      const int groups = (c1 - c0) / kGroup + 1;
       // Three counters a team.  Only one shared segment begins in a team's range (its last), and a group of another segment
       // that begins with this team goes by the counter of those that only pass through.
       int* const group_counter = p.counters + 3 * lead + (lead == c0 ? 1 : 0);
@@ -838,7 +838,7 @@ attn_int4_kernel(const AttnInt4Params p) {
       // Adds up `many` partial results in their order; `emit(r, d, sums, sum, top)` takes four columns of a row.
       auto add_up = [&](int many, auto slot_at, auto emit) {
         // Four at a time, all on their way at once, in the last batch too; most segments are shared by two or three (16 at a
-        // time: 1 x 777 tokens 12.3 us for 10.9, and the registers make the loop above spill)
+        // time: 1 x 777 tokens 12.3 us where this takes 10.8, and the registers make the loop above spill)
         constexpr int kBatch = 4;
         const int items = rows * (DIM / 4), rounds = (items + 32 * kWarps - 1) / (32 * kWarps);
         for (int k = 0; k < rounds; ++k) {
@@ -901,7 +901,7 @@ attn_int4_kernel(const AttnInt4Params p) {
           }
           team_sync();
           if (arrive(seg_counter, groups - 1))
-            add_up(groups, [&](int i) { return slot_of(max(c0, (c0 / kGroup + i) * kGroup)); }, to_out);
+            add_up(groups, [&](int i) { return slot_of(c0 + i * kGroup); }, to_out);
         }
       }
     }
