@@ -55,7 +55,7 @@ struct AttnInt4Params {
   void* out;
   int batch, s_q, h_q, h_kv, per, page_size, max_pages, num_pages, len_cap;
   int rows, q_tiles;                   // query rows of a kv head (s_q * per), tiles of them
-  FastDiv page_div;                    // t / page_size
+  FastDiv page_div, per_div;           // t / page_size, row / per
   float scale_log2;
   int* counters;                       // three per team, zero between calls
   float* partial;                      // [2 * teams][kRows * (dim + 2)]
@@ -132,6 +132,9 @@ __device__ __forceinline__ void widen4(uint32_t r, uint32_t (&u)[4]) {
 template <typename T> __device__ __forceinline__ float2 widen_scale(uint32_t w) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ float inverse_pow2(float f) {        // 1 / f for a power of two of 2^-120 to 2^120, 0 for 0
+  return f == 0.f ? 0.f : __uint_as_float((254u << 23) - __float_as_uint(f));
 }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -368,7 +371,7 @@ attn_int4_kernel(const AttnInt4Params p) {
       for (int nt = 0; nt < NT; ++nt) {
         const int r = nt * 8 + g, row = it.qt * Cfg::kRows + r;
         const bool ok = r < rows;
-        const int qi = ok ? row / p.per : 0;
+        const int qi = ok ? (int)p.per_div((uint32_t)row) : 0;
         const T* src = reinterpret_cast<const T*>(p.q) + it.b * p.q_sb + qi * p.q_ss + ((int64_t)it.h * p.per + (ok ? row - qi * p.per : 0)) * DIM;
 #pragma unroll
         for (int x = 0; x < DIM / 32; ++x) {
@@ -376,7 +379,7 @@ attn_int4_kernel(const AttnInt4Params p) {
           raw[nt][x] = ok ? __ldg(reinterpret_cast<const uint4*>(src + col)) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) limit[nt][e] = it.len - p.s_q + (it.qt * Cfg::kRows + nt * 8 + 2 * j + e) / p.per + 1;
+        for (int e = 0; e < 2; ++e) limit[nt][e] = it.len - p.s_q + (int)p.per_div((uint32_t)(it.qt * Cfg::kRows + nt * 8 + 2 * j + e)) + 1;
       }
       if (first) {                                    // fill the ring: lane k looks up the page of tile k, all at once
         first = false;
@@ -390,7 +393,7 @@ attn_int4_kernel(const AttnInt4Params p) {
       }
       if (lane < 2 * NT && it.units - it.u < left) {  // the queries of the next segment here: on their way to L2 by then
         const UnitIter n = ahead_of(it, it.units - it.u);
-        const int row = n.qt * Cfg::kRows + (warp * 2 * NT + lane), qi = row / p.per;
+        const int row = n.qt * Cfg::kRows + (warp * 2 * NT + lane), qi = (int)p.per_div((uint32_t)row);
         if (row < p.rows) {
           const T* at = reinterpret_cast<const T*>(p.q) + n.b * p.q_sb + qi * p.q_ss + ((int64_t)n.h * p.per + (row - qi * p.per)) * DIM;
 #pragma unroll
@@ -596,9 +599,9 @@ attn_int4_kernel(const AttnInt4Params p) {
             // change, so a weight is below 2^14; one that is 2^-22 of the largest is still normal
             const int ex = max((int)(__float_as_uint(big) >> 23) - 127, -112);
             const float f_new = __uint_as_float((uint32_t)(127 + 8 - min(ex, 127)) << 23);
-            ratio = f == 0.f ? 0.f : f_new / f;
+            ratio = f_new * inverse_pow2(f);
             f = f_new;
-            most = 1024.f / f_new;                    // infinity at the upper end
+            most = __uint_as_float((uint32_t)min(127 + 2 + ex, 255) << 23);         // 1024 / f; infinity at the upper end
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -737,7 +740,7 @@ attn_int4_kernel(const AttnInt4Params p) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) join_m[warp * Cfg::kRows + nt * 8 + 2 * j + e] = m[nt][e];
     team_sync();
-    const float inv_f = f == 0.f ? 0.f : 1.f / f;
+    const float inv_f = inverse_pow2(f);
     float part[NT][2];                                // this warp's weight in the joint result
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -753,7 +756,7 @@ attn_int4_kernel(const AttnInt4Params p) {
     const int64_t seg_first = sh.seq_base + ((int64_t)it.h * p.q_tiles + it.qt) * it.units, seg_end = seg_first + it.units;
     const bool whole = seg_first >= sh.start && seg_end <= sh.end;
     auto store_out = [&](int r, int d, float4 v) {
-      const int row = it.qt * Cfg::kRows + r, qi = row / p.per;
+      const int row = it.qt * Cfg::kRows + r, qi = (int)p.per_div((uint32_t)row);
       T* dst = reinterpret_cast<T*>(p.out) + (((int64_t)it.b * p.s_q + qi) * p.h_q + (int64_t)it.h * p.per + (row - qi * p.per)) * DIM + d;
       union { uint2 raw; T e[4]; } o;
       o.e[0] = from_f32<T>(v.x); o.e[1] = from_f32<T>(v.y); o.e[2] = from_f32<T>(v.z); o.e[3] = from_f32<T>(v.w);
@@ -796,7 +799,7 @@ attn_int4_kernel(const AttnInt4Params p) {
           top = fmaxf(top, join_m[w * Cfg::kRows + r]);
         }
         if (whole) {
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);      // two steps of fp32; the sum is below 2^40
           store_out(r, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         } else {
           __stcg(reinterpret_cast<float4*>(slot + r * DIM + d), v);
@@ -876,7 +879,7 @@ attn_int4_kernel(const AttnInt4Params p) {
         }
       };
       auto to_out = [&](int r, int d, float4 v, float sum, float) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);      // two steps of fp32; the sum is below 2^40
         store_out(r, d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
       };
       if (arrive(group_counter, tail - lead)) {
@@ -1028,6 +1031,7 @@ extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache
   p.len_cap = num_pages == 0 ? 0 : (int)(cap < 0x7fff0000ll ? cap : 0x7fff0000ll);
   p.rows = (int)(s_q * (h_q / h_kv)); p.q_tiles = plan.q_tiles;
   p.page_div = FastDiv((uint32_t)page_size);
+  p.per_div = FastDiv((uint32_t)p.per);
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   TL_REQUIRE((batch * h_kv * plan.q_tiles) / plan.grid + 1 < (1ll << 31) / (p.len_cap / kUnit + 1),
              "attn_decode_paged_int4: more units of work than a CTA counts");
