@@ -34,9 +34,10 @@
 // last adds them up in their fixed order, so the result does not depend on who that is.
 //
 // Measured (bf16, dim 128, one group, 32 query and 8 kv heads, at a copy rate of 6.55 TB/s): 64 sequences of 2048 to 12288
-// tokens 114 us, 4.4 TB/s of cache; one of 131077 tokens 48 us, 3.1 TB/s; one of 777 tokens 9.7 us.  A round of 32 tokens
-// issues some 300 instructions a warp, and issue slots are what the long loop is bound by; about 17 us of a call are the
-// first loads, the joins and the launch.
+// tokens 107.5 us, 4.65 TB/s of cache; one of 131077 tokens 48.7 us, 3.1 TB/s; one of 777 tokens 8.6 us.  A round of 32 tokens
+// issues some 300 instructions a warp, and issue slots are what the long loop is bound by; about 15 us of a call are the
+// first loads, the joins and the launch.  Each integer or IEEE division between segments is felt: without those by run-time
+// sizes 200 sequences of 40 to 300 tokens take 32.4 us instead of 36.4 us.
 #include "sm100.cuh"
 #include "mla_common.cuh"
 
@@ -55,7 +56,7 @@ struct AttnInt4Params {
   void* out;
   int batch, s_q, h_q, h_kv, per, page_size, max_pages, num_pages, len_cap;
   int rows, q_tiles;                   // query rows of a kv head (s_q * per), tiles of them
-  FastDiv page_div, per_div;           // t / page_size, row / per
+  FastDiv page_div, per_div, tile_div, team_div;     // t / page_size, row / per, tile / q_tiles, unit / teams
   float scale_log2;
   int* counters;                       // three per team, zero between calls
   float* partial;                      // [2 * teams][kRows * (dim + 2)]
@@ -64,7 +65,7 @@ struct AttnInt4Params {
 constexpr int kWarps = 4, kHalf = 16 * kWarps, kUnit = 2 * kHalf;      // a warp's two tiles of a unit lie kHalf tokens apart
 
 // Teams per SM, by the registers a thread needs: 128 (four teams), 168 with four groups' steps and sums (32 x 4096 tokens:
-// 62 us, 73 us with four teams that spill), 255 with twice the accumulators (24 sequences of 4 tokens, dim 64: 39 us, 42 us).
+// 59 us, 73 us with four teams that spill), 255 with twice the accumulators (24 sequences of 4 tokens, dim 64, in an earlier form: 39 us, 42 us).
 __host__ __device__ constexpr int i4_teams(int dim, int groups, int nt) {
   return nt == 2 || dim == 256 ? 2 : dim == 128 && groups == 4 ? 3 : 4;
 }
@@ -190,8 +191,9 @@ attn_int4_kernel(const AttnInt4Params p) {
   // what only the ends of segments need stays in shared memory
   struct Shared {
     int64_t sums[kWarps];
-    int64_t total, ctas, start, end, seq_base;         // seq_base: first unit of sequence it.b
-    int first_b, last;
+    int64_t total, quot, start, end, seq_base;         // seq_base: first unit of sequence it.b
+    int ctas, first_b, last;
+    uint32_t rest;
   };
   Shared& sh = *reinterpret_cast<Shared*>(join_l + kWarps * Cfg::kRows);
   uint8_t* const ring = smem + warp * ST * Cfg::kStage;                    // this warp's stages
@@ -222,10 +224,10 @@ attn_int4_kernel(const AttnInt4Params p) {
     const int64_t ctas = total < all_teams ? total : all_teams;          // every one of them has a unit
     if (me >= ctas) return;                                              // the whole team
     // team i begins at floor(i * total / ctas)
-    const int64_t quot = total >> 32 ? total / ctas : (int64_t)((uint32_t)total / (uint32_t)ctas);
-    const uint32_t rest = (uint32_t)(total - quot * ctas);               // times a team's number: below 2^32
-    const int64_t start = me * quot + me * rest / (uint32_t)ctas;
-    const int64_t end = (me + 1) * quot + (me + 1) * rest / (uint32_t)ctas;
+    const int64_t quot = total <= all_teams ? 1 : total >> 31 ? total / all_teams : (int64_t)p.team_div((uint32_t)total);
+    const uint32_t rest = (uint32_t)(total - quot * ctas);               // times a team's number: below 2^31
+    const int64_t start = me * quot + p.team_div(me * rest);
+    const int64_t end = (me + 1) * quot + p.team_div((me + 1) * rest);
     int64_t base = before + incl - mine;
     if (base * per_unit <= start && start < (base + mine) * per_unit) {  // exactly one thread
       int b = b0, units = 0;
@@ -237,7 +239,9 @@ attn_int4_kernel(const AttnInt4Params p) {
       sh.first_b = b;
       sh.seq_base = base * per_unit;
       sh.total = total;
-      sh.ctas = ctas;
+      sh.ctas = (int)ctas;
+      sh.quot = quot;
+      sh.rest = rest;
       sh.start = start;
       sh.end = end;
     }
@@ -249,7 +253,7 @@ attn_int4_kernel(const AttnInt4Params p) {
     const int64_t off = start - sh.seq_base;
     const int seg = off >> 32 ? (int)(off / it.units) : (int)((uint32_t)off / (uint32_t)it.units);
     it.u = (int)(off - (int64_t)seg * it.units);
-    it.h = seg / p.q_tiles;
+    it.h = (int)p.tile_div((uint32_t)seg);
     it.qt = seg - it.h * p.q_tiles;
   }
 
@@ -816,10 +820,13 @@ attn_int4_kernel(const AttnInt4Params p) {
       // its partial results up into the slot of the group's first team, the last group to be done adds up the groups'.  (One
       // team adding up 74 takes 12 us.)
       const int64_t total = sh.total, ctas = sh.ctas;
-      const int c0 = seg_first >= sh.start ? me : (int)(((seg_first + 1) * ctas - 1) / total);
-      const int c1 = seg_end <= sh.end ? me : (int)((seg_end * ctas - 1) / total);
+      auto team_of = [&](int64_t unit) {               // the last team that begins at or before a unit
+        const int64_t a = (unit + 1) * ctas - 1;
+        return (a | total) >> 32 ? (int)(a / total) : (int)((uint32_t)a / (uint32_t)total);
+      };
+      const int c0 = seg_first >= sh.start ? me : team_of(seg_first), c1 = seg_end <= sh.end ? me : team_of(seg_end - 1);
       // the segment is the last of team c0 (slot 1 unless it is its first as well) and the first of all others (slot 0)
-      const int in_c0 = seg_first > (int64_t)c0 * total / ctas ? 1 : 0;
+      const int in_c0 = seg_first > c0 * sh.quot + p.team_div(c0 * sh.rest) ? 1 : 0;
       auto slot_of = [&](int c) { return p.partial + ((int64_t)c * 2 + (c == c0 ? in_c0 : 0)) * kSlot; };
       constexpr int kGroup = 12;
       const int lead = c0 + (me - c0) / kGroup * kGroup, tail = min(c1, lead + kGroup - 1);
@@ -1032,6 +1039,8 @@ extern "C" int tl_b200_attn_decode_paged_int4(const void* q, const void* k_cache
   p.rows = (int)(s_q * (h_q / h_kv)); p.q_tiles = plan.q_tiles;
   p.page_div = FastDiv((uint32_t)page_size);
   p.per_div = FastDiv((uint32_t)p.per);
+  p.tile_div = FastDiv((uint32_t)p.q_tiles);
+  p.team_div = FastDiv((uint32_t)plan.grid);
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   TL_REQUIRE((batch * h_kv * plan.q_tiles) / plan.grid + 1 < (1ll << 31) / (p.len_cap / kUnit + 1),
              "attn_decode_paged_int4: more units of work than a CTA counts");
