@@ -34,7 +34,7 @@
 // last adds them up in their fixed order, so the result does not depend on who that is.
 //
 // Measured (bf16, dim 128, one group, 32 query and 8 kv heads, at a copy rate of 6.55 TB/s): 64 sequences of 2048 to 12288
-// tokens 107.5 us, 4.65 TB/s of cache; one of 131077 tokens 48.7 us, 3.1 TB/s; one of 777 tokens 8.6 us.  A round of 32 tokens
+// tokens 107.5 us, 4.65 TB/s of cache; one of 131077 tokens 50 us, 3.0 TB/s; one of 777 tokens 8.6 us.  A round of 32 tokens
 // issues some 300 instructions a warp, and issue slots are what the long loop is bound by; about 15 us of a call are the
 // first loads, the joins and the launch.  Each integer or IEEE division between segments is felt: without those by run-time
 // sizes 200 sequences of 40 to 300 tokens take 32.4 us instead of 36.4 us.
@@ -947,25 +947,15 @@ static I4Plan i4_plan(int64_t batch, int64_t s_q, int64_t h_q, int64_t h_kv, int
 
 template <typename T, int DIM, int GROUP, int NT>
 static int launch_i4(const AttnInt4Params& p, int grid, cudaStream_t s) {
-  auto launch = [&](auto teams) {
-    constexpr int N = decltype(teams)::value, smem = N * I4Cfg<DIM, GROUP, NT>::kSmem;
-    auto kernel = attn_int4_kernel<T, DIM, GROUP, NT, N>;
-    if (const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return rc;
-    return launch_overlapped(kernel, dim3(grid / N), dim3(32 * kWarps * N), smem, s, p);
-  };
-  cudaError_t rc;
-  // Four small teams to an SM are one CTA where there are many segments: the schedulers favour the oldest warps, and as CTAs
-  // of their own the teams end at 80, 92, 105 and 118 us (64 sequences of 2048 to 12288 tokens: 120 us; 115 us as one CTA,
-  // whose teams have a warp of every age).  With few, long segments the early ends pay, since each sets off an addition of
-  // partial results: one sequence of 131077 tokens 49.4 and 52.1 us, 24 of 4096 44.5 and 44.8 us, 32 of 4096 50.8 and 50.0 us.
-  // Two and three teams an SM: 52.0 us as CTAs and 54.4 us as one (16 x 4096 tokens, dim 256).
-  if constexpr (I4Cfg<DIM, GROUP, NT>::kTeams == 4) {
-    if ((int64_t)p.batch * p.h_kv * p.q_tiles * 3 >= grid) rc = launch(std::integral_constant<int, 4>());
-    else rc = launch(std::integral_constant<int, 1>());
-  } else {
-    rc = launch(std::integral_constant<int, 1>());
-  }
-  TL_CUDA(rc);
+  // Four small teams to an SM are one CTA: the schedulers favour the oldest warps, and as CTAs of their own the teams end at 80,
+  // 92, 105 and 118 us (64 sequences of 2048 to 12288 tokens: 112.7 us; 107.8 us as one CTA, whose teams have a warp of every
+  // age; 32 x 4096 tokens 44.8 and 44.0 us, one sequence of 131077 49.2 and 49.7 us).  Two and three teams an SM:
+  // 47.6 us as CTAs and 49.5 us as one (16 x 4096 tokens, dim 256), 60.5 and 63.4 us (32 x 4096, 16 rows).
+  using Cfg = I4Cfg<DIM, GROUP, NT>;
+  constexpr int teams = Cfg::kTeams == 4 ? 4 : 1, smem = teams * Cfg::kSmem;
+  auto kernel = attn_int4_kernel<T, DIM, GROUP, NT, teams>;
+  TL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  TL_CUDA(launch_overlapped(kernel, dim3(grid / teams), dim3(32 * kWarps * teams), smem, s, p));
   TL_LAUNCH_CHECK("attn_int4_kernel");
   return TL_B200_OK;
 }
