@@ -333,3 +333,28 @@ def test_the_same_through_compiled_programs(cuda_device):
     proj = tilelang.compile(P.gemm_epilogue(2, 96, h_q * dim, bias=True, activation="silu", residual=True, transpose_b=True), out_idx=-1, target="b200")
     assert proj(out.view(2, -1), wo, bias, res, c) == 0
     assert torch.allclose(c.double(), O.gemm_epilogue(out.view(2, -1), wo, bias, "silu", res, True), rtol=2.0 ** -8, atol=1e-4)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_long_sequences_keep_the_precision_of_their_output(cuda_device, dtype):
+    """Errors of one sign must not add up over a long sequence.  Relative to the output in the 2-norm, its own rounding is uniform
+    within half a step at most, 2^-11 / sqrt 3 for fp16 (2^-8 / sqrt 3 for bf16), and the weights' (2^-11 each, of either sign,
+    so they add up like the values themselves) 2^-11 / sqrt 3 again: together 2^-11 sqrt(2/3).  A bf16 output's weights meet
+    codes of one sign, at most twice the values about zero."""
+    g = torch.Generator(device=cuda_device).manual_seed(4)
+    n, d, page, batch, h_q = 100000, 64, 64, 60, 8
+    pages = (n + page - 1) // page
+    w = {"block_table": torch.arange(pages, dtype=torch.int32, device=cuda_device).repeat(batch, 1),       # one cache, 60 queries
+         "cache_seqlens": torch.full((batch,), n, dtype=torch.int32, device=cuda_device)}
+    for s in "kv":
+        x = torch.randn(pages * page, 1, d, generator=g, device=cuda_device).to(dtype)
+        w[s + "_cache"] = torch.empty(pages, 1, page, d // 2, dtype=torch.uint8, device=cuda_device)
+        w[s + "_scale"] = torch.empty(pages, 1, page, 1, 2, dtype=dtype, device=cuda_device)
+        ops.kv_cache_write(torch.arange(pages * page, device=cuda_device), x, w[s + "_cache"], w[s + "_scale"])
+    w["q"] = torch.randn(batch, 1, h_q, d, generator=g, device=cuda_device).to(dtype)
+    out = run(w, cuda_device).double().flatten(0, 2)
+    k, v = (O.values_u4g(w[s + "_cache"].cpu(), w[s + "_scale"].cpu()).double().reshape(-1, d)[:n].to(cuda_device) for s in "kv")
+    ref = (torch.softmax(w["q"].double().reshape(-1, d) @ k.T * d ** -0.5, -1) @ v).cpu()
+    bound = 2.0 ** -11 * (2 / 3) ** 0.5 if dtype is HF else (2.0 ** -16 / 3 + 4 * 2.0 ** -22 / 3) ** 0.5
+    err = float((out - ref).norm() / ref.norm())
+    assert err <= bound, (err, bound)

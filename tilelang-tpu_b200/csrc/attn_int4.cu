@@ -19,9 +19,12 @@
 //   * V: a register of the A operand is one column of two neighbouring tokens: one byte permute joins half words of the two.
 //   * Steps and minima never touch the codes:  q . k = s (q . c) + lo sum(q) per group, and the value's step multiplies p
 //     (rounded to fp16 with a power-of-two factor per warp that keeps p s in range: 2^-12 of each weight), its minimum
-//     adds p lo in fp32.  For fp16 outputs the weights' rounding should meet c - 8, not c: 8 times the sum of the ROUNDED
-//     weights, from an MMA with ones, is taken off, and 8 s goes to the minimum (error against 64 bits 2.5e-4 of the
-//     output, 3.4e-4 without; of a bf16 output it is a fiftieth of the rounding either way, so there it is left out).
+//     adds p lo in fp32.  The codes of V become c - 8 (an addition per pair of codes) and 8 s goes to the
+//     minimum: the weights' rounding then meets numbers about zero, and so do the sums, which with codes of one sign are
+//     hundreds of times the output of a long sequence and carry the tensor core's truncation into it (error against 64 bits,
+//     60 sequences of 100000 tokens, fp16: 2.6e-4 of the output, of which 2.1e-4 is its own rounding; 1.1e-3 without, 4.7e-4
+//     with 8 times the sum of the weights taken off at the end; bf16 1.68e-3, all of it rounding, and up to 2.3e-3 without).
+//     It costs 5%: 64 sequences of 2048 to 12288 tokens 108.6 and 114 us.
 // Every group of columns has its own MMAs, so a group's step can multiply the score or the weight.
 //
 // Work.  Sequences are cut into units of 128 tokens; the list of all (sequence, kv head, query tile, unit) is dealt out in
@@ -34,10 +37,10 @@
 // last adds them up in their fixed order, so the result does not depend on who that is.
 //
 // Measured (bf16, dim 128, one group, 32 query and 8 kv heads, at a copy rate of 6.55 TB/s): 64 sequences of 2048 to 12288
-// tokens 107.5 us, 4.65 TB/s of cache; one of 131077 tokens 50 us, 3.0 TB/s; one of 777 tokens 8.6 us.  A round of 32 tokens
-// issues some 300 instructions a warp, and issue slots are what the long loop is bound by; about 15 us of a call are the
+// tokens 114 us, 4.4 TB/s of cache; one of 131077 tokens 52 us, 2.9 TB/s; one of 777 tokens 9.0 us.  A round of 32 tokens
+// issues some 350 instructions a warp, and issue slots are what the long loop is bound by; about 15 us of a call are the
 // first loads, the joins and the launch.  Each integer or IEEE division between segments is felt: without those by run-time
-// sizes 200 sequences of 40 to 300 tokens take 32.4 us instead of 36.4 us.
+// sizes 200 sequences of 40 to 300 tokens took 32.4 us instead of 36.4 us.
 #include "sm100.cuh"
 #include "mla_common.cuh"
 
@@ -130,6 +133,15 @@ __device__ __forceinline__ void widen4(uint32_t r, uint32_t (&u)[4]) {
   u[2] = h & 0x000f000fu;
   u[3] = h & 0x00f000f0u;
 }
+// The same of c - 8 (exact: multiples of 2^-24 below 2^-16).
+__device__ __forceinline__ void centre4(uint32_t (&u)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t minus8 = i & 1 ? 0x80808080u : 0x80088008u;
+    const __half2 c = __hadd2(*reinterpret_cast<const __half2*>(&u[i]), *reinterpret_cast<const __half2*>(&minus8));
+    u[i] = *reinterpret_cast<const uint32_t*>(&c);
+  }
+}
 template <typename T> __device__ __forceinline__ float2 widen_scale(uint32_t w) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   else return __half22float2(*reinterpret_cast<const __half2*>(&w));
@@ -169,7 +181,6 @@ __global__ void __launch_bounds__(32 * kWarps * TEAMS, I4Cfg<DIM, GROUP, NT>::kT
 attn_int4_kernel(const AttnInt4Params p) {
   using Cfg = I4Cfg<DIM, GROUP, NT>;
   constexpr int NG = Cfg::kGroups, ST = Cfg::kStages, MT = DIM / 16, MG = GROUP / 16;
-  constexpr bool kCentre = std::is_same<T, __half>::value;       // the weights' rounding meets c - 8 (see above); bf16 outputs do not show it
   extern __shared__ __align__(128) uint8_t all_smem[];
   // With TEAMS > 1, warp w of the block runs on scheduler w % 4 and is the (w / 4)-th oldest there; a team has one warp on each scheduler,
   // each of another age.
@@ -448,7 +459,7 @@ attn_int4_kernel(const AttnInt4Params p) {
     }
     const int all_see = it.len - p.s_q + 1;           // tokens before this one are seen by every query
 
-    float acc[MT][NT][4], wsum[NG][NT][4], low[NG][NT][2], m[NT][2], l[NT][2];
+    float acc[MT][NT][4], low[NG][NT][2], m[NT][2], l[NT][2];
     float f = 0.f, most = 0.f;                        // the weights are p * step * f, steps up to `most`; 0: none seen yet
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -457,7 +468,7 @@ attn_int4_kernel(const AttnInt4Params p) {
         m[nt][e] = -FLT_MAX;                          // finite, so that a score of -inf weighs 0 and not NaN
         l[nt][e] = 0.f;
 #pragma unroll
-        for (int gg = 0; gg < NG; ++gg) low[gg][nt][e] = wsum[gg][nt][e] = wsum[gg][nt][2 + e] = 0.f;     // wsum: fp16 only
+        for (int gg = 0; gg < NG; ++gg) low[gg][nt][e] = 0.f;
       }
 #pragma unroll
       for (int t = 0; t < MT; ++t)
@@ -566,10 +577,8 @@ attn_int4_kernel(const AttnInt4Params p) {
 #pragma unroll
           for (int gg = 0; gg < NG; ++gg) {
             big = fmaxf(big, fmaxf(fabsf(v0[t][gg].x), fabsf(v1[t][gg].x)));
-            if constexpr (kCentre) {                  // the middle of the range
-              v0[t][gg].y = fmaf(8.f, v0[t][gg].x, v0[t][gg].y);
-              v1[t][gg].y = fmaf(8.f, v1[t][gg].x, v1[t][gg].y);
-            }
+            v0[t][gg].y = fmaf(8.f, v0[t][gg].x, v0[t][gg].y);       // the middle of the range
+            v1[t][gg].y = fmaf(8.f, v1[t][gg].x, v1[t][gg].y);
           }
         // ---- whether the running maximum or the factor f has to move -----------------------------------------------------
         // the maximum may lag by 2^4: p stays below 16, and sums are exact whatever the reference is
@@ -615,13 +624,7 @@ attn_int4_kernel(const AttnInt4Params p) {
               m[nt][e] = m_new;
               l[nt][e] *= alpha;
 #pragma unroll
-              for (int gg = 0; gg < NG; ++gg) {
-                low[gg][nt][e] *= alpha;
-                if constexpr (kCentre) {
-                  wsum[gg][nt][e] *= both;
-                  wsum[gg][nt][2 + e] *= both;
-                }
-              }
+              for (int gg = 0; gg < NG; ++gg) low[gg][nt][e] *= alpha;
 #pragma unroll
               for (int t = 0; t < MT; ++t) {
                 acc[t][nt][e] *= both;
@@ -669,10 +672,6 @@ attn_int4_kernel(const AttnInt4Params p) {
               }
               pb[t][nt][0] = movmatrix_trans(pack_f16(w[0], w[1]));
               pb[t][nt][1] = movmatrix_trans(pack_f16(w[2], w[3]));
-              if constexpr (kCentre) {
-                const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-                mma16816(wsum[gg][nt], ones, pb[t][nt][0], pb[t][nt][1]);
-              }
             }
           }
           // words of the tokens of operand rows 2j, 2j + 1, 2j + 8, 2j + 9
@@ -693,6 +692,8 @@ attn_int4_kernel(const AttnInt4Params p) {
                 uint32_t ua[4], ub[4];
                 widen4(__byte_perm(w[0][x], w[1][x], sel), ua);
                 widen4(__byte_perm(w[2][x], w[3][x], sel), ub);
+                centre4(ua);
+                centre4(ub);
                 const int mt = gg * MG + (GROUP >= 64 ? 4 * x + 2 * half : 0);
                 const uint32_t a0[4] = {ua[0], ua[1], ub[0], ub[1]}, a1[4] = {ua[2], ua[3], ub[2], ub[3]};
 #pragma unroll
@@ -782,8 +783,7 @@ attn_int4_kernel(const AttnInt4Params p) {
 #pragma unroll
               for (int t = 0; t < MG; ++t) {
                 const int d = gg * GROUP + g * (GROUP / 8) + 2 * t;
-                const float off = kCentre ? -8.f * wsum[gg][nt][e] : 0.f;
-                const float a0 = fmaf(acc[gg * MG + t][nt][e], 0x1p24f, off), a1 = fmaf(acc[gg * MG + t][nt][2 + e], 0x1p20f, off);
+                const float a0 = acc[gg * MG + t][nt][e] * 0x1p24f, a1 = acc[gg * MG + t][nt][2 + e] * 0x1p20f;
                 *reinterpret_cast<float2*>(dst + d) =
                     make_float2(fmaf(a0, inv_f, low[gg][nt][e]) * part[nt][e], fmaf(a1, inv_f, low[gg][nt][e]) * part[nt][e]);
               }
