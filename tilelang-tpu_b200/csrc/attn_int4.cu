@@ -18,8 +18,9 @@
 //     sequence; a power of two per query brings Q into fp16's range, and what falls below it is 2^-35 of its largest.
 //   * V: a register of the A operand is one column of two neighbouring tokens: one byte permute joins half words of the two.
 //   * Steps and minima never touch the codes:  q . k = s (q . c) + lo sum(q) per group, and the value's step multiplies p
-//     (rounded to fp16 with a power-of-two factor per warp that keeps p s in range: 2^-12 of each weight), its minimum
-//     adds p lo in fp32.  The codes of V become c - 8 (an addition per pair of codes) and 8 s goes to the
+//     (rounded to fp16: half a step, 2^-11 of each weight, or 2^-29 of the query's largest where that is more, for every query
+//     has a power of two per group of columns that keeps its p s in range, whatever other queries and groups meet), its
+//     minimum adds p lo in fp32.  The codes of V become c - 8 (an addition per pair of codes) and 8 s goes to the
 //     minimum: the weights' rounding then meets numbers about zero, and so do the sums, which with codes of one sign are
 //     hundreds of times the output of a long sequence and carry the tensor core's truncation into it (error against 64 bits,
 //     60 sequences of 100000 tokens, fp16: 2.6e-4 of the output, of which 2.1e-4 is its own rounding; 1.1e-3 without, 4.7e-4
@@ -146,8 +147,8 @@ template <typename T> __device__ __forceinline__ float2 widen_scale(uint32_t w) 
   if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   else return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
-__device__ __forceinline__ float inverse_pow2(float f) {        // 1 / f for a power of two of 2^-120 to 2^120, 0 for 0
-  return f == 0.f ? 0.f : __uint_as_float((254u << 23) - __float_as_uint(f));
+__device__ __forceinline__ float inverse_pow2(float f) {        // 1 / f for a power of two of 2^-126 to 2^126
+  return __uint_as_float((254u << 23) - __float_as_uint(f));
 }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -460,9 +461,11 @@ attn_int4_kernel(const AttnInt4Params p) {
     const int all_see = it.len - p.s_q + 1;           // tokens before this one are seen by every query
 
     float acc[MT][NT][4], low[NG][NT][2], m[NT][2], l[NT][2];
-    float f = 0.f, most = 0.f;                        // the weights are p * step * f, steps up to `most`; 0: none seen yet
+    float2 f[NG][NT];                                 // the weights of queries 2j, 2j + 1 are p * step * f, a power of two
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int gg = 0; gg < NG; ++gg) f[gg][nt] = make_float2(0x1p120f, 0x1p120f);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         m[nt][e] = -FLT_MAX;                          // finite, so that a score of -inf weighs 0 and not NaN
@@ -542,7 +545,6 @@ attn_int4_kernel(const AttnInt4Params p) {
         }
         // ---- the values' steps and minima; what is not seen --------------------------------------------------------------
         float2 v0[2][NG], v1[2][NG];
-        float big = 0.f;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -566,23 +568,28 @@ attn_int4_kernel(const AttnInt4Params p) {
                 see |= (ok2 ? 1u : 0u) << (4 * NT * t + 4 * nt + e);
               }
 #pragma unroll
-            for (int gg = 0; gg < NG; ++gg) {         // rows behind the last token hold anything
-              v0[t][gg] = live0 ? v0[t][gg] : make_float2(0.f, 0.f);
-              v1[t][gg] = live1 ? v1[t][gg] : make_float2(0.f, 0.f);
+            for (int gg = 0; gg < NG; ++gg) {         // rows behind the last token hold anything; NaN counts for nothing below
+              v0[t][gg].x = live0 ? v0[t][gg].x : __uint_as_float(0x7fffffffu);
+              v1[t][gg].x = live1 ? v1[t][gg].x : __uint_as_float(0x7fffffffu);
             }
           }
         }
+        // ---- whether the running maximum or a factor f has to move -------------------------------------------------------
+        // the maximum may lag by 2^4: p stays below 16, and sums are exact whatever the reference is
+        float over = 0.f, rel[2][NT][4];
+        bool coarse = false;                          // a step times f above 2^11: its weight could pass fp16's range
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int gg = 0; gg < NG; ++gg) {
+          const float big = fmaxf(fmaxf(fabsf(v0[0][gg].x), fabsf(v1[0][gg].x)), fmaxf(fabsf(v0[1][gg].x), fabsf(v1[1][gg].x)));
+          float finest = fmaxf(f[gg][0].x, f[gg][0].y);
+          if constexpr (NT == 2) finest = fmaxf(finest, fmaxf(f[gg][1].x, f[gg][1].y));
+          coarse |= big * finest > 0x1p11f;
 #pragma unroll
-          for (int gg = 0; gg < NG; ++gg) {
-            big = fmaxf(big, fmaxf(fabsf(v0[t][gg].x), fabsf(v1[t][gg].x)));
+          for (int t = 0; t < 2; ++t) {
             v0[t][gg].y = fmaf(8.f, v0[t][gg].x, v0[t][gg].y);       // the middle of the range
             v1[t][gg].y = fmaf(8.f, v1[t][gg].x, v1[t][gg].y);
           }
-        // ---- whether the running maximum or the factor f has to move -----------------------------------------------------
-        // the maximum may lag by 2^4: p stays below 16, and sums are exact whatever the reference is
-        float over = 0.f, rel[2][NT][4];
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -592,48 +599,72 @@ attn_int4_kernel(const AttnInt4Params p) {
               rel[t][nt][e] = sc[t][nt][e] - m[nt][e & 1];
               over = fmaxf(over, rel[t][nt][e]);
             }
-        if (__any_sync(0xffffffffu, over > 4.f || big > most)) {
+        if (__any_sync(0xffffffffu, over > 4.f || coarse)) {
           float top[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) top[nt][e] = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][2 + e]), fmaxf(sc[1][nt][e], sc[1][nt][2 + e]));
 #pragma unroll
-          for (int o = 4; o < 32; o *= 2) {
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+          for (int o = 4; o < 32; o *= 2)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int e = 0; e < 2; ++e) top[nt][e] = fmaxf(top[nt][e], __shfl_xor_sync(0xffffffffu, top[nt][e], o));
-          }
-          float ratio = 1.f;                          // what the factor f changes by
-          if (big > most) {
-            // f = 2^(8 - exponent): the largest step times f lies in [256, 512), and steps up to twice as large need no
-            // change, so a weight is below 2^14; one that is 2^-22 of the largest is still normal
-            const int ex = max((int)(__float_as_uint(big) >> 23) - 127, -112);
-            const float f_new = __uint_as_float((uint32_t)(127 + 8 - min(ex, 127)) << 23);
-            ratio = f_new * inverse_pow2(f);
-            f = f_new;
-            most = __uint_as_float((uint32_t)min(127 + 2 + ex, 255) << 23);         // 1024 / f; infinity at the upper end
-          }
+          float alpha[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float m_new = fmaxf(m[nt][e], top[nt][e]), alpha = ex2_approx(m[nt][e] - m_new), both = alpha * ratio;
+              const float m_new = fmaxf(m[nt][e], top[nt][e]);
+              alpha[nt][e] = ex2_approx(m[nt][e] - m_new);
               m[nt][e] = m_new;
-              l[nt][e] *= alpha;
-#pragma unroll
-              for (int gg = 0; gg < NG; ++gg) low[gg][nt][e] *= alpha;
-#pragma unroll
-              for (int t = 0; t < MT; ++t) {
-                acc[t][nt][e] *= both;
-                acc[t][nt][2 + e] *= both;
-              }
+              l[nt][e] *= alpha[nt][e];
 #pragma unroll
               for (int t = 0; t < 2; ++t) {
                 rel[t][nt][e] = sc[t][nt][e] - m_new;
                 rel[t][nt][2 + e] = sc[t][nt][2 + e] - m_new;
+              }
+            }
+          // A query's factor f for a group of columns: 2^4 over its largest weight so far (to a power of two), so that what
+          // falls below fp16's range is 2^-29 of that, and a step may be 2^6 times it before this place is come to again.  By
+          // the weights and not the steps: a step may be huge, or infinite, and hardly weigh, or be hidden from this query.
+          // Of the weights before, f has what is needed: they lost alpha since.  Where nothing has weighed f stays at 2^120.
+          // (Straight on: with votes and branches around what is seldom needed, 16 x 4096 tokens at dim 256 and groups of 32 took
+          // 80.4 us where this takes 78.4, and 24 sequences of 4 tokens 29.6 us where this takes 28.9.)
+          float p_now[2][NT][4];
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) p_now[t][nt][e] = ex2_approx(rel[t][nt][e]);
+#pragma unroll
+          for (int gg = 0; gg < NG; ++gg)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              uint32_t heavy[2];                      // bits of the largest weight of the round (NaN, 0 times infinity, aside)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                heavy[e] = __float_as_uint(fmaxf(fmaxf(fmaxf(0.f, p_now[0][nt][e] * fabsf(v0[0][gg].x)), fmaxf(p_now[0][nt][2 + e] * fabsf(v1[0][gg].x),
+                                                       p_now[1][nt][e] * fabsf(v0[1][gg].x))), p_now[1][nt][2 + e] * fabsf(v1[1][gg].x)));
+              uint32_t both16 = __byte_perm(heavy[0], heavy[1], 0x7632);       // the upper halves of the two are ordered like them
+#pragma unroll
+              for (int o = 4; o < 32; o *= 2) both16 = __vmaxu2(both16, __shfl_xor_sync(0xffffffffu, both16, o));
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float& fe = e ? f[gg][nt].y : f[gg][nt].x;
+                const float old = fe, a = alpha[nt][e];
+                const int by_new = 254 + 4 - (int)(both16 >> (e ? 23 : 7) & 0xff);
+                const int by_old = (int)(__float_as_uint(old) >> 23) + 127 - (int)(__float_as_uint(a) >> 23);
+                fe = __uint_as_float((uint32_t)min(min(by_new, by_old), 247) << 23);
+                const float both = a > 0.f ? a * (inverse_pow2(old) * fe) : 0.f;         // 2 at most
+                low[gg][nt][e] *= a;
+#pragma unroll
+                for (int t = 0; t < MG; ++t) {
+                  acc[gg * MG + t][nt][e] *= both;
+                  acc[gg * MG + t][nt][2 + e] *= both;
+                }
               }
             }
         }
@@ -654,11 +685,13 @@ attn_int4_kernel(const AttnInt4Params p) {
           uint32_t pb[2][NT][2];
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const float f0 = v0[t][gg].x * f, f1 = v1[t][gg].x * f;
+            const float2 s0 = make_float2(v0[t][gg].x, v0[t][gg].x), s1 = make_float2(v1[t][gg].x, v1[t][gg].x);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               const float(&pr)[4] = sc[t][nt];
-              float w[4] = {pr[0] * f0, pr[1] * f0, pr[2] * f1, pr[3] * f1};
+              // p f first: f may be as small as a step is large
+              float2 w01 = sm100::mul2(sm100::mul2(make_float2(pr[0], pr[1]), f[gg][nt]), s0);
+              float2 w23 = sm100::mul2(sm100::mul2(make_float2(pr[2], pr[3]), f[gg][nt]), s1);
               if (full) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) low[gg][nt][e] = fmaf(pr[e], v0[t][gg].y, fmaf(pr[2 + e], v1[t][gg].y, low[gg][nt][e]));
@@ -666,12 +699,13 @@ attn_int4_kernel(const AttnInt4Params p) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const bool ok2 = see >> (4 * NT * t + 4 * nt + e) & 1;
-                  w[e] = ok2 ? w[e] : 0.f;
+                  float& w = e == 0 ? w01.x : e == 1 ? w01.y : e == 2 ? w23.x : w23.y;
+                  w = ok2 ? w : 0.f;
                   low[gg][nt][e & 1] += ok2 ? pr[e] * (e < 2 ? v0[t][gg].y : v1[t][gg].y) : 0.f;
                 }
               }
-              pb[t][nt][0] = movmatrix_trans(pack_f16(w[0], w[1]));
-              pb[t][nt][1] = movmatrix_trans(pack_f16(w[2], w[3]));
+              pb[t][nt][0] = movmatrix_trans(pack_f16(w01.x, w01.y));
+              pb[t][nt][1] = movmatrix_trans(pack_f16(w23.x, w23.y));
             }
           }
           // words of the tokens of operand rows 2j, 2j + 1, 2j + 8, 2j + 9
@@ -745,7 +779,6 @@ attn_int4_kernel(const AttnInt4Params p) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) join_m[warp * Cfg::kRows + nt * 8 + 2 * j + e] = m[nt][e];
     team_sync();
-    const float inv_f = inverse_pow2(f);
     float part[NT][2];                                // this warp's weight in the joint result
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -779,7 +812,8 @@ attn_int4_kernel(const AttnInt4Params p) {
           if (r >= 0 && r < Cfg::kJoinRows) {
             float* dst = join + (warp * Cfg::kJoinRows + r) * DIM;
 #pragma unroll
-            for (int gg = 0; gg < NG; ++gg)
+            for (int gg = 0; gg < NG; ++gg) {
+              const float inv_f = inverse_pow2(e ? f[gg][nt].y : f[gg][nt].x);
 #pragma unroll
               for (int t = 0; t < MG; ++t) {
                 const int d = gg * GROUP + g * (GROUP / 8) + 2 * t;
@@ -787,6 +821,7 @@ attn_int4_kernel(const AttnInt4Params p) {
                 *reinterpret_cast<float2*>(dst + d) =
                     make_float2(fmaf(a0, inv_f, low[gg][nt][e]) * part[nt][e], fmaf(a1, inv_f, low[gg][nt][e]) * part[nt][e]);
               }
+            }
           }
         }
       team_sync();
