@@ -251,9 +251,12 @@ kv_write_e4m3_kernel(const CacheArgs p, const int dim) {
   float amax = to_f32(__hmax_nan(top.x, top.y));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(amax) : "f"(1e-4f));
   const float s = amax / 448.0f;
-  const float y = __frcp_rn(s);
-  const float2 y2 = make_float2(y, y), s2 = make_float2(-s, -s);
+  // The quick quotient is that by -s, and the bytes' signs are turned over: so the correction, whose remainder of an exact
+  // quotient is +0, leaves both zeros their sign (by s, -0 would come out as +0).
+  const float y = -__frcp_rn(s);
+  const float2 y2 = make_float2(y, y), s2 = make_float2(s, s);
   const bool quick = s <= 0x1p100f;                            // s >= 2^-23 always
+  const uint32_t turn = quick ? 0x80808080u : 0u;
   uint8_t* dst = reinterpret_cast<uint8_t*>(side.cache) + slot * dim;
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
@@ -266,7 +269,7 @@ kv_write_e4m3_kernel(const CacheArgs p, const int dim) {
         const float2 q = quick ? div2(a, s2, y2) : make_float2(a.x / s, a.y / s);
         w[e / 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(q, __NV_SATFINITE, __NV_E4M3) << (16 * (e & 1));
       }
-      *reinterpret_cast<uint2*>(dst + c) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(dst + c) = make_uint2(w[0] ^ turn, w[1] ^ turn);
     }
   }
   if (lane == 0) reinterpret_cast<float*>(side.scale)[slot] = s;
