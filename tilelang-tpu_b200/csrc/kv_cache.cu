@@ -369,7 +369,7 @@ static int launch_cache(const CacheArgs& a, int64_t dim, int64_t group, int form
     TL_LAUNCH_CHECK("kv_write_e4m3_kernel");
   } else {
     const bool sixteen = dim % 16 == 0 && a.wide;
-    const int vecs = (int)dim / (sixteen ? 16 : 8), per_block = vecs > 512 ? 1 : 512 / vecs;
+    const int vecs = (int)dim / (sixteen ? 16 : 8), per_block = 512 / vecs;      // at most 1024 columns: 4 tokens or more
     CacheArgs b = a;
     b.vec_div = FastDiv((uint32_t)vecs);
     const dim3 grid((a.tokens + per_block - 1) / per_block, (unsigned)sides);
