@@ -304,8 +304,7 @@ int tl_b200_kv_cache_read(const int64_t* slots, const void* k_cache, const void*
  * tl_b200_mla_decode_paged_gqa); head h reads kv head h / (h_q / h_kv).  K and V are caches of format TL_U4G (above).
  * q [batch, s_q, h_q, dim] with q_stride_batch / q_stride_token elements between sequences / tokens (heads of a token
  * contiguous), out dense.  A row that sees no key is zero; lengths are clamped to the table's width, tokens of a page id
- * outside the cache are masked, and cache rows behind a sequence's last token may hold anything.  Queries up to 2^117 in
- * size (a larger finite one may give NaN).
+ * outside the cache are masked, and cache rows behind a sequence's last token may hold anything.
  * `workspace`: tl_b200_attn_decode_paged_int4_workspace_bytes(...) bytes (0 for sizes the call refuses), 16-byte aligned.
  * Its first TL_B200_ATTN_INT4_ZERO_BYTES bytes must be zero before the first call and are zero again after each call,
  * whatever the sizes of the calls; calls that may overlap on the GPU need workspaces of their own.                 */

@@ -381,6 +381,7 @@ attn_int4_kernel(const AttnInt4Params p) {
     uint32_t qf[NT][DIM / 16][2];
     float qsum[NG][NT][2], to_score[NT][2];           // for queries 2j, 2j + 1: scale * sum of q over the group; scale of the dot products
     int limit[NT][2];                                 // keys that queries 2j and 2j + 1 see
+    bool huge = false;                                // a query above 2^74: its to_score could pass fp32, so scores are 2^-24 of theirs
     {
       uint4 raw[NT][DIM / 32];
 #pragma unroll
@@ -416,6 +417,7 @@ attn_int4_kernel(const AttnInt4Params p) {
           for (int i = 0; i < DIM; i += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + i));
         }
       }
+      int up[NT];                                     // query g of the tile (and g + 8) goes times 2^up
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float big = 0.f;
@@ -431,11 +433,17 @@ attn_int4_kernel(const AttnInt4Params p) {
         }
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        const int up = min(14 - ((int)(__float_as_uint(big) >> 23) - 127), 120);       // big < 2^128, so up >= -113
-        const float mul = __uint_as_float((uint32_t)(127 + up) << 23), mul16 = mul * 0.0625f;
+        up[nt] = min(14 - ((int)(__float_as_uint(big) >> 23) - 127), 120);             // big < 2^128, so up >= -113
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) huge |= up[nt] < -60;
+      }
+      huge = __any_sync(0xffffffffu, huge);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float mul = __uint_as_float((uint32_t)(127 + up[nt]) << 23), mul16 = mul * 0.0625f;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          to_score[nt][e] = p.scale_log2 * (__uint_as_float((uint32_t)(127 - __shfl_sync(0xffffffffu, up, (2 * j + e) * 4)) << 23) * 0x1p24f);
+          to_score[nt][e] = p.scale_log2 * (__uint_as_float((uint32_t)(127 - __shfl_sync(0xffffffffu, up[nt], (2 * j + e) * 4)) << 23) *
+                                            (huge ? 1.f : 0x1p24f));
 #pragma unroll
         for (int x = 0; x < DIM / 32; ++x) {
           const float2 e01 = widen_scale<T>(raw[nt][x].x), e23 = widen_scale<T>(raw[nt][x].y), e45 = widen_scale<T>(raw[nt][x].z),
@@ -542,6 +550,14 @@ attn_int4_kernel(const AttnInt4Params p) {
                 sc[t][nt][2 + e] = fmaf(k1.x, d[t][nt][2 + e] * to_score[nt][e], gg ? sc[t][nt][2 + e] + lo1 : lo1);
               }
           }
+        }
+        if (std::is_same<T, __nv_bfloat16>::value && huge) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[t][nt][e] *= 0x1p24f;
         }
         // ---- the values' steps and minima; what is not seen --------------------------------------------------------------
         float2 v0[2][NG], v1[2][NG];

@@ -609,7 +609,7 @@ def attn_decode_paged_int4(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torc
     the heads of a token contiguous, caches (num_pages, h_kv, page, D / 2) uint8 with scales
     (num_pages, h_kv, page, groups, 2) of q's dtype, block_table (B, max_pages) int32, cache_seqlens (B,) int32 (the new
     tokens included), out (B, s_q, h_q, D).  Query token i sees the keys before len - s_q + i + 1; a row that sees none
-    is zero.  D 64, 128 or 256; elements of q up to 2^117 in size (a larger finite one may give NaN)."""
+    is zero.  D 64, 128 or 256."""
     qshape, dtype = q.shape, q.dtype
     if len(qshape) != 4 or out.shape != qshape or out.dtype != dtype or dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("attn_decode_paged_int4: q and out must be (B, s_q, h_q, D) bfloat16 or float16")
