@@ -160,6 +160,8 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 struct UnitIter {
   int b, h, qt, u, units, len;
 };
+// Lengths, page table and queries are read by ordinary loads: the kernel before may write them while this one is resident.
+__device__ __forceinline__ int length_of(const AttnInt4Params& p, int b) { return min(max(p.lens[b], 0), p.len_cap); }
 __device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + kUnit - 1) / kUnit : 1; }
 __device__ __forceinline__ bool advance(UnitIter& it, const AttnInt4Params& p) {      // true: a new segment begins
   if (++it.u < it.units) return false;
@@ -169,7 +171,7 @@ __device__ __forceinline__ bool advance(UnitIter& it, const AttnInt4Params& p) {
     if (++it.h == p.h_kv) {
       it.h = 0;
       if (++it.b < p.batch) {
-        it.len = mla_len(p.lens, it.b, p.len_cap);
+        it.len = length_of(p, it.b);
         it.units = units_of(it.len);
       }
     }
@@ -195,7 +197,6 @@ attn_int4_kernel(const AttnInt4Params p) {
   };
   dependency_wait();
   dependency_release();
-  const int* lens = behind_wait(p.lens);
   uint8_t* tail = smem + kWarps * ST * Cfg::kStage;
   float* join = reinterpret_cast<float*>(tail);                  // [warps][join rows][pitch]
   float* join_m = join + kWarps * Cfg::kJoinRows * DIM;  // [warps][rows]
@@ -218,7 +219,7 @@ attn_int4_kernel(const AttnInt4Params p) {
     const int chunk = (p.batch + 32 * kWarps - 1) / (32 * kWarps);
     const int b0 = min((int)tid * chunk, p.batch), b1 = min(b0 + chunk, p.batch);
     int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += units_of(mla_len(lens, b, p.len_cap));
+    for (int b = b0; b < b1; ++b) mine += units_of(length_of(p, b));
     int64_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -244,7 +245,7 @@ attn_int4_kernel(const AttnInt4Params p) {
     if (base * per_unit <= start && start < (base + mine) * per_unit) {  // exactly one thread
       int b = b0, units = 0;
       for (; b < b1; ++b) {
-        units = units_of(mla_len(lens, b, p.len_cap));
+        units = units_of(length_of(p, b));
         if (start < (base + units) * per_unit) break;
         base += units;
       }
@@ -260,7 +261,7 @@ attn_int4_kernel(const AttnInt4Params p) {
     team_sync();
     left = (int)(end - start);                                           // the host checks that it fits
     it.b = sh.first_b;
-    it.len = mla_len(lens, it.b, p.len_cap);
+    it.len = length_of(p, it.b);
     it.units = units_of(it.len);
     const int64_t off = start - sh.seq_base;
     const int seg = off >> 32 ? (int)(off / it.units) : (int)((uint32_t)off / (uint32_t)it.units);
@@ -337,7 +338,7 @@ attn_int4_kernel(const AttnInt4Params p) {
       bool live = my < w.len;
       uint32_t row = 0;
       if (live) {
-        const int id = __ldg(p.table + (int64_t)w.b * p.max_pages + p.page_div((uint32_t)my));
+        const int id = p.table[(int64_t)w.b * p.max_pages + p.page_div((uint32_t)my)];
         live = mla_page_ok(id, p.num_pages);
         row = row_of(id, w.h, my);
       }
@@ -358,7 +359,7 @@ attn_int4_kernel(const AttnInt4Params p) {
   };
   auto page_at = [&](const UnitIter& w, int half) {
     const int t0 = w.u * kUnit + half * kHalf + warp * 16;
-    return tile_in_page && t0 < w.len ? __ldg(p.table + (int64_t)w.b * p.max_pages + p.page_div((uint32_t)t0)) : -1;
+    return tile_in_page && t0 < w.len ? p.table[(int64_t)w.b * p.max_pages + p.page_div((uint32_t)t0)] : -1;
   };
   // the unit `by` behind `it`
   auto ahead_of = [&](UnitIter w, int by) {
@@ -393,7 +394,7 @@ attn_int4_kernel(const AttnInt4Params p) {
 #pragma unroll
         for (int x = 0; x < DIM / 32; ++x) {
           const int col = x / (GROUP / 32) * GROUP + (j * (GROUP / 32) + x % (GROUP / 32)) * 8;
-          raw[nt][x] = ok ? __ldg(reinterpret_cast<const uint4*>(src + col)) : make_uint4(0, 0, 0, 0);
+          raw[nt][x] = ok ? *reinterpret_cast<const uint4*>(src + col) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) limit[nt][e] = it.len - p.s_q + (int)p.per_div((uint32_t)(it.qt * Cfg::kRows + nt * 8 + 2 * j + e)) + 1;
@@ -497,8 +498,8 @@ attn_int4_kernel(const AttnInt4Params p) {
       int page0 = 0, page1 = 0;
       if (easy) {
         const int* table = p.table + (int64_t)it.b * p.max_pages;
-        page0 = __ldg(table + p.page_div((uint32_t)next0));
-        page1 = __ldg(table + p.page_div((uint32_t)next1));
+        page0 = table[p.page_div((uint32_t)next0)];
+        page1 = table[p.page_div((uint32_t)next1)];
       }
       cp_async_wait<ST - 2>();
       __syncwarp();                                           // every lane's copies have landed

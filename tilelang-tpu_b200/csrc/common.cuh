@@ -50,13 +50,6 @@ void count_launch(int n = 1);
 __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void dependency_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// A pointer whose loads cannot be moved in front of the dependency_wait() before this (loads through the read-only path
-// are not held back by a memory clobber).
-template <typename T> __device__ __forceinline__ const T* behind_wait(const T* p) {
-  asm volatile("" : "+l"(p)::"memory");
-  return p;
-}
-
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
                                      Args... args) {
@@ -175,6 +168,21 @@ template <typename T> __device__ __forceinline__ void st_stream32(void* p, const
   asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v.w[0]),
                "r"(v.w[1]), "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
                : "memory");
+}
+// The same of data that the kernel before may still be writing when this one becomes resident (launch_overlapped): not by the
+// read-only path, which asks that it stay constant for the kernel's whole life.
+__device__ __forceinline__ uint4 ld_fresh16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+template <typename T> __device__ __forceinline__ Vec32<T> ld_fresh32(const void* p) {
+  Vec32<T> v;
+  asm volatile("ld.global.L1::no_allocate.L2::evict_first.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+               : "l"(p)
+               : "memory");
+  return v;
 }
 inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 

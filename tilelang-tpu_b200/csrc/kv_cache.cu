@@ -86,25 +86,24 @@ kv_write_u4g_kernel(const CacheArgs p) {
   constexpr int kLanes = DIM / 16, kGroupLanes = GROUP / 16;
   dependency_wait();
   dependency_release();
-  const int64_t* slots = behind_wait(p.slots);
   const Side side = blockIdx.y ? p.v : p.k;
   const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   const int part = threadIdx.x % kLanes;
   const uint32_t t = p.head_div(row);
   const int h = (int)(row - t * p.heads);
-  const int64_t slot = row < p.rows ? __ldg(slots + t) : -1;
+  const int64_t slot = row < p.rows ? p.slots[t] : -1;
   const bool live = slot >= 0 && slot < p.total_slots;
   union { uint4 raw[2]; P v[8]; } in;
   in.raw[0] = in.raw[1] = make_uint4(0, 0, 0, 0);
   if (row < p.rows) {                 // whatever the slot: the two loads need not wait for each other
     const T* src = reinterpret_cast<const T*>(side.x) + t * side.stride + h * DIM + part * 16;
     if (p.wide) {                     // two 16-byte loads would each fetch every sector
-      const Vec32<T> v = ld_stream32<T>(src);
+      const Vec32<T> v = ld_fresh32<T>(src);
       in.raw[0] = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
       in.raw[1] = make_uint4(v.w[4], v.w[5], v.w[6], v.w[7]);
     } else {
-      in.raw[0] = ld_stream16(src);
-      in.raw[1] = ld_stream16(src + 8);
+      in.raw[0] = ld_fresh16(src);
+      in.raw[1] = ld_fresh16(src + 8);
     }
   }
   P lo2 = in.v[0], hi2 = in.v[0];
@@ -166,7 +165,6 @@ kv_read_u4g_kernel(const CacheArgs p) {
   constexpr int kLanes = DIM / 16, kGroupLanes = GROUP / 16, kRows = 256 / kLanes;
   dependency_wait();
   dependency_release();
-  const int64_t* slots = behind_wait(p.slots);
   const Side side = blockIdx.y ? p.v : p.k;
   const int part = threadIdx.x % kLanes;
   uint32_t t[2];
@@ -177,7 +175,7 @@ kv_read_u4g_kernel(const CacheArgs p) {
     const uint32_t row = (blockIdx.x * 2 + k) * kRows + threadIdx.x / kLanes;
     t[k] = p.head_div(row);
     h[k] = (int)(row - t[k] * p.heads);
-    slot[k] = row < p.rows ? __ldg(slots + t[k]) : -1;
+    slot[k] = row < p.rows ? p.slots[t[k]] : -1;
   }
   uint2 codes[2];
   P scale[2];
@@ -227,18 +225,17 @@ kv_write_e4m3_kernel(const CacheArgs p, const int dim) {
   using P = typename Pair<T>::type;
   dependency_wait();
   dependency_release();
-  const int64_t* slots = behind_wait(p.slots);
   const Side side = blockIdx.y ? p.v : p.k;
   const int lane = threadIdx.x % 32;
   const uint32_t t = blockIdx.x * 8 + threadIdx.x / 32;
   if (t >= p.tokens) return;                                   // the whole warp
-  const int64_t slot = __ldg(slots + t);
+  const int64_t slot = p.slots[t];
   const T* src = reinterpret_cast<const T*>(side.x) + t * side.stride;
   union { uint4 raw; P v[4]; } in[PASSES];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
     const int c = (i * 32 + lane) * 8;
-    in[i].raw = c < dim ? ld_stream16(src + c) : make_uint4(0, 0, 0, 0);
+    in[i].raw = c < dim ? ld_fresh16(src + c) : make_uint4(0, 0, 0, 0);
   }
   P top = __habs2(in[0].v[0]);
 #pragma unroll
@@ -281,7 +278,6 @@ __global__ void __launch_bounds__(256)
 kv_read_e4m3_kernel(const CacheArgs p, const int dim, const int per_block) {
   dependency_wait();
   dependency_release();
-  const int64_t* slots = behind_wait(p.slots);
   const Side side = blockIdx.y ? p.v : p.k;
   const int vecs = dim / COLS;
   const uint32_t t0 = blockIdx.x * (uint32_t)per_block;
@@ -295,7 +291,7 @@ kv_read_e4m3_kernel(const CacheArgs p, const int dim, const int per_block) {
     const uint32_t in_block = p.vec_div((uint32_t)i);
     t[k] = t0 + in_block;
     col[k] = (i - (int)in_block * vecs) * COLS;
-    slot[k] = i < items ? __ldg(slots + t[k]) : -1;
+    slot[k] = i < items ? p.slots[t[k]] : -1;
   }
   uint32_t codes[2][COLS / 4];
   float s[2];
