@@ -355,6 +355,36 @@ def tile_program(dev, rank, world, peaks, rows=8192, cols=4096):
     return e
 
 
+def operators(dev, rank, world, peaks, most_bytes=None):
+    """The cases of perf/operators.py (quantised cache, attention over 4 bits, GEMM with epilogue), one entry each, those up to
+    `most_bytes`: a CUDA graph of 12 back-to-back calls over three sets of inputs, the median of 10 replays, as time of one call.
+    Inputs of the small cases stay in L2, as those of a caller whose producer has just written them.  The peak is the larger of
+    the two floors, bytes at the copy rate or flop at the GEMM rate."""
+    from perf import operators as P
+    P.own = True
+    out = []
+    for case in P.listed():
+        work = P.work(case)
+        if most_bytes is not None and work["bytes"] > most_bytes:
+            continue
+        sets = [P.prepare(case, seed) for seed in (1, 2, 3)]
+        for s in sets:
+            P.run(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for i in range(12):
+                P.run(sets[i % 3])
+        ms = sorted(_time(graph.replay, 1, reps=1) / 12 for _ in range(10))[5]
+        by_bytes = work["bytes"] / peaks["hbm_gbs"] >= work["flops"] / (peaks["bf16_tflops"] * 1e3)
+        e = _entry(case["op"], case["name"], work["bytes"] if by_bytes else work["flops"], 1e9 if by_bytes else 1e12,
+                   "GB/s" if by_bytes else "TFLOP/s", ms, ms, peaks["hbm_gbs" if by_bytes else "bf16_tflops"], peaks["note"], "none", 1)
+        e["floor_ms"] = e["ms"] * e["frac_of_peak"]
+        out.append(e)
+        del sets, graph
+        torch.cuda.empty_cache()
+    return out
+
+
 def run_all(dev, rank, world, peaks):
     out = []
     plain_fp8 = None
@@ -394,6 +424,7 @@ SMALL = {      # reduced shapes for profiler captures: inputs above the 126 MB L
     "mla_decode": dict(batch=32),
     "mla_decode_bf16": dict(batch=32),
     "small_ops": dict(rows=2048),
+    "operators": dict(most_bytes=200_000_000),
     "tile_program": dict(rows=2048),
 }
 
