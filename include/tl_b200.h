@@ -287,8 +287,9 @@ int tl_b200_mla_decode_paged_noalloc(const void* q, const void* kv_cache, const 
  *   format TL_E4M3: heads 1; k [tokens, dim], cache [num_pages, page_size, dim] e4m3, scale [num_pages, page_size]
  *     fp32: s = max(amax |x|, 1e-4) / 448, byte = e4m3(x / s), value = s * byte.  dim a multiple of 8, at most 1024;
  *     `group` is ignored.  The cache of tl_b200_mla_decode_paged.
- * A group (row) with a NaN or an infinity, or one whose max - min exceeds fp32, reads back as NaN.  v, v_cache, v_scale: the values, in the same launch
- * (all three NULL: only k).  Rows and caches 16-byte aligned, strides a multiple of 8 elements; dtype TL_BF16 or
+ * A group (row) with a NaN or an infinity, or one whose max - min exceeds fp32, reads back as NaN.  A value is rounded to the
+ * 16-bit type when it is read back, so a group within a step of that type's largest number may read back an infinity there.
+ * v, v_cache, v_scale: the values, in the same launch (all three NULL: only k).  Rows and caches 16-byte aligned, strides a multiple of 8 elements; dtype TL_BF16 or
  * TL_F16.  (The reference quantises per token and per block on the host side of its FP8 examples,
  * examples/deepseek_deepgemm/example_deepgemm_fp8_2xAcc.py:93-112; it has no cache writer.)                       */
 int tl_b200_kv_cache_write(const int64_t* slots, const void* k, void* k_cache, void* k_scale, const void* v, void* v_cache,

@@ -5,8 +5,9 @@
 //
 // What bounds it.  A key of one kv head is dim/2 + 4 groups bytes, twice with its value (136 bytes at dim 128 and one
 // group), against 4 dim flop for each of the few query heads that share it: HBM, if the codes can be widened fast enough.
-// At the measured copy rate an SM receives 43 codes a clock, so every instruction spent on eight codes counts; a score
-// costs next to nothing beside that.
+// At the measured copy rate an SM receives 43 codes a clock, so every instruction spent on eight codes counts.  As it stands
+// neither memory nor any one unit is full: a warp's steps depend on one another, and the registers and the rings leave four
+// warps a scheduler to hide that (figures below).
 //
 // Layout.  The MMAs are the warp-level m16n8k16 ones: at most 8 or 16 query rows share a key, so a 128-row tensor-memory
 // tile would be 90% padding, and codes have to pass through registers to be widened anyway.  Keys (and columns of V) are
@@ -25,7 +26,7 @@
 //     hundreds of times the output of a long sequence and carry the tensor core's truncation into it (error against 64 bits,
 //     60 sequences of 100000 tokens, fp16: 2.6e-4 of the output, of which 2.1e-4 is its own rounding; 1.1e-3 without, 4.7e-4
 //     with 8 times the sum of the weights taken off at the end; bf16 1.68e-3, all of it rounding, and up to 2.3e-3 without).
-//     It costs 5%: 64 sequences of 2048 to 12288 tokens 108.6 and 114 us.
+//     It cost 5% when it was made: 64 sequences of 2048 to 12288 tokens 108.6 and 114 us.
 // Every group of columns has its own MMAs, so a group's step can multiply the score or the weight.
 //
 // Work.  Sequences are cut into units of 128 tokens; the list of all (sequence, kv head, query tile, unit) is dealt out in
@@ -38,10 +39,13 @@
 // last adds them up in their fixed order, so the result does not depend on who that is.
 //
 // Measured (bf16, dim 128, one group, 32 query and 8 kv heads, at a copy rate of 6.55 TB/s): 64 sequences of 2048 to 12288
-// tokens 114 us, 4.4 TB/s of cache; one of 131077 tokens 52 us, 2.9 TB/s; one of 777 tokens 9.0 us.  A round of 32 tokens
-// issues some 350 instructions a warp, and issue slots are what the long loop is bound by; about 15 us of a call are the
-// first loads, the joins and the launch.  Each integer or IEEE division between segments is felt: without those by run-time
-// sizes 200 sequences of 40 to 300 tokens took 32.4 us instead of 36.4 us.
+// tokens 115.5 us, 4.3 TB/s of cache; one of 131077 tokens (groups of 64) 52 us, 2.9 TB/s; one of 777 tokens 9.0 us.  Counters of
+// 32 sequences of 8192: 662 instructions a round of 32 tokens, all told; while an SM is busy its issue slots are 61% taken and the
+// integer pipe 53%, memory 45%; in 39% of the cycles none of a scheduler's four warps can issue.  A warp's 6.6 cycles an
+// instruction are 1.3 waiting for its turn, 1.3 for results of fixed latency, 1.0 for a busy pipe, 0.5 for shared memory and
+// shuffles, hardly any for global loads.  Launch, first loads and joins take 15% of that call.  Each integer or IEEE
+// division between segments is felt: without those by run-time sizes 200 sequences of 40 to 300 tokens took 32.4 us instead
+// of 36.4 us, in an earlier form.
 #include "sm100.cuh"
 #include "mla_common.cuh"
 
@@ -68,8 +72,8 @@ struct AttnInt4Params {
 
 constexpr int kWarps = 4, kHalf = 16 * kWarps, kUnit = 2 * kHalf;      // a warp's two tiles of a unit lie kHalf tokens apart
 
-// Teams per SM, by the registers a thread needs: 128 (four teams), 168 with four groups' steps and sums (32 x 4096 tokens:
-// 59 us, 73 us with four teams that spill), 255 with twice the accumulators (24 sequences of 4 tokens, dim 64, in an earlier form: 39 us, 42 us).
+// Teams per SM, by the registers a thread needs: 128 (four teams), 168 with four groups' steps and sums (32 x 4096 tokens, in an
+// earlier form: 59 us, 73 us with four teams that spill), 255 with twice the accumulators (24 sequences of 4 tokens, dim 64, likewise: 39 us, 42 us).
 __host__ __device__ constexpr int i4_teams(int dim, int groups, int nt) {
   return nt == 2 || dim == 256 ? 2 : dim == 128 && groups == 4 ? 3 : 4;
 }
@@ -1001,7 +1005,8 @@ template <typename T, int DIM, int GROUP, int NT>
 static int launch_i4(const AttnInt4Params& p, int grid, cudaStream_t s) {
   // Four small teams to an SM are one CTA: the schedulers favour the oldest warps, and as CTAs of their own the teams end at 80,
   // 92, 105 and 118 us (64 sequences of 2048 to 12288 tokens: 112.7 us; 107.8 us as one CTA, whose teams have a warp of every
-  // age; 32 x 4096 tokens 44.8 and 44.0 us, one sequence of 131077 49.2 and 49.7 us).  Two and three teams an SM:
+  // age; 32 x 4096 tokens 44.8 and 44.0 us, one sequence of 131077 49.2 and 49.7 us; all before V's codes were taken about zero, like
+  // what follows).  Two and three teams an SM:
   // 47.6 us as CTAs and 49.5 us as one (16 x 4096 tokens, dim 256), 60.5 and 63.4 us (32 x 4096, 16 rows).
   using Cfg = I4Cfg<DIM, GROUP, NT>;
   constexpr int teams = Cfg::kTeams == 4 ? 4 : 1, smem = teams * Cfg::kSmem;

@@ -589,8 +589,9 @@ _int4_workspaces: dict = {}
 
 def _int4_workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """Scratch of attn_decode_paged_int4, kept apart from the other operators': its counters have to be zero between calls.
-    One buffer per (device, stream), as in _workspace; a call that is being captured gets one of its own from the graph's
-    pool, so that two graphs never share counters, however their replays overlap."""
+    One buffer per (device, stream), as in _workspace.  A call that is being captured gets one of its own from the graph's
+    pool, with a fill of the counters that every replay repeats: graphs with pools of their own share nothing, however their
+    replays overlap.  Graphs captured into one pool share its memory, and must not run at the same time, as torch asks of them."""
     if torch.cuda.is_current_stream_capturing():
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
         buf[:N.ATTN_INT4_ZERO_BYTES].zero_()
